@@ -74,6 +74,16 @@ SIGNATURES = {
     "gptoss_kv_pages_copy": (ctypes.c_int, [_P, _P, _I32, _I32, _P, _I32, _I32, _I64, _I64, _P, _P, _I32, _P]),
     "gptoss_attn_merge": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P]),
     "gptoss_attn_sink_rescale": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P]),
+    "gptoss_attn_chunk_workspace_bytes": (_I64, []),
+    "gptoss_attn_chunk": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I32, _I64, _P, _I32, _I32, _P, _P, _P, _I32, _I64,
+                                         _I32, _I32, _I32, _I32, _I32, _F, _P, _P, _I64, _P, _P, _P]),
+    "gptoss_qkv_rope_append_f8": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _F, _P, _P, _P, _P, _P,
+                                                 _P]),
+    "gptoss_kv_pages_copy_f8": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _P, _I32, _I32, _I64, _I64, _P, _P,
+                                               _I32, _P]),
+    "gptoss_verify_drafts_scratch_bytes": (_I64, [_I64]),
+    "gptoss_verify_drafts": (ctypes.c_int, [_P, _I32, _I64, _P, _P, _I64, _I32, _I32, ctypes.c_double, _P, _P, _P,
+                                            _I64, _P, _I64, _P, _P, _P]),
     "gptoss_moe_plan_tiles": (ctypes.c_int, [_P, _I32, _P, _P, _P]),
     "gptoss_moe_segment_copy": (ctypes.c_int, [_P, _P, _P, _I32, _I32, _I64, _I32, _P, _P]),
     "gptoss_stream_set_flag": (ctypes.c_int, [_P, ctypes.c_uint32, _P]),

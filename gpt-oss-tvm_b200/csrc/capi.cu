@@ -9,6 +9,7 @@
 
 #include "../../include/gptoss_b200.h"
 #include "common.cuh"
+#include "chunk.cuh"
 
 #include "launch.h"
 
@@ -524,6 +525,126 @@ int gptoss_attn_sink_rescale(uint16_t* o, const float* lse, const uint16_t* sink
                              void* stream) {
   if (T < 0 || Hq <= 0 || D <= 0) return fail(-1, "gptoss_attn_sink_rescale: bad shape");
   return check_launch(launch_sink_rescale(o, lse, sinks, T, Hq, D, GPTOSS_STREAM(stream)), "sink_rescale");
+}
+
+// ------------------------------------------- chunks over the paged cache --
+int64_t gptoss_attn_chunk_workspace_bytes(void) { return chunk_workspace_bytes(); }
+
+int gptoss_attn_chunk(const uint16_t* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                      const uint8_t* k_codes, const uint8_t* v_codes, int32_t kv_f8, int64_t num_pages,
+                      const int32_t* page_table, int32_t table_rows, int32_t table_stride, const int32_t* seq_rows,
+                      const int32_t* q_start, const int32_t* kv_len, int32_t N, int64_t T, int32_t max_q, int32_t Hq,
+                      int32_t Hkv, int32_t D, int32_t window, float sm_scale, const uint16_t* sinks, void* workspace,
+                      int64_t workspace_bytes, uint16_t* o, float* lse, void* stream) {
+  if (D != 64) return fail(-1, "gptoss_attn_chunk: head_dim must be 64");
+  if (N < 0 || N > kChunkMaxSeqs || T < 0 || T >= (1ll << 31) || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > 64)
+    return fail(-1, "gptoss_attn_chunk: bad shape N=%d T=%lld Hq=%d Hkv=%d (0..%d chunks, Hq a multiple of Hkv, at "
+                    "most 64 query heads per kv head)", N, (long long)T, Hq, Hkv, kChunkMaxSeqs);
+  if (N == 0 || T == 0) return 0;
+  if (!q || !k_pages || !v_pages || !page_table || !seq_rows || !q_start || !kv_len || !workspace || !o)
+    return fail(-1, "gptoss_attn_chunk: null pointer");
+  if (kv_f8 && (!k_codes || !v_codes)) return fail(-1, "gptoss_attn_chunk: 8-bit pages need their codes");
+  if (table_rows <= 0 || table_stride <= 0 || num_pages <= 0 || num_pages >= (1ll << 27))
+    return fail(-1, "gptoss_attn_chunk: bad page table (%d x %d) or pool (%lld pages, below 2^27)", table_rows,
+                table_stride, (long long)num_pages);
+  if (max_q <= 0) return fail(-1, "gptoss_attn_chunk: max_q must be positive");
+  if (!(sm_scale == sm_scale)) return fail(-1, "gptoss_attn_chunk: sm_scale is NaN");
+  if (((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15) || ((uintptr_t)o & 15) ||
+      ((uintptr_t)workspace & 15) || (kv_f8 && (((uintptr_t)k_codes & 15) || ((uintptr_t)v_codes & 15))))
+    return fail(-1, "gptoss_attn_chunk: q, the pools, the codes, the workspace and o must be 16-byte aligned");
+  if (q_stride < (int64_t)Hq * D || q_stride % 8)
+    return fail(-1, "gptoss_attn_chunk: q_stride must be a multiple of 8 elements, at least Hq * D");
+  if (workspace_bytes < chunk_workspace_bytes())
+    return fail(-1, "gptoss_attn_chunk: workspace smaller than gptoss_attn_chunk_workspace_bytes()");
+  ChunkParams p = {};
+  p.q = q;
+  p.q_stride = q_stride;
+  p.k_code = k_codes;
+  p.v_code = v_codes;
+  p.pool_pages = num_pages;
+  p.table = page_table;
+  p.table_rows = table_rows;
+  p.tstride = table_stride;
+  p.seq_rows = seq_rows;
+  p.q_start = q_start;
+  p.kv_len = kv_len;
+  p.N = N;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  p.window = window > 0 ? window : 0;
+  p.T = T;
+  p.scale2 = sm_scale * 1.4426950408889634f;
+  p.sinks = sinks;
+  p.o = o;
+  p.lse = lse;
+  return check_launch(launch_attn_chunk(p, k_pages, v_pages, kv_f8, max_q, workspace, GPTOSS_STREAM(stream)),
+                      "attn_chunk");
+}
+
+int gptoss_qkv_rope_append_f8(const uint16_t* qkv, const int32_t* positions, const int32_t* slots, int64_t S,
+                              int64_t num_pages, int32_t Hq, int32_t Hkv, int32_t D, const float* inv_freq,
+                              float concentration, uint16_t* q_out, uint8_t* k_pages, uint8_t* v_pages,
+                              uint8_t* k_codes, uint8_t* v_codes, void* stream) {
+  if (D != 64) return fail(-1, "gptoss_qkv_rope_append_f8: head_dim must be 64");
+  if (S < 0 || S >= (1ll << 31) || Hq <= 0 || Hkv <= 0 || num_pages < 0)
+    return fail(-1, "gptoss_qkv_rope_append_f8: bad shape");
+  if (S == 0) return 0;
+  if (!qkv || !positions || !inv_freq || !q_out || !k_pages || !v_pages || !k_codes || !v_codes)
+    return fail(-1, "gptoss_qkv_rope_append_f8: null pointer");
+  if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15))
+    return fail(-1, "gptoss_qkv_rope_append_f8: qkv, q_out and the pools must be 16-byte aligned");
+  return check_launch(launch_qkv_rope_append_f8(qkv, positions, slots, S, num_pages * 16, Hq, Hkv, inv_freq,
+                                                concentration, q_out, k_pages, v_pages, k_codes, v_codes,
+                                                GPTOSS_STREAM(stream)),
+                      "qkv_rope_append_f8");
+}
+
+int gptoss_kv_pages_copy_f8(uint8_t* k_pages, uint8_t* v_pages, uint8_t* k_codes, uint8_t* v_codes, int64_t num_pages,
+                            int32_t Hkv, int32_t D, const int32_t* page_table, int32_t table_stride, int32_t seq,
+                            int64_t pos0, int64_t n, uint16_t* k_rows, uint16_t* v_rows, int32_t to_pages,
+                            void* stream) {
+  if (D != 64) return fail(-1, "gptoss_kv_pages_copy_f8: head_dim must be 64");
+  if (n < 0 || pos0 < 0 || seq < 0 || Hkv <= 0 || table_stride <= 0 || num_pages < 0)
+    return fail(-1, "gptoss_kv_pages_copy_f8: bad arguments");
+  if (n == 0) return 0;
+  if (!page_table || !k_pages || !v_pages || !k_codes || !v_codes || !k_rows || !v_rows)
+    return fail(-1, "gptoss_kv_pages_copy_f8: null pointer");
+  if (((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15) || ((uintptr_t)k_rows & 15) || ((uintptr_t)v_rows & 15))
+    return fail(-1, "gptoss_kv_pages_copy_f8: the pools and the rows must be 16-byte aligned");
+  if (to_pages && n > (int64_t)table_stride * 16)
+    return fail(-1, "gptoss_kv_pages_copy_f8: %lld rows do not fit the %d pages of the table row (two rows of the "
+                    "call would share a pool row)", (long long)n, table_stride);
+  return check_launch(launch_kv_pages_f8(k_pages, v_pages, k_codes, v_codes, num_pages * 16,
+                                         page_table + (int64_t)seq * table_stride, table_stride, pos0, n, Hkv, k_rows,
+                                         v_rows, to_pages, GPTOSS_STREAM(stream)),
+                      "kv_pages_copy_f8");
+}
+
+int64_t gptoss_verify_drafts_scratch_bytes(int64_t T) { return T > 0 ? verify_scratch_bytes(T) : 64; }
+
+int gptoss_verify_drafts(const void* logits, int32_t logits_bf16, int64_t ld_logits, const int32_t* tokens,
+                         const int32_t* row_start, int64_t T, int32_t N, int32_t V, double temperature,
+                         const float* accept_u, const float* next_u, const float* draft_probs, int64_t ld_draft,
+                         void* scratch, int64_t scratch_bytes, int32_t* accepted, int32_t* next_tokens,
+                         void* stream) {
+  if (T < 0 || T >= (1ll << 27) || N < 0 || N >= (1 << 27) || V <= 0 || V > (1 << 22))
+    return fail(-1, "gptoss_verify_drafts: bad shape T=%lld N=%d V=%d (V at most 2^22)", (long long)T, N, V);
+  if (!(temperature >= 0.0) || std::isinf(temperature))
+    return fail(-1, "gptoss_verify_drafts: temperature must be finite and not negative");
+  if (N == 0) return 0;
+  if (!row_start || !accepted || !next_tokens || (T > 0 && (!logits || !tokens || !scratch)))
+    return fail(-1, "gptoss_verify_drafts: null pointer");
+  if (temperature >= 1e-6 && T > 0 && (!accept_u || !next_u))
+    return fail(-1, "gptoss_verify_drafts: random numbers are required above temperature 0");
+  if (ld_logits < V || (draft_probs && ld_draft < V))
+    return fail(-1, "gptoss_verify_drafts: a row stride is smaller than V");
+  if (scratch_bytes < gptoss_verify_drafts_scratch_bytes(T))
+    return fail(-1, "gptoss_verify_drafts: scratch smaller than gptoss_verify_drafts_scratch_bytes()");
+  return check_launch(launch_verify(logits, logits_bf16, ld_logits, tokens, row_start, T, N, V, temperature, accept_u,
+                                    next_u, draft_probs, ld_draft, scratch, accepted, next_tokens,
+                                    GPTOSS_STREAM(stream)),
+                      "verify_drafts");
 }
 
 int gptoss_dense_gemv_max_tokens(void) { return dense_gemv_max_tokens(); }

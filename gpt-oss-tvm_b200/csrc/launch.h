@@ -160,6 +160,26 @@ int launch_attn_merge(const uint16_t* o1, const float* l1, const uint16_t* o2, c
 int launch_sink_rescale(uint16_t* o, const float* lse, const uint16_t* sinks, int64_t T, int32_t Hq, int32_t D,
                         cudaStream_t s);
 
+// chunk.cu: attention of the sequences' new tokens over the paged cache
+struct ChunkParams;
+int64_t chunk_workspace_bytes();
+int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, int32_t max_q, void* workspace,
+                      cudaStream_t s);
+// kv8.cu: the 8-bit cache
+int launch_qkv_rope_append_f8(const uint16_t* qkv, const int32_t* pos, const int32_t* slot, int64_t S,
+                              int64_t pool_rows, int32_t Hq, int32_t Hkv, const float* inv_freq, float conc,
+                              uint16_t* q_out, uint8_t* kp, uint8_t* vp, uint8_t* kcode, uint8_t* vcode,
+                              cudaStream_t s);
+int launch_kv_pages_f8(uint8_t* kp, uint8_t* vp, uint8_t* kcode, uint8_t* vcode, int64_t pool_rows,
+                       const int32_t* table, int32_t tstride, int64_t pos0, int64_t n, int32_t Hkv, uint16_t* kb,
+                       uint16_t* vb, int32_t to_pages, cudaStream_t s);
+// verify.cu: drafted tokens against the target's logits
+int64_t verify_scratch_bytes(int64_t T);
+int launch_verify(const void* logits, int32_t bf16, int64_t ld, const int32_t* tokens, const int32_t* row_start,
+                  int64_t T, int32_t N, int32_t V, double temperature, const float* accept_u, const float* next_u,
+                  const float* draft, int64_t ld_draft, void* scratch, int32_t* accepted, int32_t* next,
+                  cudaStream_t s);
+
 // capi.cu: the expert part of the MoE block (gather or quantize, both grouped
 // GEMMs) on the path the sizes and GPTOSS_MOE_MX select; shared by the
 // workspace and the no-allocation forwards

@@ -242,6 +242,56 @@ int gptoss_kv_pages_copy(uint16_t* k_pages, uint16_t* v_pages, int32_t Hkv, int3
                          int32_t table_stride, int32_t seq, int64_t pos0, int64_t n, uint16_t* k_rows,
                          uint16_t* v_rows, int32_t to_pages, void* stream);
 
+/* Attention of the new tokens of N sequences over the paged cache, in one call
+ * (no counterpart in the reference, whose extend takes one sequence).  Chunk b
+ * is tokens q_start[b] .. q_start[b + 1] - 1 of q ([T, Hq, D] bf16, q_stride
+ * elements between tokens); its keys and values, the chunk's own included, are
+ * already in the pages of row seq_rows[b] of page_table ([table_rows,
+ * table_stride] int32; the row formula above, so a ring works when it still
+ * holds window + chunk - 1 keys), and the chunk is the last of kv_len[b]
+ * positions.  Token i sees key j iff 0 <= j <= pos_i and, with window W > 0,
+ * j > pos_i - W; one that sees nothing (kv_len[b] smaller than its chunk, or a
+ * seq_rows[b] outside the table) gives o = 0 and lse = -inf.  What pages hold
+ * beyond the visible keys does not matter, NaN included.
+ * Pages: bf16, or with kv_f8 e4m3 values and codes as gptoss_qkv_rope_append_f8
+ * writes them; num_pages pages in each pool.  max_q: the longest chunk, known
+ * to the host (it picks the kernel; a longer chunk is still computed right).
+ * sinks [Hq] bf16 or NULL: exp(sink) joins the softmax denominator, in fp32
+ * before the one rounding of o [T, Hq, D].  lse [T, Hq] fp32 or NULL, as above.
+ * q_start, kv_len, seq_rows: device memory, so a CUDA graph may replay the call
+ * with other lengths.  workspace: gptoss_attn_chunk_workspace_bytes() bytes of
+ * device memory, zeroed once before its first use and used by one stream at a
+ * time; word 0 collects device errors (a bounded wait that ran out: zero the
+ * workspace again after one). */
+int64_t gptoss_attn_chunk_workspace_bytes(void);
+int gptoss_attn_chunk(const uint16_t* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                      const uint8_t* k_codes, const uint8_t* v_codes, int32_t kv_f8, int64_t num_pages,
+                      const int32_t* page_table, int32_t table_rows, int32_t table_stride, const int32_t* seq_rows,
+                      const int32_t* q_start, const int32_t* kv_len, int32_t N, int64_t T, int32_t max_q, int32_t Hq,
+                      int32_t Hkv, int32_t D, int32_t window, float sm_scale, const uint16_t* sinks, void* workspace,
+                      int64_t workspace_bytes, uint16_t* o, float* lse, void* stream);
+
+/* The 8-bit cache (no counterpart in the reference).  A pool holds e4m3 values
+ * [num_pages * 16, Hkv, 64] and one E8M0 code per row and head, [num_pages,
+ * Hkv, 16].  For a head row with largest magnitude a: e = the smallest integer
+ * in -60..60 with a <= 448 * 2^e, code = e + 127, value = e4m3(x * 2^-e) to the
+ * nearest, ties to even, at most 448 in magnitude.  value * 2^e is exact in
+ * bf16.  A row with a NaN has code 255 and reads back as NaN; magnitudes beyond
+ * 448 * 2^60 saturate.
+ * gptoss_qkv_rope_append_f8: gptoss_qkv_rope_append whose keys (rotated, and
+ * rounded to bf16 as there) and values are quantised into such pools; a slot
+ * outside the pool is not written.  The same q_out, bit for bit.
+ * gptoss_kv_pages_copy_f8: gptoss_kv_pages_copy between bf16 rows and such
+ * pages, quantising (to_pages, at most 16 * table_stride rows) or reading back. */
+int gptoss_qkv_rope_append_f8(const uint16_t* qkv, const int32_t* positions, const int32_t* slots, int64_t S,
+                              int64_t num_pages, int32_t Hq, int32_t Hkv, int32_t D, const float* inv_freq,
+                              float concentration, uint16_t* q_out, uint8_t* k_pages, uint8_t* v_pages,
+                              uint8_t* k_codes, uint8_t* v_codes, void* stream);
+int gptoss_kv_pages_copy_f8(uint8_t* k_pages, uint8_t* v_pages, uint8_t* k_codes, uint8_t* v_codes, int64_t num_pages,
+                            int32_t Hkv, int32_t D, const int32_t* page_table, int32_t table_stride, int32_t seq,
+                            int64_t pos0, int64_t n, uint16_t* k_rows, uint16_t* v_rows, int32_t to_pages,
+                            void* stream);
+
 /* merge_attn_output_inplace (model/attention.py:231-233): two partial
  * attention states over disjoint keys -> one (o bf16 [T, Hq, D], lse). */
 int gptoss_attn_merge(const uint16_t* o1, const float* lse1, const uint16_t* o2, const float* lse2, int64_t T,
@@ -288,6 +338,32 @@ int64_t gptoss_sample_top_p_scratch_bytes(int64_t B, int64_t V);
 int gptoss_sample_top_p_from_logits(const float* logits, int64_t B, int64_t V, double temperature, double top_p,
                                     const double* uniform, double uniform0, void* scratch, int64_t scratch_bytes,
                                     int32_t* tokens, void* stream);
+
+/* Speculative decoding's test of drafted tokens against the target's logits,
+ * from given random numbers (no counterpart in the reference).  Rows
+ * row_start[b] .. row_start[b + 1] - 1 of logits ([T, V] fp32, or bf16 with
+ * logits_bf16; ld_logits elements between rows) are sequence b's: row r is the
+ * target's for the token that follows tokens[r], and tokens[r + 1] is the draft
+ * it is checked against (the last row of a sequence has none).  With p =
+ * softmax(logits / temperature), its weights held as whole multiples of 2^-40
+ * of the largest so that no sum depends on its order, and q = row r of
+ * draft_probs ([T, V] fp32, the distribution tokens[r + 1] was drawn from; NULL:
+ * drafts that were looked up, q = 1):
+ *   draft accepted  iff accept_u[r] * q(x) < p(x)
+ *   accepted[b]     the number of drafts before the first that is not
+ *   next_tokens[b]  the token after them: drawn with next_u[b] from
+ *                   max(p - q, 0) at that row (p without x when q is NULL, p
+ *                   where nothing is left), or from p of the last row.
+ * temperature < 1e-6: a draft is accepted iff it is the argmax (lowest index),
+ * and the next token is the argmax; the random numbers may be NULL.  A NaN
+ * logit counts as -inf; a draft outside 0 .. V - 1 is not accepted; a sequence
+ * without rows gives 0 and -1.  All memory on the device; V at most 2^22. */
+int64_t gptoss_verify_drafts_scratch_bytes(int64_t T);
+int gptoss_verify_drafts(const void* logits, int32_t logits_bf16, int64_t ld_logits, const int32_t* tokens,
+                         const int32_t* row_start, int64_t T, int32_t N, int32_t V, double temperature,
+                         const float* accept_u, const float* next_u, const float* draft_probs, int64_t ld_draft,
+                         void* scratch, int64_t scratch_bytes, int32_t* accepted, int32_t* next_tokens,
+                         void* stream);
 
 /* The routing half of gptoss_moe_forward for M normalised tokens t (the
  * output of gptoss_rms_norm): router logits, top-k + softmax and the
