@@ -548,7 +548,7 @@ int gptoss_attn_chunk(const uint16_t* q, int64_t q_stride, const void* k_pages, 
     return fail(-1, "gptoss_attn_chunk: bad page table (%d x %d) or pool (%lld pages, below 2^27)", table_rows,
                 table_stride, (long long)num_pages);
   if (max_q <= 0) return fail(-1, "gptoss_attn_chunk: max_q must be positive");
-  if (!(sm_scale == sm_scale)) return fail(-1, "gptoss_attn_chunk: sm_scale is NaN");
+  if (!(sm_scale > 0.f) || std::isinf(sm_scale)) return fail(-1, "gptoss_attn_chunk: sm_scale must be positive");
   if (((uintptr_t)q & 15) || ((uintptr_t)k_pages & 15) || ((uintptr_t)v_pages & 15) || ((uintptr_t)o & 15) ||
       ((uintptr_t)workspace & 15) || (kv_f8 && (((uintptr_t)k_codes & 15) || ((uintptr_t)v_codes & 15))))
     return fail(-1, "gptoss_attn_chunk: q, the pools, the codes, the workspace and o must be 16-byte aligned");

@@ -8,12 +8,16 @@
 //   l_i  = sum_j 2^(s2_ij - m_i),  lse_i = m_i + log2(l_i),  s2 = s * log2(e);
 //   a token that sees nothing gets o = 0 and lse = -inf.
 //
-// chunk_rows_kernel   up to 64 rows (tokens x heads of a kv head): one pass
-//                     over the keys, bound by their bytes
+// chunk_keys_kernel   up to 64 rows (tokens x heads of a kv head) against a
+//                     line of keys: S^T = K Q^T and O^T = V^T P^T on tcgen05
+//                     with the keys on the 128-row side
+// chunk_rows_kernel   longer chunks: 256 rows against the keys, S = Q K^T and
+//                     O = P V with the rows on the 128-row side
 //
 // The output is rounded once, from fp32; P is rounded to bf16 as the operand
 // of P V (its relative error of 2^-9 an element is the size of the output's
-// own rounding), the sum l takes the unrounded values.
+// own rounding; 8-bit pages split it into two e4m3 terms, with less error), the
+// sum l takes the unrounded values.
 #include "chunk.cuh"
 #include "launch.h"
 
@@ -23,25 +27,6 @@ namespace {
 
 constexpr float kChLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ void ch_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ch_ldsm(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ch_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
 __device__ __forceinline__ uint32_t ch_bf16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -52,16 +37,57 @@ __device__ __forceinline__ float ch_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 128-byte rows, 16-byte piece c of row r (the 128-byte TMA swizzle)
-__device__ __forceinline__ uint32_t ch_swz128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
-// 64-byte rows (the 64-byte TMA swizzle)
-__device__ __forceinline__ uint32_t ch_swz64(int r, int c) { return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); }
-// bytes (b0, b2) and (b1, b3) of w, e4m3, as bf16 pairs that read 2^-120 of their value
-__device__ __forceinline__ uint32_t ch_e4m3_even(uint32_t w) { return ((w << 4) & 0x07F007F0u) | ((w << 8) & 0x80008000u); }
-__device__ __forceinline__ uint32_t ch_e4m3_odd(uint32_t w) { return ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u); }
-// 2^(code - 127 + bias) as fp32, NaN for code 255 (a row that held a NaN)
-__device__ __forceinline__ float ch_code_scale(uint32_t code, int bias) {
-  return code == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float((uint32_t)((int)code + bias) << 23);
+// lo -> byte 0, hi -> byte 1; saturates, NaN stays NaN
+__device__ __forceinline__ uint32_t ch_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// x rounded to 4 significant bits (half away from zero), exact in e4m3 for 2^-6 <= |x| <= 448
+__device__ __forceinline__ float ch_round4(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x80000u) & 0xFFF00000u);
+}
+// Four e4m3 bytes as two bf16 pairs (b0, b1), (b2, b3) times 2^e, exactly: the
+// bits moved into a bf16 read 2^-120 of the value, then come 2^60 and `mul`
+// (ch_code_mul: 2^(e + 60), NaN for the code of a row that held one).
+__device__ __forceinline__ void ch_e4m3_to_bf16(uint32_t w, uint32_t mul, uint32_t& p01, uint32_t& p23) {
+  const uint32_t ev = ((w << 4) & 0x07F007F0u) | ((w << 8) & 0x80008000u);  // (b0, b2)
+  const uint32_t od = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);         // (b1, b3)
+  const uint32_t e2 = bf16x2_mul(bf16x2_mul(ev, 0x5D805D80u), mul), o2 = bf16x2_mul(bf16x2_mul(od, 0x5D805D80u), mul);
+  p01 = prmt(e2, o2, 0x5410u);
+  p23 = prmt(e2, o2, 0x7632u);
+}
+__device__ __forceinline__ uint32_t ch_code_mul(uint32_t code) {
+  const uint32_t h = code == 255u ? 0x7FC0u : ((min(code, 194u) + 60u) << 7);
+  return h | (h << 16);
+}
+// Two fp32 at a time.
+typedef unsigned long long ch_f2;
+__device__ __forceinline__ ch_f2 ch_pair(float a, float b) {
+  return ((ch_f2)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ float ch_lo(ch_f2 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float ch_hi(ch_f2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ ch_f2 ch_fma2(ch_f2 a, ch_f2 b, ch_f2 c) {
+  ch_f2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ ch_f2 ch_add2(ch_f2 a, ch_f2 b) {
+  ch_f2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ ch_f2 ch_mul2(ch_f2 a, ch_f2 b) {
+  ch_f2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Largest of the warp's values (a NaN counts as the smallest).
+__device__ __forceinline__ float ch_warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 __device__ __forceinline__ void ch_named_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
@@ -78,417 +104,1180 @@ __device__ __forceinline__ bool ch_named_or(int id, int n, bool v) {
       : "memory");
   return r != 0;
 }
-// Untiled 16-byte-granular copy, completion as tx bytes.
-__device__ __forceinline__ void ch_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+__device__ __forceinline__ void ch_tma_4d(void* dst, const void* tmap, int32_t z, int32_t w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4}], "
+      "[%5];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(0), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]: bf16, or e4m3 (kind::f8f6f4).
+template <bool F8>
+__device__ __forceinline__ void ch_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (!F8) {
+    tc_mma_ss(d, a, b, idesc, accumulate);
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// Shared-memory matrix descriptor: 8-row groups `group` bytes apart; rows of
+// 128 bytes with the 128-byte swizzle, or of 64 with the 64-byte one.
+__device__ __forceinline__ uint64_t ch_sdesc(uint32_t addr, uint32_t group, bool sw64) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(group >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)(sw64 ? 4 : 2) << 61);
+}
+// 8 or 16 consecutive 32-bit columns of this warp's 32 lanes, no wait.
+__device__ __forceinline__ void ch_ld8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void ch_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
 
-// ------------------------------------------------------------- few rows --
-// CTA = 4 compute warps and one that loads.  Key tiles of 64 keys (4 pages) go
-// through a ring of stages by TMA, one box of 16 keys x 64 values per page.
-// Per tile, warp w takes keys 16 w .. 16 w + 15 of Q K^T for all rows, and after
-// P went through shared memory, dims 16 w .. 16 w + 15 of P V over all 64 keys:
-// no fragment of K or V is loaded (or, in 8 bits, unpacked) twice.  The softmax
-// reference of a row moves only when a score exceeds it by 8 (P <= 2^8), which
-// one barrier that also carries the vote tells all warps.
-//
-// 8-bit pages: e4m3 bits shifted into a bf16 read 2^-120 of the value, so no
-// conversion is needed beyond two masks per pair; Q carries a factor 2^60, the
-// key's power of two and the remaining 2^60 meet the score in fp32, and V's go
-// to the column of P before it is rounded.  A key's code is one byte, applied
-// exactly.
-constexpr int kRowsKT = 64;
-constexpr int kRowsWarps = 4;
-constexpr int kRowsThreads = kRowsWarps * 32 + 32;
+// One row's value from its sum, maximum and unnormalised output.
+__device__ __forceinline__ float ch_norm(const ChunkParams& p, int h, float l, float m) {
+  float den = l;
+  if (p.sinks) den += exp2f(bf16_bits_to_f32(p.sinks[h]) * kChLog2e - m);
+  return l == 0.f ? 0.f : 1.0f / den;
+}
 
-template <bool F8, int RT>
-struct RowsCfg {
-  static constexpr int kRows = 16 * RT;
-  static constexpr int kStages = F8 ? 4 : 4;
+// The partial results of a unit, joined in the order of the keys: 16 threads
+// per row, 4 dims each, four parts' loads in flight.  `heads` kv heads of
+// `rows` rows each per slot.
+__device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg& sg, int heads, int rows, int tid,
+                                           int nthreads) {
+  const int c0 = sg.c0, c1 = sg.c1, s0 = sg.first_slot;
+  const int64_t rs = (int64_t)heads * rows;
+  for (int x = tid; x < heads * sg.nrows * 16; x += nthreads) {
+    const int hr = x >> 4, d = (x & 15) * 4;
+    const int hb = hr / sg.nrows, r = hr - hb * sg.nrows;
+    const int64_t at = (int64_t)hb * rows + r;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0; c <= c1; c += 4) {
+      float2 ml[4];
+      float4 y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int cc = min(c + k, c1);
+        const int64_t row = (cc == c0 ? s0 : 2 * cc) * rs + at;
+        ml[k] = __ldcg((const float2*)(p.part_ml + row * 2));
+        y[k] = __ldcg((const float4*)(p.part_o + row * kChunkD + d));
+      }
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mn = fmaxf(mn, ml[k].x);
+      const float me = mn == -INFINITY ? 0.f : mn, f0 = exp2f(m - me);
+      l *= f0;
+      a.x *= f0;
+      a.y *= f0;
+      a.z *= f0;
+      a.w *= f0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = c + k <= c1 ? exp2f(ml[k].x - me) : 0.f;
+        if (c + k > c1) break;
+        l += ml[k].y * f;
+        a.x += y[k].x * f;
+        a.y += y[k].y * f;
+        a.z += y[k].z * f;
+        a.w += y[k].w * f;
+      }
+      m = mn;
+    }
+    const int tk = r / p.G, h = (sg.hg * heads + hb) * p.G + r - tk * p.G;
+    const int64_t tok = sg.tok0 + tk;
+    if (p.lse && d == 0) p.lse[tok * p.Hq + h] = m + log2f(l);
+    const float inv = ch_norm(p, h, l, m);
+    *(uint2*)(p.o + (tok * p.Hq + h) * kChunkD + d) =
+        make_uint2(ch_bf16x2(a.x * inv, a.y * inv), ch_bf16x2(a.z * inv, a.w * inv));
+  }
+}
+
+// ---------------------------------------------------------- keys on M --
+// CTA = two streams of 4 softmax warps (a kv head each), one warp that loads
+// and one that issues the products.  A tile is 128 keys of both heads (8
+// pages); one TMA box brings a page's keys of both, in groups of 8 rows of 128
+// bytes (bf16: a head's, 8-bit: both heads' side by side), so that a head's 128
+// keys are one matrix operand with an even stride.  K and V have a loading
+// warp each: the copy engine takes 2 KB in about 97 cycles from two issuers,
+// 135 from one.  Per tile and stream:
+//   S^T [128 keys x W] = K Q^T    A = the K tile as it lies, B = Q, in TMEM
+//   a thread owns a key: its W scores are registers, the key's mask, scale
+//     and V exponent are its own constants
+//   O^T [64 dims x W] += V^T P^T  A = the V tile read dims-major, B = P^T,
+//     which the threads wrote to shared memory row by key
+// With the keys on the 128-row side nothing is padded to 128 queries: 8 rows
+// (one token's group of heads) cost W = 16 columns.  (An mma.sync form of this
+// kernel, rows on M, ran 32 x 5 tokens over 8191 8-bit keys in 317 us: legacy
+// mma.sync reaches 1009 multiply-adds per cycle and SM here, a quarter of
+// tcgen05's, and each 8-bit value had to be widened.)
+//
+// 8-bit pages are operands as they are (kind::f8f6f4).  The other side is then
+// e4m3 too, as two terms in columns of their own, W = 2 N: Q is scaled by a
+// power of two per unit and head, hi = Q to 4 significant bits, lo = 16 times
+// the rest (S = hi + lo / 16, 2^-22 of the largest); P likewise (2^-16 of the
+// row's largest).  The key's power of two meets the
+// score in fp32; the value's goes into the exponent, t = s + e_v, and the
+// softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
+//
+// The reference m of a row moves only when a score exceeds it by 8 (8-bit:
+// when P would pass 448), which one barrier of the stream's warps tells; then
+// O^T in TMEM is rescaled.
+constexpr int kKeysKT = 128;
+constexpr int kKeysThreads = 12 * 32;
+
+template <bool F8, int N_>
+struct KeysCfg {
+  static constexpr int N = N_;                            // rows of a unit
+  static constexpr int W = F8 ? 2 * N : N;                // columns of S^T and O^T
   static constexpr int kRowBytes = F8 ? 64 : 128;
-  static constexpr int kTile = kRowsKT * kRowBytes;           // K or V of one stage
-  static constexpr int kCodes = F8 ? 2 * kRowsKT : 0;         // K and V codes of one stage
-  static constexpr int kStageBytes = 2 * kTile;
-  static constexpr int kOffCodes = kStages * kStageBytes;
-  static constexpr int kOffP = kOffCodes + kStages * kCodes;  // P [rows][64] bf16
-  static constexpr int kOffRed = kOffP + kRows * 128;         // [4][rows] floats
-  static constexpr int kOffPre = kOffRed + kRowsWarps * kRows * 4;
-  static constexpr int kOffBar = kOffPre + (kChunkMaxSeqs + 1 + 7) / 8 * 64;
-  static constexpr int kAlloc = kOffBar + 2 * kStages * 8 + 16 + 1024;
+  static constexpr int kSide = 2 * kKeysKT * kRowBytes;   // K or V of a tile, two heads
+  static constexpr int kCodes = F8 ? 2 * 2 * kKeysKT : 0;  // [K, V][head][128]
+  static constexpr int kStages = F8 ? 4 : 2;
+  static constexpr int kQ = N * 128;                      // per stream: N rows of 128 bytes, or 2 N of 64
+  static constexpr int kP = kKeysKT * 128;                // per stream
+  static constexpr int kTmem = 4 * W <= 64 ? 64 : 4 * W <= 128 ? 128 : 4 * W <= 256 ? 256 : 512;
+  static constexpr int kOffP = kStages * 2 * kSide;
+  static constexpr int kOffQ = kOffP + 2 * kP;
+  static constexpr int kOffCodes = kOffQ + 2 * kQ;
+  static constexpr int kOffRed = kOffCodes + kStages * kCodes;      // per stream: [4][N] maxima or sums
+  static constexpr int kOffRef = kOffRed + 2 * 4 * N * 4;           // per stream: m [N], factor [N]
+  static constexpr int kOffPre = kOffRef + 2 * 2 * N * 4;
+  static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
+  static constexpr int kOffBar = kOffSeg + 2 * (int)sizeof(ChunkSeg);
+  static constexpr int kAlloc = kOffBar + (4 * kStages + 4 + 10) * 8 + 32 + 1024;
+  static_assert(kAlloc <= 227 * 1024, "shared memory");
 };
 
-template <bool F8, int RT>
-__global__ void __launch_bounds__(kRowsThreads, RT == 1 ? 4 : RT == 2 ? 3 : 2)
-    chunk_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                      const ChunkParams p) {
-  using C = RowsCfg<F8, RT>;
+template <bool F8, int N_>
+__global__ void __launch_bounds__(kKeysThreads, 1)
+    chunk_keys_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                      const ChunkParams p, const int HB) {
+  using C = KeysCfg<F8, N_>;
+  constexpr int N = C::N, W = C::W, RB = C::kRowBytes, NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* red = (float*)(smem + C::kOffRed);
-  int64_t* pre = (int64_t*)(smem + C::kOffPre);
-  uint64_t* full = (uint64_t*)(smem + C::kOffBar);
-  uint64_t* empty = full + C::kStages;
-  volatile uint32_t* flag = (volatile uint32_t*)(empty + C::kStages);
+  int32_t* pre = (int32_t*)(smem + C::kOffPre);
+  ChunkSeg* segs = (ChunkSeg*)(smem + C::kOffSeg);
+  uint64_t* kfull = (uint64_t*)(smem + C::kOffBar);
+  uint64_t* kempty = kfull + NS;
+  uint64_t* vfull = kempty + NS;  // V and the codes
+  uint64_t* vempty = vfull + NS;
+  uint64_t* seg_full = vempty + NS;
+  uint64_t* seg_empty = seg_full + 2;
+  uint64_t* qfull = seg_empty + 2;  // per stream from here on
+  uint64_t* sfull = qfull + 2;
+  uint64_t* sfree = sfull + 2;
+  uint64_t* pfull = sfree + 2;
+  uint64_t* ofull = pfull + 2;
+  volatile uint32_t* flag = (volatile uint32_t*)(ofull + 2);
+  volatile uint32_t* tmem_slot = flag + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kRowsWarps);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&kfull[s], 1);
+      mbar_init(&kempty[s], HB);
+      mbar_init(&vfull[s], F8 ? 33 : 1);  // 8 bit: the loading warp's lanes arrive with their copies of the codes
+      mbar_init(&vempty[s], HB);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&seg_full[s], 1);
+      mbar_init(&seg_empty[s], 9 + HB);
+      mbar_init(&qfull[s], 4);
+      mbar_init(&sfull[s], 1);
+      mbar_init(&sfree[s], 4);
+      mbar_init(&pfull[s], 4);
+      mbar_init(&ofull[s], 1);
     }
     fence_mbar_init();
   }
-  ChunkWalk<kRowsKT>::plan(p, pre, kRowsThreads);  // ends with a __syncthreads
-  ChunkWalk<kRowsKT> walk;
-  walk.begin(p, pre, gridDim.x, blockIdx.x);
-  ChunkSeg sg;
-  int it = 0;  // key tiles through the ring so far
+  if (warp == 9) {
+    tmem_alloc((uint32_t*)tmem_slot, C::kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  chunk_plan(p, pre, kKeysThreads);  // with a __syncthreads at its end
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  int it = 0;  // key tiles so far
   bool bad = false;
 
-  if (warp == kRowsWarps) {
+  if (warp == 8 || warp == 10) {
     // ------------------------------------------------------------- loads
-    while (walk.next(p, sg)) {
-      if (sg.n == 0) continue;
-      const int32_t* trow = p.table + (int64_t)sg.s.row * p.tstride;
-      for (int i = sg.i0; i < sg.i1; ++i, ++it) {
-        const int st = it % C::kStages;
-        const uint32_t ph = (uint32_t)(it / C::kStages) & 1u;
-        // lanes 0..3: the pages of this tile that hold a key to look at
-        const int32_t j0 = sg.k0 + i * kRowsKT + lane * kChunkPage;
-        const bool on = lane < kRowsKT / kChunkPage && j0 < sg.hi && j0 + kChunkPage > sg.lo;
-        int32_t page = 0;
-        if (on) page = __ldg(trow + (j0 / kChunkPage) % p.tstride);
-        const bool in = on && page >= 0 && page < p.pool_pages;  // a page outside the pool is not read
-        const int np = __popc(__ballot_sync(0xffffffffu, in));
-        if (!bad) bad = !mbar_wait(&empty[st], ph ^ 1u, p.err, kErrTimeoutEmpty);
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(np * (2 * kChunkPage * C::kRowBytes + (F8 ? 32 : 0))));
-        __syncwarp();
-        if (in) {
-          uint8_t* kd = smem + st * C::kStageBytes + lane * kChunkPage * C::kRowBytes;
-          tma_load_3d(kd, &tmap_k, 0, sg.hk, page * kChunkPage, &full[st]);
-          tma_load_3d(kd + C::kTile, &tmap_v, 0, sg.hk, page * kChunkPage, &full[st]);
-          if (F8) {
-            uint8_t* cd = smem + C::kOffCodes + st * C::kCodes + lane * kChunkPage;
-            const int64_t ca = ((int64_t)page * p.Hkv + sg.hk) * kChunkPage;
-            ch_bulk(cd, p.k_code + ca, kChunkPage, &full[st]);
-            ch_bulk(cd + kRowsKT, p.v_code + ca, kChunkPage, &full[st]);
-          }
+    const bool is_v = warp == 10;  // V and the codes; warp 8: K, and the parts' descriptions
+    ChunkWalk walk;
+    if (!is_v) walk.begin(p, pre, gridDim.x, blockIdx.x);
+    const uint32_t box = (uint32_t)(HB * kChunkPage * RB);
+    const CUtensorMap* tmap = is_v ? &tmap_v : &tmap_k;
+    uint64_t* full = is_v ? vfull : kfull;
+    uint64_t* empty = is_v ? vempty : kempty;
+    for (int sn = 0;; ++sn) {
+      const int sb = sn & 1;
+      if (!is_v) {
+        ChunkSeg sg;
+        const bool more = walk.next(p, sg);
+        if (!bad) bad = !mbar_wait(&seg_empty[sb], ((uint32_t)(sn >> 1) & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
+        if (lane == 0) {
+          if (!more) sg.nrows = -1;
+          segs[sb] = sg;
+          mbar_arrive(&seg_full[sb]);
         }
         __syncwarp();
-      }
-    }
-    return;
-  }
-
-  // ------------------------------------------------------------- compute
-  const int g = lane >> 2, t4 = lane & 3;
-  const uint32_t sp = smem_u32(smem + C::kOffP);
-  while (walk.next(p, sg)) {
-    const int32_t tok0 = sg.t * p.TQ, ntok = min(p.TQ, sg.s.ql - tok0);
-    const int nrows = ntok * p.G;
-    // Q fragments, straight from global memory (the row index is token * G + head of the group)
-    uint32_t qf[RT][4][4];
-    int32_t pos_r[RT][2];  // position of the row's token, or -1 beyond the rows
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = rt * 16 + hf * 8 + g;
-        const bool ok = r < nrows;
-        const int tk = ok ? r / p.G : 0, hh = ok ? r % p.G : 0;
-        pos_r[rt][hf] = ok ? sg.s.off + tok0 + tk : -1;
-        const uint16_t* qr = p.q + (sg.s.q0 + tok0 + tk) * p.q_stride + (int64_t)(sg.hk * p.G + hh) * kChunkD;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t a_lo = 0, a_hi = 0;
-          if (ok) {
-            if (F8) {
-              // k-slots (2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9) are dims 4 t4 + (0, 2, 1, 3): the order in which
-              // the bytes of a key unpack
-              const uint2 x = *(const uint2*)(qr + kk * 16 + 4 * t4);
-              a_lo = bf16x2_mul(prmt(x.x, x.y, 0x5410u), 0x5D805D80u);  // times 2^60
-              a_hi = bf16x2_mul(prmt(x.x, x.y, 0x7632u), 0x5D805D80u);
-            } else {
-              a_lo = *(const uint32_t*)(qr + kk * 16 + 2 * t4);
-              a_hi = *(const uint32_t*)(qr + kk * 16 + 2 * t4 + 8);
-            }
-          }
-          qf[rt][kk][hf] = a_lo;
-          qf[rt][kk][2 + hf] = a_hi;
-        }
-      }
-    }
-    float m_ref[RT][2], l_r[RT][2], acc[RT][2][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m_ref[rt][0] = m_ref[rt][1] = -INFINITY;
-      l_r[rt][0] = l_r[rt][1] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[rt][0][e] = acc[rt][1][e] = 0.f;
-    }
-    const int ntile = sg.n == 0 ? 0 : sg.i1 - sg.i0;
-    for (int ii = 0; ii < ntile; ++ii, ++it) {
-      const int st = it % C::kStages;
-      const int32_t j0 = sg.k0 + (sg.i0 + ii) * kRowsKT;
-      const uint32_t sk = smem_u32(smem + st * C::kStageBytes), sv = sk + C::kTile;
-      const uint8_t* ck = smem + C::kOffCodes + st * C::kCodes;
-      if (!bad) bad = !mbar_wait(&full[st], (uint32_t)(it / C::kStages) & 1u, p.err, kErrTimeoutFull);
-      // scores of keys 16 warp .. + 15
-      float sc[RT][2][4];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[rt][0][e] = sc[rt][1][e] = 0.f;
-      if (F8) {
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          uint32_t w[4];
-          ch_ldsm(w, sk + ch_swz64(warp * 16 + nt * 8 + (lane & 7), lane >> 3));
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t b0 = ch_e4m3_even(w[kk]), b1 = ch_e4m3_odd(w[kk]);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) ch_mma(sc[rt][nt], qf[rt][kk], b0, b1);
-          }
-        }
+        if (!more || bad) break;
       } else {
+        if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+        if (bad || segs[sb].nrows < 0) break;
+      }
+      const int32_t ntile = segs[sb].ntile, j0 = segs[sb].j0, lo = segs[sb].lo, hi = segs[sb].hi;
+      const int32_t head = segs[sb].hg * HB;
+      const int32_t* trow = p.table + (int64_t)segs[sb].row * p.tstride;
+      for (int i = 0; i < ntile; ++i, ++it) {
+        const int st = it % NS;
+        // lanes 0..7: the pages of this tile that hold a key to look at
+        const int32_t j = j0 + i * kKeysKT + (lane & 7) * kChunkPage;
+        const bool on = j < hi && j + kChunkPage > lo;
+        int32_t page = -1;
+        if (on) page = __ldg(trow + (uint32_t)(j / kChunkPage) % (uint32_t)p.tstride);
+        if (page >= p.pool_pages) page = -1;  // a page outside the pool is not read
+        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0 && lane < 8)) * box;
+        if (!bad) bad = !mbar_wait(&empty[st], ((uint32_t)(it / NS) & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
+        __syncwarp();
+        if (page >= 0 && lane < 8)
+          ch_tma_4d(smem + st * 2 * C::kSide + (is_v ? C::kSide : 0) + lane * box, tmap, F8 && HB == 2 ? head / 2 : head,
+                    page * 2, &full[st]);
+        if (F8 && is_v) {
+          // 16 bytes of codes per page and head: lane = [K, V][head][page]
+          const int half = lane >> 4, hb = (lane >> 3) & 1;
+          if (page >= 0 && hb < HB) {
+            const uint8_t* src = (half ? p.v_code : p.k_code) + ((int64_t)page * p.Hkv + head + hb) * kChunkPage;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
+                             smem_u32(smem + C::kOffCodes + st * C::kCodes + lane * kChunkPage)),
+                         "l"(src)
+                         : "memory");
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
+        }
+        __syncwarp();
+      }
+      if (is_v) {
+        if (lane == 0) mbar_arrive(&seg_empty[sb]);
+        __syncwarp();
+      }
+    }
+  } else if (warp == 9 || warp == 11) {
+    // ---------------------------------------------------------- products
+    // one thread per stream: S^T, A = K (K-major, 128 keys), B = Q (K-major, W rows); O^T, A = V^T (dims-major),
+    // B = P^T (rows-major)
+    const int s = warp == 11;
+    if (s < HB && elect_one()) {
+      const uint32_t fmt = F8 ? (1u << 4) : ((1u << 4) | (1u << 7) | (1u << 10));
+      const uint32_t idesc_s = fmt | ((uint32_t)(W >> 3) << 17) | (8u << 24);
+      const uint32_t idesc_o = fmt | (1u << 15) | (1u << 16) | ((uint32_t)(W >> 3) << 17) | (4u << 24);
+      // bytes between groups of 8 keys, and from one head to the next
+      const uint32_t group = (uint32_t)(HB * 8 * RB), to_head = F8 ? 64u : 1024u;
+      const bool sw64 = F8 && HB == 1;
+      const uint64_t dk = ch_sdesc(smem_u32(smem) + s * to_head, group, sw64);
+      const uint64_t dv = ch_sdesc(smem_u32(smem + C::kSide) + s * to_head, group, sw64);
+      const uint64_t dq = ch_sdesc(smem_u32(smem + C::kOffQ + s * C::kQ), 8 * RB, F8);
+      const uint64_t dp = ch_sdesc(smem_u32(smem + C::kOffP + s * C::kP), 1024, false);
+      constexpr int kStep = F8 ? 32 : 16;  // keys of one product of O^T
+      const uint32_t v_step = (kStep / 8) * (group >> 4);
+      int ks = 0, vs = 0;               // stages of the next S^T and the next O^T
+      uint32_t kp = 0, vp = 0, tp = 0;  // their parities, and that of S^T's tile
+      uint32_t op = 0;                  // parity of O^T's tile
+      auto issue_s = [&]() {
+        if (!bad) bad = !mbar_wait(&kfull[ks], kp, p.err, kErrTimeoutFull);
+        if (!bad) bad = !mbar_wait(&sfree[s], tp ^ 1u, p.err, kErrTimeoutAccum);  // the tile before has been read
+        tc_fence_after();
+        const uint64_t a = dk + (uint32_t)ks * (2 * C::kSide >> 4);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t w[4];
-          ch_ldsm(w, sk + ch_swz128(warp * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+        for (int kk = 0; kk < (F8 ? 2 : 4); ++kk)
+          ch_mma_ss<F8>(tmem + s * W, a + 2 * kk, dq + 2 * kk, idesc_s, kk > 0 ? 1u : 0u);
+        tc_commit(&sfull[s]);
+        tc_commit(&kempty[ks]);
+        tp ^= 1u;
+        if (++ks == NS) {
+          ks = 0;
+          kp ^= 1u;
+        }
+      };
+      for (int sn = 0; !bad; ++sn) {
+        const int sb = sn & 1;
+        bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+        if (bad || segs[sb].nrows < 0) break;
+        const int nt = segs[sb].ntile;
+        bad = !mbar_wait(&qfull[s], (uint32_t)sn & 1u, p.err, kErrTimeoutFull);
+        if (nt > 0) issue_s();
+        for (int i = 0; i < nt; ++i) {
+          if (i + 1 < nt) issue_s();
+          if (!bad) bad = !mbar_wait(&vfull[vs], vp, p.err, kErrTimeoutFull);
+          if (!bad) bad = !mbar_wait(&pfull[s], op, p.err, kErrTimeoutAccum);
+          tc_fence_after();
+          const uint64_t a = dv + (uint32_t)vs * (2 * C::kSide >> 4);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            ch_mma(sc[rt][0], qf[rt][kk], w[0], w[1]);
-            ch_mma(sc[rt][1], qf[rt][kk], w[2], w[3]);
+          for (int kk = 0; kk < kKeysKT / kStep; ++kk)
+            ch_mma_ss<F8>(tmem + (2 + s) * W, a + kk * v_step, dp + kk * (kStep / 8) * 64, idesc_o,
+                          (i > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(&ofull[s]);
+          tc_commit(&vempty[vs]);
+          op ^= 1u;
+          if (++vs == NS) {
+            vs = 0;
+            vp ^= 1u;
           }
         }
+        mbar_arrive(&seg_empty[sb]);
       }
-      const int32_t first_pos = sg.s.off + tok0;
-      const bool whole = j0 + kRowsKT - 1 <= first_pos && j0 >= sg.lo &&
-                         (p.window <= 0 || j0 > first_pos + ntok - 1 - p.window);
-      float vscale[2][2];  // per key of this thread: 2^(e_v + 60)
-      float mx[RT][2];
+    }
+    __syncwarp();
+  } else {
+    // ----------------------------------------------------------- softmax
+    const int s = warp >> 2, wq = warp & 3, tid = threadIdx.x & 127;  // tid: key of the tile, TMEM lane
+    const bool mine = s < HB;
+    const uint32_t tl = tmem + ((uint32_t)(wq * 32) << 16);
+    const uint32_t t_s = tl + s * W, t_o = tl + (2 + s) * W;
+    float* red = (float*)(smem + C::kOffRed) + s * 4 * N;
+    float* nref = (float*)(smem + C::kOffRef) + s * 2 * N;  // -m of a row
+    float* fac = nref + N;
+    uint8_t* qs = smem + C::kOffQ + s * C::kQ;
+    uint8_t* ps = smem + C::kOffP + s * C::kP;
+    constexpr float kUp = F8 ? 8.75f : 8.0f;   // P at most 2^kUp (448 is the most e4m3 holds)
+    constexpr float kBase = F8 ? 2.0f : 0.0f;  // log2 P of the largest when the reference moves
+    for (int sn = 0;; ++sn) {
+      const int sb = sn & 1;
+      if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+      bad = ch_named_or(6, 256, bad);  // all eight warps leave together
+      const ChunkSeg& sg = segs[sb];
+      const int nrows = sg.nrows;
+      if (nrows < 0 || bad) break;
+      const int ntile = sg.ntile;
+      const int32_t lo = sg.lo, hi = sg.hi, first_pos = sg.first_pos;
+      const int head0 = (sg.hg * HB + s) * p.G;
+      float q_unit = 1.0f;
+      ch_f2 l[N / 2];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) mx[rt][0] = mx[rt][1] = -INFINITY;
+      for (int r = 0; r < N / 2; ++r) l[r] = 0ull;
+      if (mine && ntile > 0) {
+        // Q into shared memory: 8 threads per row, 16 rows at a time
+        uint4 x[N / 16];
+        uint32_t am = 0;
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        float ks[2] = {p.scale2, p.scale2};
+        for (int k = 0; k < N / 16; ++k) {
+          const int r = k * 16 + (tid >> 3);
+          x[k] = make_uint4(0, 0, 0, 0);
+          if (r < nrows) {
+            const int tk = r / p.G;
+            x[k] = *(const uint4*)(p.q + (sg.tok0 + tk) * p.q_stride + (int64_t)(head0 + r - tk * p.G) * kChunkD +
+                                   (tid & 7) * 8);
+          }
+          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) am = max(am, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
+        }
+        float up = 1.0f;
         if (F8) {
-          const int key = warp * 16 + nt * 8 + 2 * t4;
-          const uint32_t kc = *(const uint16_t*)(ck + key), vc = *(const uint16_t*)(ck + kRowsKT + key);
-          ks[0] = p.scale2 * ch_code_scale(kc & 0xFFu, 60);
-          ks[1] = p.scale2 * ch_code_scale(kc >> 8, 60);
-          vscale[nt][0] = ch_code_scale(vc & 0xFFu, 60);
-          vscale[nt][1] = ch_code_scale(vc >> 8, 60);
+          // largest magnitude of the unit's finite values into [128, 256)
+          am = __reduce_max_sync(0xffffffffu, am >= 0x7F800000u ? 0u : am);
+          if (lane == 0) red[wq] = __uint_as_float(am);
+          ch_named_sync(1 + s, 128);
+          am = max(max(__float_as_uint(red[0]), __float_as_uint(red[1])),
+                   max(__float_as_uint(red[2]), __float_as_uint(red[3])));
+          const int ex = max((int)(am >> 23), 14);
+          up = __uint_as_float((uint32_t)min(261 - ex, 254) << 23);
+          q_unit = 1.0f / up;
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+        for (int k = 0; k < N / 16; ++k) {
+          const int r = k * 16 + (tid >> 3), c = tid & 7;
+          if (!F8) {
+            *(uint4*)(qs + r * 128 + ((c ^ (r & 7)) << 4)) = x[k];
+          } else {
+            const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+            uint32_t h4[2], l4[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float v[4] = {__uint_as_float(w[2 * e] << 16) * up, __uint_as_float(w[2 * e] & 0xFFFF0000u) * up,
+                                  __uint_as_float(w[2 * e + 1] << 16) * up,
+                                  __uint_as_float(w[2 * e + 1] & 0xFFFF0000u) * up};
+              float hh[4];
+#pragma unroll
+              // what is not finite stays: e4m3 makes it NaN, and with it the row
+              for (int y = 0; y < 4; ++y) hh[y] = fabsf(v[y]) < 1e30f ? ch_round4(v[y]) : __uint_as_float(0x7FC00000u);
+              h4[e] = ch_e4m3x2(hh[0], hh[1]) | (ch_e4m3x2(hh[2], hh[3]) << 16);
+              l4[e] = ch_e4m3x2(16.f * (v[0] - hh[0]), 16.f * (v[1] - hh[1])) |
+                      (ch_e4m3x2(16.f * (v[2] - hh[2]), 16.f * (v[3] - hh[3])) << 16);
+            }
+            const int r2 = N + r;
+            *(uint2*)(qs + r * 64 + (((c >> 1) ^ ((r >> 1) & 3)) << 4) + (c & 1) * 8) = make_uint2(h4[0], h4[1]);
+            *(uint2*)(qs + r2 * 64 + (((c >> 1) ^ ((r2 >> 1) & 3)) << 4) + (c & 1) * 8) = make_uint2(l4[0], l4[1]);
+          }
+        }
+        if (tid < N) nref[tid] = tid < nrows ? INFINITY : -INFINITY;  // unused rows: P = 0
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        ch_named_sync(1 + s, 128);
+        if (lane == 0) mbar_arrive(&qfull[s]);
+      } else if (!mine || ntile == 0) {
+        // an idle stream keeps the barriers' count of segments
+        if (lane == 0) mbar_arrive(&qfull[s]);
+      }
+      for (int i = 0; i < ntile; ++i, ++it) {
+        const int st = it % NS;
+        if (!mine) continue;
+        const int32_t j = sg.j0 + i * kKeysKT + tid;
+        // rows [r_lo, r_hi) see this key
+        int r_lo = 0, r_hi = nrows;
+        const int32_t jt = sg.j0 + i * kKeysKT;
+        const bool whole = jt + kKeysKT - 1 <= first_pos && jt >= lo &&
+                           (p.window <= 0 || jt > first_pos + sg.ntok - 1 - p.window);
+        if (!whole) {
+          r_lo = max(0, min(j - first_pos, 1 << 16)) * p.G;
+          if (p.window > 0) r_hi = min(nrows, max(0, min(j + p.window - first_pos, 1 << 16)) * p.G);
+        }
+        float kf = p.scale2, ev = 0.f, einv = 1.f;
+        if (F8 || !whole) {
+          if (!bad) bad = !mbar_wait(&vfull[st], (uint32_t)(it / NS) & 1u, p.err, kErrTimeoutFull);
+        }
+        if (F8) {
+          const uint8_t* cc = smem + C::kOffCodes + st * C::kCodes + s * kKeysKT + tid;
+          const uint32_t kc = cc[0], vc = cc[2 * kKeysKT];
+          const float nan = __uint_as_float(0x7FC00000u);
+          kf = kc == 255u ? nan : p.scale2 * q_unit * __uint_as_float(kc << 23);
+          ev = vc == 255u ? nan : (float)((int)vc - 127);
+          einv = __uint_as_float((254u - min(vc, 253u)) << 23);
+        }
+        if (!whole && (j < lo || j >= hi)) {
+          // a key nobody may see: 0 times what its V row (or an earlier tile) holds must be 0
+          // (swizzled within the row, but for two heads in one row: 16-byte piece c of head s is 4 s + c)
+          uint8_t* vr = smem + st * 2 * C::kSide + C::kSide +
+                        (F8 ? tid * (HB * RB) : ((tid >> 3) * HB + s) * 8 * RB + (tid & 7) * RB);
+#pragma unroll
+          for (int c = 0; c < RB / 16; ++c)
+            *(uint4*)(vr + (F8 && HB == 2 ? (4 * s + c) ^ (tid & 7) : c) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        if (!bad) bad = !mbar_wait(&sfull[s], (uint32_t)it & 1u, p.err, kErrTimeoutAccum);
+        tc_fence_after();
+        ch_f2 x[N / 2];
+        const ch_f2 kf2 = ch_pair(kf, kf), ev2 = ch_pair(ev, ev);
+        // t - m (nm: -m of the rows) of 8 rows from TMEM; -inf where the key is hidden from the row
+        auto scores = [&](int r0, ch_f2 (&t)[4], const ch_f2 (&nm)[4]) {
+          uint32_t a[8], b[8];
+          ch_ld8(t_s + r0, a);
+          if (F8) ch_ld8(t_s + N + r0, b);
+          tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float v = sc[rt][nt][e] * ks[e & 1];
-            if (!whole) {
-              const int32_t kj = j0 + warp * 16 + nt * 8 + 2 * t4 + (e & 1), ps = pos_r[rt][e >> 1];
-              if (kj > ps || (p.window > 0 && kj <= ps - p.window)) v = -INFINITY;
+            ch_f2 v = ((ch_f2)a[2 * e + 1] << 32) | a[2 * e];
+            if (F8) {
+              v = ch_fma2(((ch_f2)b[2 * e + 1] << 32) | b[2 * e], ch_pair(0.0625f, 0.0625f), v);
+              t[e] = ch_add2(ch_fma2(v, kf2, ev2), nm[e]);
+            } else {
+              t[e] = ch_fma2(v, kf2, nm[e]);
             }
-            sc[rt][nt][e] = v;
-            mx[rt][e >> 1] = fmaxf(mx[rt][e >> 1], v);
           }
-      }
-      bool need = false;
+          if (!whole) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+            for (int e = 0; e < 4; ++e) {
+              const int r = r0 + 2 * e;
+              t[e] = ch_pair(r < r_lo || r >= r_hi ? -INFINITY : ch_lo(t[e]),
+                             r + 1 < r_lo || r + 1 >= r_hi ? -INFINITY : ch_hi(t[e]));
+            }
+          }
+        };
+        for (int again = 0;; ++again) {
+          float mx = -INFINITY;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          mx[rt][hf] = fmaxf(mx[rt][hf], __shfl_xor_sync(0xffffffffu, mx[rt][hf], 1));
-          mx[rt][hf] = fmaxf(mx[rt][hf], __shfl_xor_sync(0xffffffffu, mx[rt][hf], 2));
-          need |= mx[rt][hf] > m_ref[rt][hf] + 8.0f;
+          for (int r0 = 0; r0 < N; r0 += 8) {
+            if (r0 < nrows) {
+              ch_f2 t[4], nm[4];
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const ulonglong2 y = *(const ulonglong2*)(nref + r0 + 2 * e);
+                nm[e] = y.x;
+                nm[e + 1] = y.y;
+              }
+              scores(r0, t, nm);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[r0 / 2 + e] = t[e];
+                mx = fmaxf(mx, fmaxf(ch_lo(t[e]), ch_hi(t[e])));
+              }
+            }
+          }
+          // the second time round nothing is left above the reference's reach
+          if (!ch_named_or(1 + s, 128, mx > kUp) || again) break;
+          const ch_f2 zero[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll 1
+          for (int r0 = 0; r0 < nrows; r0 += 8) {
+            ch_f2 t[4];
+            scores(r0, t, zero);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float m0 = ch_warp_max(ch_lo(t[e])), m1 = ch_warp_max(ch_hi(t[e]));
+              if (lane == 0) *(float2*)(red + wq * N + r0 + 2 * e) = make_float2(m0, m1);
+            }
+          }
+          ch_named_sync(3 + s, 128);
+          if (tid < nrows) {
+            const float m = fmaxf(fmaxf(red[tid], red[N + tid]), fmaxf(red[2 * N + tid], red[3 * N + tid]));
+            const float m0 = -nref[tid], m1 = m > m0 + kUp ? m - kBase : m0;
+            fac[tid] = m1 == m0 ? 1.0f : ch_exp2(m0 - m1);
+            nref[tid] = -m1;
+          }
+          ch_named_sync(3 + s, 128);
+#pragma unroll
+          for (int r = 0; r < N; r += 2)
+            if (r < nrows) l[r / 2] = ch_mul2(l[r / 2], *(const ch_f2*)(fac + r));
+          if (i > 0) {
+            // O^T of the tiles before, once their products are done
+            if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < W; c0 += 8) {
+              const int r0 = F8 && c0 >= N ? c0 - N : c0;
+              if (r0 >= nrows) continue;
+              uint32_t o8[8];
+              ch_ld8(t_o + c0, o8);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o8[e] = __float_as_uint(__uint_as_float(o8[e]) * fac[r0 + e]);
+              ch_st8(t_o + c0, o8);
+            }
+            tmem_st_wait();
+          }
         }
-      if (!F8 && !whole) {
-        // V rows of keys nobody may see: 0 times what the page holds there must be 0
-        for (int c = threadIdx.x; c < kRowsKT * 8; c += kRowsWarps * 32) {
-          const int32_t kj = j0 + (c >> 3);
-          if (kj < sg.lo || kj >= sg.hi)
-            *(uint4*)(smem + st * C::kStageBytes + C::kTile + c * 16) = make_uint4(0, 0, 0, 0);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sfree[s]);  // S^T is in registers
+        // P^T of the tile before has been used
+        if (i > 0) {
+          if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
+        }
+        uint8_t* pr = ps + tid * 128;
+        const int sw = tid & 7;
+        const ch_f2 einv2 = ch_pair(einv, einv);
+        constexpr int kPer = F8 ? 16 : 8;  // rows of a 16-byte piece
+#pragma unroll
+        for (int r0 = 0; r0 < N; r0 += kPer) {
+          if (r0 >= nrows) break;  // columns of rows that are not there: whatever they hold, nobody reads their results
+          uint32_t w[4], w2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ch_f2 pe[kPer / 8];
+#pragma unroll
+            for (int y = 0; y < kPer / 8; ++y) {
+              const int k = r0 / 2 + e * (kPer / 8) + y;
+              pe[y] = ch_pair(ch_exp2(ch_lo(x[k])), ch_exp2(ch_hi(x[k])));
+              l[k] = F8 ? ch_fma2(pe[y], einv2, l[k]) : ch_add2(pe[y], l[k]);
+            }
+            if (!F8) {
+              w[e] = ch_bf16x2(ch_lo(pe[0]), ch_hi(pe[0]));
+            } else {
+              // hi: 4 significant bits; lo: 16 times the rest
+              uint32_t h4[2], l4[2];
+#pragma unroll
+              for (int y = 0; y < kPer / 8; ++y) {
+                const ch_f2 h = ch_pair(ch_round4(ch_lo(pe[y])), ch_round4(ch_hi(pe[y])));
+                const ch_f2 d = ch_mul2(ch_fma2(h, ch_pair(-1.f, -1.f), pe[y]), ch_pair(16.f, 16.f));
+                h4[y] = ch_e4m3x2(ch_lo(h), ch_hi(h));
+                l4[y] = ch_e4m3x2(ch_lo(d), ch_hi(d));
+              }
+              w[e] = h4[0] | (h4[kPer / 8 - 1] << 16);
+              w2[e] = l4[0] | (l4[kPer / 8 - 1] << 16);
+            }
+          }
+          *(uint4*)(pr + (((r0 / kPer) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (F8) *(uint4*)(pr + ((((N + r0) / kPer) ^ sw) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pfull[s]);
       }
-      if (ch_named_or(1, kRowsWarps * 32, need)) {
-        if (t4 == 0) {
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) red[warp * C::kRows + rt * 16 + hf * 8 + g] = mx[rt][hf];
+
+      // ----------------------------------------------------- end of a part
+      const int slot = sg.slot;
+      if (mine) {
+        if (ntile > 0) {
+          if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
+          tc_fence_after();
         }
-        ch_named_sync(2, kRowsWarps * 32);
+        // sums over the keys
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            float m = m_ref[rt][hf];
-#pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) m = fmaxf(m, red[w * C::kRows + rt * 16 + hf * 8 + g]);
-            const float c = m == m_ref[rt][hf] ? 1.0f : ch_exp2(m_ref[rt][hf] - m);
-            m_ref[rt][hf] = m;
-            l_r[rt][hf] *= c;
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) {
-              acc[rt][dt][2 * hf] *= c;
-              acc[rt][dt][2 * hf + 1] *= c;
-            }
-          }
-      }
-      // P, and its bf16 form for P V
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const float m = m_ref[rt][hf] == -INFINITY ? 0.f : m_ref[rt][hf];
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            float p0 = ch_exp2(sc[rt][nt][2 * hf] - m), p1 = ch_exp2(sc[rt][nt][2 * hf + 1] - m);
-            l_r[rt][hf] += p0 + p1;
-            if (F8) {
-              p0 = p0 == 0.f ? 0.f : p0 * vscale[nt][0];
-              p1 = p1 == 0.f ? 0.f : p1 * vscale[nt][1];
-            }
-            const int r = rt * 16 + hf * 8 + g;
-            *(uint32_t*)(smem + C::kOffP + ch_swz128(r, 2 * warp + nt) + 4 * t4) = ch_bf16x2(p0, p1);
+        for (int r = 0; r < N; ++r) {
+          if (r < nrows) {
+            float v = r & 1 ? ch_hi(l[r / 2]) : ch_lo(l[r / 2]);
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) red[wq * N + r] = v;
           }
         }
-      ch_named_sync(3, kRowsWarps * 32);
-      // O += P V, dims 16 warp .. + 15
+        // O^T from TMEM to rows of 64 floats in P's place: lane < 16 of warp wq holds dim 16 wq + lane
+        float* os = (float*)ps;
+        if (ntile > 0) {
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        uint32_t w8[4];
-        if (F8) ch_ldsm_t(w8, sv + ch_swz64(k2 * 32 + lane, warp));
+          for (int r0 = 0; r0 < N; r0 += 8) {
+            if (r0 < nrows) {
+              uint32_t a[8], b[8];
+              ch_ld8(t_o + r0, a);
+              if (F8) ch_ld8(t_o + N + r0, b);
+              tmem_ld_wait();
+              if (lane < 16) {
 #pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-          const int kk = 2 * k2 + kh;
-          uint32_t b[4];
-          if (F8) {
-            b[0] = ch_e4m3_even(w8[2 * kh]);
-            b[1] = ch_e4m3_even(w8[2 * kh + 1]);
-            b[2] = ch_e4m3_odd(w8[2 * kh]);
-            b[3] = ch_e4m3_odd(w8[2 * kh + 1]);
+                for (int e = 0; e < 8; ++e)
+                  os[(r0 + e) * 64 + wq * 16 + lane] =
+                      F8 ? fmaf(__uint_as_float(b[e]), 0.0625f, __uint_as_float(a[e])) : __uint_as_float(a[e]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        ch_named_sync(3 + s, 128);
+        for (int x = tid; x < nrows * 16; x += 128) {
+          const int r = x >> 4, d = (x & 15) * 4;
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+          float lr = 0.f, m = -INFINITY;
+          if (ntile > 0) {
+            y = *(const float4*)(os + r * 64 + d);
+            lr = red[r] + red[N + r] + red[2 * N + r] + red[3 * N + r];
+            m = -nref[r];
+          }
+          if (slot >= 0) {
+            const int64_t row = ((int64_t)slot * HB + s) * N + r;
+            *(float4*)(p.part_o + row * kChunkD + d) = y;
+            if (d == 0) *(float2*)(p.part_ml + row * 2) = make_float2(m, lr);
           } else {
-            ch_ldsm_t(b, sv + ch_swz128(kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), 2 * warp + (lane >> 4)));
-          }
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            uint32_t a[4];
-            ch_ldsm(a, sp + ch_swz128(rt * 16 + (lane & 15), 2 * kk + (lane >> 4)));
-            ch_mma(acc[rt][0], a, b[0], b[1]);
-            ch_mma(acc[rt][1], a, b[2], b[3]);
+            const int tk = r / p.G, h = head0 + r - tk * p.G;
+            const int64_t tok = sg.tok0 + tk;
+            if (p.lse && d == 0) p.lse[tok * p.Hq + h] = m + log2f(lr);
+            const float inv = ch_norm(p, h, lr, m);
+            *(uint2*)(p.o + (tok * p.Hq + h) * kChunkD + d) =
+                make_uint2(ch_bf16x2(y.x * inv, y.y * inv), ch_bf16x2(y.z * inv, y.w * inv));
           }
         }
+        ch_named_sync(3 + s, 128);  // red, nref and os are free again
+      }
+      if (slot >= 0) {
+        __threadfence();
+        ch_named_sync(5, 256);
+        if (threadIdx.x == 0) {
+          const uint32_t old = atomicAdd(&p.counters[sg.c0], 1u);
+          const uint32_t last = old == (uint32_t)(sg.c1 - sg.c0);
+          if (last) p.counters[sg.c0] = 0u;
+          *flag = last;
+        }
+        ch_named_sync(6, 256);
+        if (*flag) {
+          __threadfence();
+          chunk_join(p, sg, HB, N, threadIdx.x, 256);
+        }
+        ch_named_sync(5, 256);  // flag is free again
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      if (lane == 0) mbar_arrive(&seg_empty[sb]);
     }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kTmem);
+  }
+}
 
-    // ------------------------------------------------------- end of a part
-    // this thread's dims of rows g, g + 8: [0..1] and [2..3] below are consecutive pairs
-    //   bf16: dims 16 warp + 2 t4, + 1 (tile 0) and 16 warp + 8 + 2 t4, + 1 (tile 1)
-    //   8 bit: dims 16 warp + 4 t4 + (0, 2) (tile 0) and + (1, 3) (tile 1)
-    ch_named_sync(1, kRowsWarps * 32);  // red is free
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        float l = l_r[rt][hf];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t4 == 0) red[warp * C::kRows + rt * 16 + hf * 8 + g] = l;
+// ---------------------------------------------------------- rows on M --
+// CTA = two tiles of 128 rows (128 / G tokens times the G heads of a kv head),
+// a softmax warpgroup each (thread = row = TMEM lane), one warp that loads, one
+// that issues the products: S_t = Q_t K^T (both in shared memory), O_t += P_t V
+// (P_t bf16 in TMEM), tiles of 128 keys.  The tiles take turns: while one's
+// softmax runs the tensor core works for the other.  Bound by the exponentials:
+// 2 x 128 x 128 of them a key tile at 16 per cycle and SM are 2048 cycles, the
+// products 1024, K and V from L2 32 KB.  The reference of a row moves when a
+// score exceeds it by 8.
+//
+// 8-bit pages: a fourth warpgroup turns a tile's values into bf16 with their
+// power of two (exact) while the one before is used, about 450 issue cycles of
+// the 2048 a tile takes; the rest of the kernel is the same.
+constexpr int kRowsKT = 128;
+
+template <bool F8>
+struct RowsCfg {
+  static constexpr int kThreads = F8 ? 512 : 384;
+  static constexpr int kStages = F8 ? 3 : 4;
+  static constexpr int kSide = kRowsKT * 128;            // K or V of a tile, bf16
+  static constexpr int kRaw = F8 ? 2 : 0;                // stages of 8-bit tiles
+  static constexpr int kRawSide = kRowsKT * 64;
+  static constexpr int kOffRaw = 2 * 128 * 128 + kStages * 2 * kSide;
+  static constexpr int kOffCodes = kOffRaw + kRaw * 2 * kRawSide;
+  static constexpr int kOffPre = kOffCodes + kRaw * 2 * kRowsKT;
+  static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
+  static constexpr int kOffBar = kOffSeg + 2 * (int)sizeof(ChunkSeg);
+  static constexpr int kAlloc = kOffBar + (2 * kStages + 4 + 4 + 2 + 8) * 8 + 16 + 1024;
+  static_assert(kAlloc <= 227 * 1024, "shared memory");
+};
+
+// 32 consecutive 32-bit columns of this warp's 32 lanes, no wait.
+__device__ __forceinline__ void ch_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void ch_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <bool F8>
+__global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
+    chunk_rows_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                      const __grid_constant__ CUtensorMap tmap_v, const ChunkParams p) {
+  using C = RowsCfg<F8>;
+  constexpr int NS = C::kStages, RB = F8 ? 64 : 128;
+  constexpr uint32_t kColO = 256, kColP = 384;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* kv0 = smem + 2 * 128 * 128;
+  int32_t* pre = (int32_t*)(smem + C::kOffPre);
+  ChunkSeg* segs = (ChunkSeg*)(smem + C::kOffSeg);
+  uint64_t* kvfull = (uint64_t*)(smem + C::kOffBar);
+  uint64_t* kvempty = kvfull + NS;
+  uint64_t* rawfull = kvempty + NS;  // [2]
+  uint64_t* rawempty = rawfull + 2;  // [2]
+  uint64_t* seg_full = rawempty + 2;
+  uint64_t* seg_empty = seg_full + 2;
+  uint64_t* qfull = seg_empty + 2;
+  uint64_t* qempty = qfull + 1;
+  uint64_t* sfull = qempty + 1;  // per tile from here on
+  uint64_t* sfree = sfull + 2;
+  uint64_t* pfull = sfree + 2;
+  uint64_t* ofull = pfull + 2;
+  volatile uint32_t* flag = (volatile uint32_t*)(ofull + 2);
+  volatile uint32_t* tmem_slot = flag + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tq1 = p.TQ / 2;  // tokens of a tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&kvfull[s], F8 ? 4 : 1);
+      mbar_init(&kvempty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&rawfull[s], 33);  // the loading warp's lanes arrive with their copies of the codes
+      mbar_init(&rawempty[s], 4);
+      mbar_init(&seg_full[s], 1);
+      mbar_init(&seg_empty[s], 9 + (F8 ? 4 : 0));
+      mbar_init(&sfull[s], 1);
+      mbar_init(&sfree[s], 4);
+      mbar_init(&pfull[s], 4);
+      mbar_init(&ofull[s], 1);
+    }
+    mbar_init(qfull, 1);
+    mbar_init(qempty, 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc((uint32_t*)tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  chunk_plan(p, pre, C::kThreads);  // with a __syncthreads at its end
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  int it = 0;  // key tiles so far
+  bool bad = false;
+  // 8 bit: 512 threads start with 128 registers each: 256 * 176 + 128 * 64 + 128 * 80 of them from here on
+
+  if (warp == 8) {
+    // ------------------------------------------------------------- loads
+    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    ChunkWalk walk;
+    walk.begin(p, pre, gridDim.x, blockIdx.x);
+    for (int sn = 0;; ++sn) {
+      const int sb = sn & 1;
+      ChunkSeg sg;
+      const bool more = walk.next(p, sg);
+      if (!bad) bad = !mbar_wait(&seg_empty[sb], ((uint32_t)(sn >> 1) & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
+      if (lane == 0) {
+        if (!more) sg.nrows = -1;
+        segs[sb] = sg;
+        mbar_arrive(&seg_full[sb]);
       }
-    ch_named_sync(2, kRowsWarps * 32);
-    const float unit = F8 ? 1152921504606846976.0f : 1.0f;  // 2^60: what P and V left out
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = rt * 16 + hf * 8 + g;
-        float l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) l += red[w * C::kRows + r];
-        const float m = m_ref[rt][hf];
-        const int d0 = F8 ? warp * 16 + 4 * t4 : warp * 16 + 2 * t4, d1 = F8 ? d0 + 2 : d0 + 8;
-        float x0 = acc[rt][0][2 * hf] * unit, x1 = acc[rt][0][2 * hf + 1] * unit;
-        float x2 = acc[rt][1][2 * hf] * unit, x3 = acc[rt][1][2 * hf + 1] * unit;
-        if (F8) {  // dims (0, 2), (1, 3) -> (0, 1), (2, 3)
-          const float s = x1;
-          x1 = x2;
-          x2 = s;
+      __syncwarp();
+      if (!more || bad) break;
+      if (!bad) bad = !mbar_wait(qempty, ((uint32_t)sn & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
+      if (lane == 0) {
+        // Q: rows (token, head of the group) of both tiles
+        const int nq = sg.ntile == 0 ? 0 : sg.ntok > tq1 ? 2 : 1;
+        mbar_arrive_expect_tx(qfull, (uint32_t)(nq * tq1 * p.G * 128));
+        for (int t = 0; t < nq; ++t)
+          tma_load_3d(smem + t * 128 * 128, &tmap_q, 0, sg.hg * p.G, (int32_t)(sg.tok0 + t * tq1), qfull);
+      }
+      __syncwarp();
+      const int32_t* trow = p.table + (int64_t)sg.row * p.tstride;
+      for (int i = 0; i < sg.ntile; ++i, ++it) {
+        // lanes 0..7: the pages of this tile that hold a key to look at
+        const int32_t j = sg.j0 + i * kRowsKT + (lane & 7) * kChunkPage;
+        const bool on = j < sg.hi && j + kChunkPage > sg.lo;
+        int32_t page = -1;
+        if (on) page = __ldg(trow + (uint32_t)(j / kChunkPage) % (uint32_t)p.tstride);
+        if (page >= p.pool_pages) page = -1;  // a page outside the pool is not read
+        const uint32_t n8 = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0 && lane < 8));
+        const int st = F8 ? it % 2 : it % NS;
+        uint64_t* full = F8 ? &rawfull[st] : &kvfull[st];
+        uint8_t* kd = F8 ? smem + C::kOffRaw + st * 2 * C::kRawSide : kv0 + st * 2 * C::kSide;
+        const int side = F8 ? C::kRawSide : C::kSide;
+        if (!bad)
+          bad = !mbar_wait(F8 ? &rawempty[st] : &kvempty[st], ((uint32_t)(it / (F8 ? 2 : NS)) & 1u) ^ 1u, p.err,
+                           kErrTimeoutEmpty);
+        if (lane == 0) mbar_arrive_expect_tx(full, n8 * 2 * kChunkPage * RB);
+        __syncwarp();
+        if (page >= 0 && lane < 8) {
+          tma_load_3d(kd + lane * kChunkPage * RB, &tmap_k, 0, sg.hg, page * kChunkPage, full);
+          tma_load_3d(kd + side + lane * kChunkPage * RB, &tmap_v, 0, sg.hg, page * kChunkPage, full);
         }
-        if (sg.slot >= 0) {
-          float* po = p.part_o + ((int64_t)sg.slot * C::kRows + r) * kChunkD;
-          *(float2*)(po + d0) = make_float2(x0, x1);
-          *(float2*)(po + d1) = make_float2(x2, x3);
-          if (warp == 0 && t4 == 0)
-            *(float2*)(p.part_ml + ((int64_t)sg.slot * C::kRows + r) * 2) = make_float2(m, l);
-        } else if (r < nrows) {
-          const int h = sg.hk * p.G + r % p.G;
-          const int64_t tok = sg.s.q0 + tok0 + r / p.G;
-          if (p.lse && warp == 0 && t4 == 0) p.lse[tok * p.Hq + h] = m + log2f(l);
-          float den = l;
-          if (p.sinks) den += exp2f(bf16_bits_to_f32(p.sinks[h]) * kChLog2e - m);
-          const float inv = l == 0.f ? 0.f : 1.0f / den;
-          uint16_t* orow = p.o + (tok * p.Hq + h) * kChunkD;
-          *(uint32_t*)(orow + d0) = ch_bf16x2(x0 * inv, x1 * inv);
-          *(uint32_t*)(orow + d1) = ch_bf16x2(x2 * inv, x3 * inv);
-        }
-      }
-    if (sg.slot >= 0) {
-      __threadfence();
-      ch_named_sync(3, kRowsWarps * 32);
-      if (threadIdx.x == 0) {
-        const uint32_t old = atomicAdd(&p.counters[sg.c0], 1u);
-        const uint32_t mine = old == (uint32_t)(sg.c1 - sg.c0);
-        if (mine) p.counters[sg.c0] = 0u;
-        *flag = mine;
-      }
-      ch_named_sync(1, kRowsWarps * 32);
-      if (*flag) {
-        __threadfence();
-        // join the parts in the order of the keys: 16 lanes per row, 4 dims each
-        for (int x = threadIdx.x; x < nrows * 16; x += kRowsWarps * 32) {
-          const int r = x >> 4, d = (x & 15) * 4;
-          float m = -INFINITY;
-          for (int c = sg.c0; c <= sg.c1; ++c) {
-            const int64_t sl = c == sg.c0 ? sg.first_slot : 2 * c;
-            m = fmaxf(m, __ldcg(p.part_ml + (sl * C::kRows + r) * 2));
+        if (F8) {
+          // 16 bytes of codes per page: lanes 0..7 K's, 8..15 V's
+          if (page >= 0 && lane < 16) {
+            const uint8_t* src = (lane >> 3 ? p.v_code : p.k_code) + ((int64_t)page * p.Hkv + sg.hg) * kChunkPage;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
+                             smem_u32(smem + C::kOffCodes + st * 2 * kRowsKT + lane * kChunkPage)),
+                         "l"(src)
+                         : "memory");
           }
-          const float me = m == -INFINITY ? 0.f : m;
-          float l = 0.f;
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int c = sg.c0; c <= sg.c1; ++c) {
-            const int64_t sl = c == sg.c0 ? sg.first_slot : 2 * c;
-            const float2 ml = __ldcg((const float2*)(p.part_ml + (sl * C::kRows + r) * 2));
-            const float4 y = __ldcg((const float4*)(p.part_o + (sl * C::kRows + r) * kChunkD + d));
-            const float f = exp2f(ml.x - me);
-            l += ml.y * f;
-            a.x += y.x * f;
-            a.y += y.y * f;
-            a.z += y.z * f;
-            a.w += y.w * f;
-          }
-          const int h = sg.hk * p.G + r % p.G;
-          const int64_t tok = sg.s.q0 + tok0 + r / p.G;
-          if (p.lse && d == 0) p.lse[tok * p.Hq + h] = m + log2f(l);
-          float den = l;
-          if (p.sinks) den += exp2f(bf16_bits_to_f32(p.sinks[h]) * kChLog2e - m);
-          const float inv = l == 0.f ? 0.f : 1.0f / den;
-          uint2 w;
-          w.x = ch_bf16x2(a.x * inv, a.y * inv);
-          w.y = ch_bf16x2(a.z * inv, a.w * inv);
-          *(uint2*)(p.o + (tok * p.Hq + h) * kChunkD + d) = w;
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
         }
+        __syncwarp();
       }
     }
-    ch_named_sync(2, kRowsWarps * 32);  // red, flag are free again
+  } else if (warp == 9) {
+    // ---------------------------------------------------------- products
+    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (elect_one()) {
+      const uint32_t idesc_s = make_idesc_bf16(128, kRowsKT);
+      const uint32_t idesc_o = make_idesc_bf16(128, 64) | (1u << 16);  // B (V) read dims-major
+      const uint64_t dq = make_sdesc_sw128(smem_u32(smem)), dk = make_sdesc_sw128(smem_u32(kv0)),
+                     dv = make_sdesc_sw128(smem_u32(kv0 + C::kSide));
+      int ks = 0, vs = 0;
+      uint32_t kp = 0, tp = 0, op = 0;  // parity of the stage; bit t: parities of S_t and P_t (a tile may sit out)
+      for (int sn = 0; !bad; ++sn) {
+        const int sb = sn & 1;
+        bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+        if (bad || segs[sb].nrows < 0) break;
+        const int nt = segs[sb].ntile, tiles = segs[sb].ntok > tq1 ? 2 : 1;
+        bad = !mbar_wait(qfull, (uint32_t)sn & 1u, p.err, kErrTimeoutFull);
+        auto issue_s = [&](int t, bool last) {
+          if (!bad) bad = !mbar_wait(&sfree[t], (tp >> t & 1u) ^ 1u, p.err, kErrTimeoutAccum);  // S_t has been read
+          tp ^= 1u << t;
+          tc_fence_after();
+          const uint64_t a = dq + t * (128 * 128 >> 4), b = dk + (uint32_t)ks * (2 * C::kSide >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) tc_mma_ss(tmem + t * 128, a + 2 * kk, b + 2 * kk, idesc_s, kk > 0 ? 1u : 0u);
+          tc_commit(&sfull[t]);
+          if (last && t == tiles - 1) tc_commit(qempty);
+        };
+        auto next_k = [&]() {
+          if (++ks == NS) {
+            ks = 0;
+            kp ^= 1u;
+          }
+        };
+        if (nt == 0) mbar_arrive(qempty);
+        if (nt > 0) {
+          if (!bad) bad = !mbar_wait(&kvfull[ks], kp, p.err, kErrTimeoutFull);
+          for (int t = 0; t < tiles; ++t) issue_s(t, nt == 1);
+          next_k();
+        }
+        for (int i = 0; i < nt; ++i) {
+          const bool more = i + 1 < nt;
+          if (more && !bad) bad = !mbar_wait(&kvfull[ks], kp, p.err, kErrTimeoutFull);
+          for (int t = 0; t < tiles; ++t) {
+            if (more) issue_s(t, i + 2 == nt);
+            if (!bad) bad = !mbar_wait(&pfull[t], op >> t & 1u, p.err, kErrTimeoutAccum);
+            op ^= 1u << t;
+            tc_fence_after();
+            const uint64_t b = dv + (uint32_t)vs * (2 * C::kSide >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              tc_mma_ts(tmem + kColO + 64 * t, tmem + kColP + 64 * t + kk * 8, b + 128 * kk, idesc_o,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+            tc_commit(&ofull[t]);
+          }
+          tc_commit(&kvempty[vs]);
+          if (more) next_k();
+          if (++vs == NS) vs = 0;
+        }
+        mbar_arrive(&seg_empty[sb]);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 12) {
+    // ------------------------------------------- 8-bit tiles to bf16 tiles
+    if (F8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+      const int tid = threadIdx.x & 127;
+      for (int sn = 0;; ++sn) {
+        const int sb = sn & 1;
+        if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+        if (bad || segs[sb].nrows < 0) break;
+        const int nt = segs[sb].ntile;
+        const int32_t j0 = segs[sb].j0, lo = segs[sb].lo, hi = segs[sb].hi;
+        for (int i = 0; i < nt; ++i, ++it) {
+          const int rs = it & 1, st = it % NS;
+          if (!bad) bad = !mbar_wait(&rawfull[rs], (uint32_t)(it >> 1) & 1u, p.err, kErrTimeoutFull);
+          if (!bad) bad = !mbar_wait(&kvempty[st], ((uint32_t)(it / NS) & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
+          const uint8_t* raw = smem + C::kOffRaw + rs * 2 * C::kRawSide;
+          const uint8_t* codes = smem + C::kOffCodes + rs * 2 * kRowsKT;
+          uint8_t* dst = kv0 + st * 2 * C::kSide;
+#pragma unroll
+          for (int side = 0; side < 2; ++side)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              // 4 threads a key, 16 values each
+              const int idx = x * 128 + tid, key = idx >> 2, c = idx & 3;
+              const int32_t j = j0 + i * kRowsKT + key;
+              uint32_t o[8];
+              // a key nobody may see: zeros, whatever its page (or an earlier tile) holds
+              if (j >= lo && j < hi) {
+                const uint4 w = *(const uint4*)(raw + side * C::kRawSide + idx * 16);
+                const uint32_t mul = ch_code_mul(codes[side * kRowsKT + key]);
+                ch_e4m3_to_bf16(w.x, mul, o[0], o[1]);
+                ch_e4m3_to_bf16(w.y, mul, o[2], o[3]);
+                ch_e4m3_to_bf16(w.z, mul, o[4], o[5]);
+                ch_e4m3_to_bf16(w.w, mul, o[6], o[7]);
+              } else {
+#pragma unroll
+                for (int y = 0; y < 8; ++y) o[y] = 0u;
+              }
+              uint8_t* row = dst + side * C::kSide + key * 128;
+              *(uint4*)(row + (((2 * c) ^ (key & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *(uint4*)(row + (((2 * c + 1) ^ (key & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&kvfull[st]);
+            mbar_arrive(&rawempty[rs]);
+          }
+        }
+        if (lane == 0) mbar_arrive(&seg_empty[sb]);
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 10) {
+    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  } else {
+    // ----------------------------------------------------------- softmax
+    if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row = TMEM lane
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lane_base + (uint32_t)t * 128;
+    const uint32_t o_col = tmem + lane_base + kColO + 64 * t;
+    const uint32_t p_col = tmem + lane_base + kColP + 64 * t;
+    const int tok_r = row / p.G;  // token of the row within the tile
+    uint32_t par = 0;             // parity of the tile's products
+    for (int sn = 0;; ++sn) {
+      const int sb = sn & 1;
+      if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+      bad = ch_named_or(6, 256, bad);  // all eight warps leave together
+      const ChunkSeg& sg = segs[sb];
+      if (sg.nrows < 0 || bad) break;
+      const int ntile = sg.ntile, ntok = sg.ntok;
+      const bool tile_on = t == 0 || ntok > tq1;
+      const int tok = t * tq1 + tok_r;
+      const bool row_ok = tok_r < tq1 && tok < ntok;
+      const bool warp_on = __any_sync(0xffffffffu, row_ok);
+      const int32_t lo = sg.lo, hi = sg.hi;
+      const int32_t pos = row_ok ? sg.first_pos + tok : -1;
+      const int32_t tile_first = sg.first_pos + t * tq1, tile_last = sg.first_pos + min(ntok, (t + 1) * tq1) - 1;
+      float m_ref = -INFINITY, l = 0.f;
+      if (tile_on) {
+        for (int i = 0; i < ntile; ++i) {
+          const int32_t j0 = sg.j0 + i * kRowsKT;
+          if (!F8 && t == 0 && (j0 < lo || j0 + kRowsKT > hi)) {
+            // keys nobody may see: 0 times what their V rows (or an earlier tile) hold must be 0; both tiles' products
+            // with V come after this tile's warps have arrived
+            const int st = (it + i) % NS;
+            if (!bad) bad = !mbar_wait(&kvfull[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
+            if (j0 + row < lo || j0 + row >= hi) {
+              uint8_t* vr = kv0 + st * 2 * C::kSide + C::kSide + row * 128;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) *(uint4*)(vr + c * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          if (!bad) bad = !mbar_wait(&sfull[t], par, p.err, kErrTimeoutAccum);
+          tc_fence_after();
+          if (!warp_on) {  // no row of this warp is in use
+            tc_fence_before();
+            if (lane == 0) {
+              mbar_arrive(&sfree[t]);
+              mbar_arrive(&pfull[t]);
+            }
+            par ^= 1u;
+            continue;
+          }
+          const bool whole = j0 + kRowsKT - 1 <= tile_first && j0 >= lo && (p.window <= 0 || j0 > tile_last - p.window);
+          auto masked = [&](uint32_t bits, int e) -> uint32_t {
+            const int32_t kj = j0 + e;
+            const bool vis = kj <= pos && (p.window <= 0 || kj > pos - p.window);
+            return vis ? bits : __float_as_uint(-INFINITY);
+          };
+          // pass 1: the row's largest raw score (scale2 > 0)
+          float mx = -INFINITY;
+#pragma unroll
+          for (int hb = 0; hb < 2; ++hb) {
+            uint32_t r[64];
+            ch_ld32(s_col + 64 * hb, r);
+            ch_ld32(s_col + 64 * hb + 32, r + 32);
+            tmem_ld_wait();
+            if (whole) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(masked(r[e], 64 * hb + e)));
+            }
+          }
+          const float mxs = mx * p.scale2;
+          const bool move = mxs > m_ref + 8.0f;
+          const float m_new = move ? mxs : m_ref;
+          const float c = move ? ch_exp2(m_ref - m_new) : 1.0f;
+          const float m_eff = m_new == -INFINITY ? 0.f : m_new;  // nothing seen so far: every P is 0
+          // P_t and O_t are free once the products of the tile before are done
+          if (i > 0) {
+            if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
+            tc_fence_after();
+          }
+          const ch_f2 sc2 = ch_pair(p.scale2, p.scale2), nm2 = ch_pair(-m_eff, -m_eff);
+          ch_f2 sum2 = 0ull;
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            uint32_t r[32], pk[16];
+            ch_ld32(s_col + 32 * q4, r);
+            tmem_ld_wait();
+            if (!whole) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) r[e] = masked(r[e], 32 * q4 + e);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const ch_f2 x = ch_fma2(((ch_f2)r[2 * e + 1] << 32) | r[2 * e], sc2, nm2);
+              const float p0 = ch_exp2(ch_lo(x)), p1 = ch_exp2(ch_hi(x));
+              sum2 = ch_add2(sum2, ch_pair(p0, p1));
+              pk[e] = ch_bf16x2(p0, p1);
+            }
+            ch_st16(p_col + 16 * q4, pk);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sfree[t]);  // S_t has been read
+          l = l * c + ch_lo(sum2) + ch_hi(sum2);
+          m_ref = m_new;
+          if (i > 0 && __any_sync(0xffffffffu, move)) {
+            // O_t of the tiles before, before this one's product adds to it
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              uint32_t ov[32];
+              tmem_ld_x32(o_col + 32 * hf, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int d = 0; d < 32; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * c);
+              tmem_st_x32(o_col + 32 * hf, ov);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[t]);
+          par ^= 1u;
+        }
+      }
+      it += ntile;
+      // ------------------------------------------------- end of a part
+      const int slot = sg.slot;
+      uint32_t ov[64];
+      if (tile_on && ntile > 0) {
+        if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
+        tc_fence_after();
+        ch_ld32(o_col, ov);
+        ch_ld32(o_col + 32, ov + 32);
+        tmem_ld_wait();
+        tc_fence_before();
+      } else {
+#pragma unroll
+        for (int d = 0; d < 64; ++d) ov[d] = 0u;
+      }
+      if (row_ok) {
+        const int hh = row - tok_r * p.G;
+        if (slot >= 0) {
+          const int64_t prow = (int64_t)slot * 256 + tok * p.G + hh;
+          *(float2*)(p.part_ml + prow * 2) = make_float2(m_ref, l);
+#pragma unroll
+          for (int d = 0; d < 16; ++d)
+            *(uint4*)(p.part_o + prow * kChunkD + 4 * d) = make_uint4(ov[4 * d], ov[4 * d + 1], ov[4 * d + 2], ov[4 * d + 3]);
+        } else {
+          const int h = sg.hg * p.G + hh;
+          const int64_t tg = sg.tok0 + tok;
+          if (p.lse) p.lse[tg * p.Hq + h] = m_ref + log2f(l);
+          const float inv = ch_norm(p, h, l, m_ref);
+          uint4* orow = (uint4*)(p.o + (tg * p.Hq + h) * kChunkD);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              w[y] = ch_bf16x2(__uint_as_float(ov[8 * d + 2 * y]) * inv, __uint_as_float(ov[8 * d + 2 * y + 1]) * inv);
+            orow[d] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (slot >= 0) {
+        __threadfence();
+        ch_named_sync(5, 256);
+        if (threadIdx.x == 0) {
+          const uint32_t old = atomicAdd(&p.counters[sg.c0], 1u);
+          const uint32_t last = old == (uint32_t)(sg.c1 - sg.c0);
+          if (last) p.counters[sg.c0] = 0u;
+          *flag = last;
+        }
+        ch_named_sync(6, 256);
+        if (*flag) {
+          __threadfence();
+          chunk_join(p, sg, 1, 256, threadIdx.x, 256);
+        }
+        ch_named_sync(5, 256);  // flag is free again
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[sb]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -497,51 +1286,76 @@ __global__ void __launch_bounds__(kRowsThreads, RT == 1 ? 4 : RT == 2 ? 3 : 2)
 // --------------------------------------------------------------- launch --
 namespace {
 
-constexpr int kChunkMaxCtasPerSm = 8;
+constexpr int kChunkSlotRows = 256;  // the most rows of a partial result
 
-struct Occupancy {
-  std::atomic<int> per_dev[kMaxAttrDevices] = {};
-};
-// Resident CTAs per SM of a kernel, asked once per device.
-int ctas_per_sm(Occupancy& c, const void* f, int threads, int smem) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxAttrDevices) dev = 0;
-  int n = c.per_dev[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, f, threads, (size_t)smem) != cudaSuccess || n < 1) {
-      (void)cudaGetLastError();
-      n = 1;
-    }
-    n = n > kChunkMaxCtasPerSm ? kChunkMaxCtasPerSm : n;
-    c.per_dev[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
+// The line of key tiles is counted in 31 bits.
+bool chunk_fits(const ChunkParams& p, int kt) {
+  const int64_t span = p.window > 0 ? (int64_t)p.window + p.TQ : (int64_t)p.tstride * kChunkPage;
+  return (p.T / p.TQ + p.N) * p.HG * (span / kt + 2) < (1ll << 31);
 }
 
-template <bool F8, int RT>
-int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, ChunkParams p, float* parts, int64_t max_slots,
-                cudaStream_t s) {
-  using C = RowsCfg<F8, RT>;
+template <bool F8, int N_>
+int launch_keys(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
+  using C = KeysCfg<F8, N_>;
   static FuncSmemAttr attr;
-  static Occupancy occ;
-  const void* f = (const void*)chunk_rows_kernel<F8, RT>;
-  ensure_dyn_smem(attr, f, C::kAlloc);
-  const int64_t most = min64((int64_t)device_sm_count() * ctas_per_sm(occ, f, kRowsThreads, C::kAlloc), max_slots);
-  p.TQ = C::kRows / p.G;
-  p.min_tiles = 2;
-  p.part_o = parts;
-  p.part_ml = parts + 2 * most * C::kRows * kChunkD;
-  chunk_rows_kernel<F8, RT><<<(unsigned)most, kRowsThreads, C::kAlloc, s>>>(tk, tv, p);
+  ensure_dyn_smem(attr, (const void*)chunk_keys_kernel<F8, N_>, C::kAlloc);
+  const int grid = device_sm_count();
+  const int HB = p.Hkv % 2 ? 1 : 2;  // with an odd number of kv heads one stream idles
+  p.TQ = N_ / p.G;
+  p.HG = p.Hkv / HB;
+  p.lg_kt = 7;
+  if (!chunk_fits(p, kKeysKT)) return -12;
+  p.part_ml = p.part_o + (int64_t)2 * grid * HB * N_ * kChunkD;
+  CUtensorMap tk, tv;
+  const uint64_t rb = C::kRowBytes, tok = (uint64_t)p.Hkv * rb;
+  const CUtensorMapDataType dt = F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // [values of a row, 8 rows, rows of a token, half pages]: a box is a page's 16 tokens in groups of 8; a row is a
+  // head's values, or in 8 bits a pair of heads'
+  const bool pair = F8 && HB == 2;
+  const uint64_t width = pair ? 128 : 64;
+  const uint64_t dims[4] = {width, 8, (uint64_t)(pair ? p.Hkv / 2 : p.Hkv), (uint64_t)p.pool_pages * 2};
+  const uint64_t strides[3] = {tok, pair ? 128 : rb, tok * 8};
+  const uint32_t box[4] = {(uint32_t)width, 8, (uint32_t)(pair ? 1 : HB), 2};
+  const CUtensorMapSwizzle sw = F8 && !pair ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  if (make_tmap_4d(&tk, k, dt, dims, strides, box, sw) || make_tmap_4d(&tv, v, dt, dims, strides, box, sw)) return -2;
+  chunk_keys_kernel<F8, N_><<<(unsigned)grid, kKeysThreads, C::kAlloc, s>>>(tk, tv, p, HB);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+template <bool F8>
+int launch_rows(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
+  using C = RowsCfg<F8>;
+  static FuncSmemAttr attr;
+  ensure_dyn_smem(attr, (const void*)chunk_rows_kernel<F8>, C::kAlloc);
+  const int grid = device_sm_count();
+  const int tq1 = 128 / p.G;
+  p.TQ = 2 * tq1;
+  p.HG = p.Hkv;
+  p.lg_kt = 7;
+  if (!chunk_fits(p, kRowsKT)) return -12;
+  p.part_ml = p.part_o + (int64_t)2 * grid * 256 * kChunkD;
+  CUtensorMap tq, tk, tv;
+  const uint64_t rb = F8 ? 64 : 128, tok = (uint64_t)p.Hkv * rb;
+  const uint64_t dq[3] = {64, (uint64_t)p.Hq, (uint64_t)p.T}, sq[2] = {128, (uint64_t)p.q_stride * 2};
+  const uint32_t bq[3] = {64, (uint32_t)p.G, (uint32_t)tq1};
+  const uint64_t dk[3] = {64, (uint64_t)p.Hkv, (uint64_t)p.pool_pages * kChunkPage}, sk[2] = {rb, tok};
+  const uint32_t bk[3] = {64, 1, kChunkPage};
+  const CUtensorMapDataType dt = F8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle sw = F8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+  if (make_tmap_3d(&tq, p.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dq, sq, bq, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      make_tmap_3d(&tk, k, dt, dk, sk, bk, sw) || make_tmap_3d(&tv, v, dt, dk, sk, bk, sw))
+    return -2;
+  chunk_rows_kernel<F8><<<(unsigned)grid, C::kThreads, C::kAlloc, s>>>(tq, tk, tv, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace
 
 // Workspace: 256 bytes (word 0: the error flags), a counter per CTA, then two
-// partial results (rows x 66 floats) per CTA.
-static int64_t chunk_max_ctas() { return (int64_t)device_sm_count() * kChunkMaxCtasPerSm; }
+// partial results per CTA (rows of 64 values, a maximum and a sum).
+static int64_t chunk_parts_at() { return 256 + ((int64_t)device_sm_count() * 4 + 255) / 256 * 256; }
 int64_t chunk_workspace_bytes() {
-  return 256 + (chunk_max_ctas() * 4 + 255) / 256 * 256 + chunk_max_ctas() * 2 * 64 * (kChunkD + 2) * 4;
+  return chunk_parts_at() + (int64_t)device_sm_count() * 2 * kChunkSlotRows * (kChunkD + 2) * 4;
 }
 
 int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, int32_t max_q, void* workspace,
@@ -549,23 +1363,14 @@ int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, i
   if (p.N <= 0 || p.T <= 0) return 0;
   p.err = (uint32_t*)workspace;
   p.counters = (uint32_t*)((uint8_t*)workspace + 256);
-  float* parts = (float*)((uint8_t*)workspace + 256 + (chunk_max_ctas() * 4 + 255) / 256 * 256);
-  CUtensorMap tk, tv;
-  const uint64_t rb = f8 ? 64 : 128;
-  const uint64_t dk[3] = {64, (uint64_t)p.Hkv, (uint64_t)p.pool_pages * kChunkPage};
-  const uint64_t sk[2] = {rb, (uint64_t)p.Hkv * rb};
-  const uint32_t box[3] = {64, 1, kChunkPage};
-  const CUtensorMapDataType dt = f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUtensorMapSwizzle sw = f8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-  if (make_tmap_3d(&tk, k, dt, dk, sk, box, sw) || make_tmap_3d(&tv, v, dt, dk, sk, box, sw)) return -2;
+  p.part_o = (float*)((uint8_t*)workspace + chunk_parts_at());
   const int64_t rows = (int64_t)max_q * p.G;
-  const int64_t m = chunk_max_ctas();
-  // the smallest tile that holds the longest chunk's rows; longer chunks go in groups of tokens
-  if (rows <= 16 && p.G <= 16)
-    return f8 ? launch_rows<true, 1>(tk, tv, p, parts, m, s) : launch_rows<false, 1>(tk, tv, p, parts, m, s);
-  if (rows <= 32 && p.G <= 32)
-    return f8 ? launch_rows<true, 2>(tk, tv, p, parts, m, s) : launch_rows<false, 2>(tk, tv, p, parts, m, s);
-  return f8 ? launch_rows<true, 4>(tk, tv, p, parts, m, s) : launch_rows<false, 4>(tk, tv, p, parts, m, s);
+  // the smallest tile that holds the longest chunk's rows
+  if (rows <= 16 && p.G <= 16) return f8 ? launch_keys<true, 16>(k, v, p, s) : launch_keys<false, 16>(k, v, p, s);
+  if (rows <= 32 && p.G <= 32) return f8 ? launch_keys<true, 32>(k, v, p, s) : launch_keys<false, 32>(k, v, p, s);
+  if (rows <= 48 && p.G <= 48) return f8 ? launch_keys<true, 48>(k, v, p, s) : launch_keys<false, 48>(k, v, p, s);
+  if (rows <= 64) return f8 ? launch_keys<true, 64>(k, v, p, s) : launch_keys<false, 64>(k, v, p, s);
+  return f8 ? launch_rows<true>(k, v, p, s) : launch_rows<false>(k, v, p, s);
 }
 
 }  // namespace gptoss

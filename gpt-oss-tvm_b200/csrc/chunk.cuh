@@ -42,7 +42,9 @@ struct ChunkParams {
   uint32_t* counters;  // [grid], zero between launches
   float* part_o;       // [2 * grid][rows][64]
   float* part_ml;      // [2 * grid][rows][2]
-  int32_t min_tiles;   // key tiles below which a part is not worth a CTA
+  int32_t HG;          // groups of kv heads: units per group of tokens
+  int32_t lg_kt;       // log2 of the keys of a tile
+  int32_t stages;      // ring stages
 };
 
 struct ChunkSeq {
@@ -64,133 +66,156 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int b) {
     kl = 0;  // no such sequence: nothing to see
     s.row = 0;
   }
+  // a full-causal sequence has no keys beyond its table row's pages (a window's ring may have gone round)
+  if (p.window <= 0) kl = (int32_t)min64(kl, (int64_t)p.tstride * kChunkPage);
   s.off = kl - s.ql;
   return s;
 }
 
 // Keys [lo, hi) that some token of group t may see, and the key tiles over them.
-template <int KT>
 __device__ __forceinline__ int chunk_tiles(const ChunkParams& p, const ChunkSeq& s, int t, int32_t& lo, int32_t& hi) {
   const int32_t t0 = t * p.TQ, t1 = min(s.ql, t0 + p.TQ);
   hi = max(0, s.off + t1);
   lo = p.window > 0 ? min(hi, max(0, s.off + t0 - p.window + 1)) : 0;
-  return hi > lo ? (hi + KT - 1) / KT - lo / KT : 0;
+  return hi > lo ? ((hi - 1) >> p.lg_kt) + 1 - (lo >> p.lg_kt) : 0;
 }
 
-// A part of a unit for one CTA.
+// A part of a unit for one CTA, as the loading warp hands it to the others.
 struct ChunkSeg {
-  ChunkSeq s;
-  int32_t t, hk;
-  int32_t lo, hi;    // keys
-  int32_t k0;        // first key of tile 0 (lo rounded down)
-  int32_t n;         // key tiles of the unit (0: nothing to see, one empty step)
-  int32_t i0, i1;    // this CTA's key tiles
-  int32_t slot;      // -1: the whole unit; else where the partial result goes
-  int32_t c0, c1;    // CTAs that share the unit
+  int64_t tok0;        // first token (row of q)
+  int32_t nrows;       // rows in use: tokens * G; -1: no more parts
+  int32_t first_pos;   // position of the first token
+  int32_t ntok;
+  int32_t hg;          // group of kv heads
+  int32_t lo, hi;      // keys some row may see
+  int32_t j0;          // first key of the part's first tile
+  int32_t ntile;       // key tiles of the part (0: a unit that sees nothing)
+  int32_t slot;        // -1: the whole unit; else where the partial result goes
+  int32_t c0, c1;      // CTAs that share the unit
   int32_t first_slot;  // slot of CTA c0's part (the others': 2 c)
+  int32_t row;         // page-table row
 };
 
-// The walk of one CTA over its part of the line.  `pre` is shared memory for
-// kChunkMaxSeqs + 1 prefix sums; init() is called by all threads of the block
-// (a multiple of 32) with a __syncthreads inside; next() by any thread, each
-// with its own walk.
-template <int KT>
+// Prefix sums of the sequences' key tiles (times head groups) in `pre`
+// [kChunkMaxSeqs + 1], shared memory; all `nthreads` threads of the block.
+// The host has made sure that the total fits 31 bits.
+__device__ __forceinline__ void chunk_plan(const ChunkParams& p, int32_t* pre, int nthreads) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = nthreads >> 5;
+  for (int b = warp; b < p.N; b += nw) {
+    const ChunkSeq s = chunk_seq(p, b);
+    const int nt = (s.ql + p.TQ - 1) / p.TQ;
+    int32_t w = 0;
+    for (int t = lane; t < nt; t += 32) {
+      int32_t lo, hi;
+      w += max(1, chunk_tiles(p, s, t, lo, hi));
+    }
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (lane == 0) pre[b + 1] = w * p.HG;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int32_t run = 0;
+    for (int b0 = 0; b0 < p.N; b0 += 32) {
+      int32_t v = b0 + lane < p.N ? pre[b0 + lane + 1] : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (b0 + lane < p.N) pre[b0 + lane + 1] = run + v;
+      run += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+  __syncthreads();
+}
+
+// The walk of one CTA over its part of the line (one warp, all lanes alike).
 struct ChunkWalk {
-  int64_t pos, end, total, ubase;
-  int32_t b, t, hk, g, cta;
+  int32_t pos, end, total, ubase;
+  int32_t b, t, hg, g, cta, per, rem;
   ChunkSeq s;
   int32_t lo, hi, n;
 
-  __device__ __forceinline__ static void plan(const ChunkParams& p, int64_t* pre, int nthreads) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = nthreads >> 5;
-    for (int b = warp; b < p.N; b += nw) {
-      const ChunkSeq s = chunk_seq(p, b);
-      const int nt = (s.ql + p.TQ - 1) / p.TQ;
-      int64_t w = 0;
-      for (int t = lane; t < nt; t += 32) {
-        int32_t lo, hi;
-        w += max(1, chunk_tiles<KT>(p, s, t, lo, hi));
-      }
-      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-      if (lane == 0) pre[b + 1] = w * p.Hkv;
-    }
-    __syncthreads();
-    if (warp == 0) {
-      int64_t run = 0;
-      for (int b0 = 0; b0 < p.N; b0 += 32) {
-        int64_t v = b0 + lane < p.N ? pre[b0 + lane + 1] : 0;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-          if (lane >= o) v += u;
-        }
-        if (b0 + lane < p.N) pre[b0 + lane + 1] = run + v;
-        run += __shfl_sync(0xffffffffu, v, 31);
-      }
-      if (lane == 0) pre[0] = 0;
-    }
-    __syncthreads();
+  // CTA c takes tiles cut(c) .. cut(c + 1) - 1: `per` of them, the first `rem` CTAs one more
+  __device__ __forceinline__ int32_t cut(int c) const { return c * per + min(c, rem); }
+  __device__ __forceinline__ int owner(int32_t x) const {
+    const int32_t big = rem * (per + 1);
+    return x < big ? (int)((uint32_t)x / (uint32_t)(per + 1)) : rem + (int)((uint32_t)(x - big) / (uint32_t)per);
   }
 
-  __device__ __forceinline__ int64_t cut(int c) const { return total * c / g; }
-  __device__ __forceinline__ int owner(int64_t x) const { return (int)(((x + 1) * g - 1) / total); }
-
-  __device__ __forceinline__ void begin(const ChunkParams& p, const int64_t* pre, int grid, int cta_) {
+  __device__ __forceinline__ void begin(const ChunkParams& p, const int32_t* pre, int grid, int cta_) {
+    const int lane = threadIdx.x & 31;
     cta = cta_;
     total = pre[p.N];
-    g = (int)max64(1, min64(grid, (total + p.min_tiles - 1) / p.min_tiles));
+    g = max(1, min(grid, total));
+    per = (int32_t)((uint32_t)total / (uint32_t)g);
+    rem = total - per * g;
     pos = end = 0;
     if (total == 0 || cta >= g) return;
     pos = cut(cta);
     end = cut(cta + 1);
-    int a = 0, z = p.N - 1;  // the last b with pre[b] <= pos and pre[b + 1] > pos
+    int a = 0, z = p.N - 1;  // the last b with pre[b] <= pos: it has tiles, since pre[b + 1] > pos
     while (a < z) {
       const int mid = (a + z + 1) >> 1;
       if (pre[mid] <= pos) a = mid;
       else z = mid - 1;
     }
     b = a;
-    while (pre[b + 1] <= pos) ++b;
     s = chunk_seq(p, b);
+    // the group of tokens that holds pos: 32 groups at a time
     ubase = pre[b];
-    t = 0;
-    for (;; ++t) {
-      n = chunk_tiles<KT>(p, s, t, lo, hi);
-      const int64_t w = (int64_t)max(1, n) * p.Hkv;
-      if (ubase + w > pos) break;
-      ubase += w;
+    for (t = 0;; t += 32) {
+      int32_t l_, h_;
+      const int nt = (s.ql + p.TQ - 1) / p.TQ;
+      int32_t w = t + lane < nt ? max(1, chunk_tiles(p, s, t + lane, l_, h_)) * p.HG : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t u = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += u;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, ubase + w > pos);
+      if (past) {
+        const int k = __ffs(past) - 1;
+        if (k > 0) ubase += __shfl_sync(0xffffffffu, w, k - 1);
+        t += k;
+        break;
+      }
+      ubase += __shfl_sync(0xffffffffu, w, 31);
+      if (t + 32 >= nt) break;  // not reached: pos lies in this sequence
     }
-    hk = (int)((pos - ubase) / max(1, n));
-    ubase += (int64_t)hk * max(1, n);
+    n = chunk_tiles(p, s, t, lo, hi);
+    hg = (int)((uint32_t)(pos - ubase) / (uint32_t)max(1, n));
+    ubase += hg * max(1, n);
   }
 
-  // The next segment; false at the end of the part.
+  // The next part; false at the end.
   __device__ __forceinline__ bool next(const ChunkParams& p, ChunkSeg& x) {
     if (pos >= end) return false;
     const int32_t c = max(1, n);
-    const int64_t uend = ubase + c;
-    x.s = s;
-    x.t = t;
-    x.hk = hk;
+    const int32_t uend = ubase + c;
+    const int32_t i0 = pos - ubase, i1 = min(c, end - ubase);
+    x.tok0 = s.q0 + (int64_t)t * p.TQ;
+    x.ntok = min(p.TQ, s.ql - t * p.TQ);
+    x.nrows = x.ntok * p.G;
+    x.first_pos = s.off + t * p.TQ;
+    x.hg = hg;
     x.lo = lo;
     x.hi = hi;
-    x.k0 = lo / KT * KT;
-    x.n = n;
-    x.i0 = (int32_t)(pos - ubase);
-    x.i1 = (int32_t)min64(c, end - ubase);
+    x.j0 = ((lo >> p.lg_kt) + i0) << p.lg_kt;
+    x.ntile = n == 0 ? 0 : i1 - i0;
+    x.row = s.row;
     x.slot = -1;
-    if (x.i0 > 0 || x.i1 < c) {
-      const bool first = pos == cut(cta);
-      x.slot = 2 * cta + (first ? 0 : 1);
+    x.c0 = x.c1 = x.first_slot = 0;
+    if (i0 > 0 || i1 < c) {
+      x.slot = 2 * cta + (pos == cut(cta) ? 0 : 1);
       x.c0 = owner(ubase);
       x.c1 = owner(uend - 1);
       x.first_slot = cut(x.c0) == ubase ? 2 * x.c0 : 2 * x.c0 + 1;
     }
-    pos = min64(end, uend);
+    pos = min(end, uend);
     if (pos >= end) return true;
-    // on to the next unit
     ubase = uend;
-    if (++hk == p.Hkv) {
-      hk = 0;
+    if (++hg == p.HG) {
+      hg = 0;
       if (++t * p.TQ >= s.ql) {
         t = 0;
         do {
@@ -198,7 +223,7 @@ struct ChunkWalk {
           s = chunk_seq(p, b);
         } while (s.ql == 0);
       }
-      n = chunk_tiles<KT>(p, s, t, lo, hi);
+      n = chunk_tiles(p, s, t, lo, hi);
     }
     return true;
   }
