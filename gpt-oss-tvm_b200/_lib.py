@@ -81,7 +81,7 @@ SIGNATURES = {
                                                  _P]),
     "gptoss_kv_pages_copy_f8": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _P, _I32, _I32, _I64, _I64, _P, _P,
                                                _I32, _P]),
-    "gptoss_verify_drafts_scratch_bytes": (_I64, [_I64]),
+    "gptoss_verify_drafts_scratch_bytes": (_I64, [_I64, _I64]),
     "gptoss_verify_drafts": (ctypes.c_int, [_P, _I32, _I64, _P, _P, _I64, _I32, _I32, ctypes.c_double, _P, _P, _P,
                                             _I64, _P, _I64, _P, _P, _P]),
     "gptoss_moe_plan_tiles": (ctypes.c_int, [_P, _I32, _P, _P, _P]),

@@ -45,45 +45,68 @@ class ChunkWorkspace:
 _workspaces: dict = {}
 
 
-def _workspace(device: torch.device, stream: int) -> ChunkWorkspace:
+def _workspace(index: int, stream: int) -> ChunkWorkspace:
     """The workspace of calls on this device and stream that bring none (a
     program's own, as long as it runs: captured graphs keep using it)."""
-    key = (device.index, stream)
-    ws = _workspaces.get(key)
+    ws = _workspaces.get((index, stream))
     if ws is None:
-        ws = _workspaces[key] = ChunkWorkspace(device)
+        ws = _workspaces[index, stream] = ChunkWorkspace(torch.device("cuda", index))
     return ws
 
 
-def _need(cond: bool, what: str):
-    if not cond:
-        raise ValueError(what)
+def _run(index: int, name: str, *args) -> None:
+    """A library call with the current stream of device `index` as its last argument."""
+    fn, stream = getattr(_lib.load(), name), torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc)
 
 
-def _i32(t, n, name, dev):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
-        raise ValueError(f"{name} must be a dense int32 tensor of {n} entries on {dev}")
+def _bad(what: str):
+    raise ValueError(what)
+
+
+def _i32(t, n, name, index):
+    if (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous()
+            or t.get_device() != index):
+        raise ValueError(f"{name} must be a dense int32 tensor of {n} entries on cuda:{index}")
     return t.data_ptr()
 
 
-def _pools(k_pages, v_pages, k_scale, v_scale, dev):
+def _table(t, index):
+    if t.dtype is not torch.int32 or t.dim() != 2 or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"page_table must be a dense int32 tensor [sequences, pages] on cuda:{index}")
+    return t.data_ptr()
+
+
+def _pools(k_pages, v_pages, k_scale, v_scale, index):
     """Checks a pair of pools; (kv heads, pages, whether 8-bit)."""
-    _need(k_pages.dim() == 3 and k_pages.shape[2] == HEAD_DIM and k_pages.shape[0] % PAGE_SIZE == 0,
-          f"page pools are [pages * {PAGE_SIZE}, kv heads, {HEAD_DIM}], got {tuple(k_pages.shape)}")
-    _need(k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype, "the two pools differ in shape or type")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.device == dev and v_pages.device == dev,
-          f"page pools must be dense and on {dev}")
-    hkv, pages = k_pages.shape[1], k_pages.shape[0] // PAGE_SIZE
-    f8 = k_pages.dtype == _F8
-    if f8:
-        _need(k_scale is not None and v_scale is not None, "8-bit pools need k_scale and v_scale")
+    shape, dt = k_pages.shape, k_pages.dtype
+    if len(shape) != 3 or shape[2] != HEAD_DIM or shape[0] % PAGE_SIZE:
+        _bad(f"page pools are [pages * {PAGE_SIZE}, kv heads, {HEAD_DIM}], got {tuple(shape)}")
+    if v_pages.shape != shape or v_pages.dtype is not dt:
+        _bad("the two pools differ in shape or type")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.get_device() == index
+            and v_pages.get_device() == index):
+        _bad(f"page pools must be dense and on cuda:{index}")
+    hkv, pages = shape[1], shape[0] // PAGE_SIZE
+    if dt is _F8:
+        if k_scale is None or v_scale is None:
+            _bad("8-bit pools need k_scale and v_scale")
+        want = (pages, hkv, PAGE_SIZE)
         for t in (k_scale, v_scale):
-            _need(t.dtype == _E8 and tuple(t.shape) == (pages, hkv, PAGE_SIZE) and t.is_contiguous()
-                  and t.device == dev, f"scales of this pool are dense float8_e8m0fnu [{pages}, {hkv}, {PAGE_SIZE}]")
-    else:
-        _need(k_pages.dtype == _BF16, f"page pools are bfloat16 or float8_e4m3fn, got {k_pages.dtype}")
-        _need(k_scale is None and v_scale is None, "bf16 pools have no scales")
-    return hkv, pages, f8
+            if t.dtype is not _E8 or t.shape != want or not t.is_contiguous() or t.get_device() != index:
+                _bad(f"scales of this pool are dense float8_e8m0fnu {want} on cuda:{index}")
+        return hkv, pages, True
+    if dt is not _BF16:
+        _bad(f"page pools are bfloat16 or float8_e4m3fn, got {dt}")
+    if k_scale is not None or v_scale is not None:
+        _bad("bf16 pools have no scales")
+    return hkv, pages, False
 
 
 def f8_pool(pages: int, kv_heads: int, device="cuda"):
@@ -109,40 +132,40 @@ def attend_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     seq_rows [N]: int32 on the device.  max_q: the longest chunk.  sinks
     [heads] bf16.  Returns o [T, heads, 64] bf16, with return_lse also lse
     [T, heads] fp32 (base 2, without the sink)."""
-    dev = q.device
-    _need(q.is_cuda and q.dtype == _BF16 and q.dim() == 3 and q.shape[2] == HEAD_DIM,
-          f"q must be a CUDA bfloat16 tensor [tokens, heads, {HEAD_DIM}]")
+    if not q.is_cuda or q.dtype is not _BF16 or q.dim() != 3 or q.shape[2] != HEAD_DIM:
+        _bad(f"q must be a CUDA bfloat16 tensor [tokens, heads, {HEAD_DIM}]")
+    index = q.get_device()
     T, Hq, _ = q.shape
     st = q.stride()
-    _need(T == 0 or (st[2] == 1 and st[1] == HEAD_DIM and (T == 1 or (st[0] >= Hq * HEAD_DIM and st[0] % 8 == 0))),
-          "q: heads and values must be dense, tokens a multiple of 8 elements apart")
-    hkv, pages, f8 = _pools(k_pages, v_pages, k_scale, v_scale, dev)
-    _need(Hq % hkv == 0 and Hq // hkv <= 64, f"{Hq} query heads do not fit {hkv} kv heads (at most 64 for each)")
-    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
-          and page_table.device == dev, f"page_table must be a dense int32 tensor [sequences, pages] on {dev}")
+    if T and (st[2] != 1 or st[1] != HEAD_DIM or (T > 1 and (st[0] < Hq * HEAD_DIM or st[0] % 8))):
+        _bad("q: heads and values must be dense, tokens a multiple of 8 elements apart")
+    hkv, pages, f8 = _pools(k_pages, v_pages, k_scale, v_scale, index)
+    if Hq % hkv or Hq // hkv > 64:
+        _bad(f"{Hq} query heads do not fit {hkv} kv heads (a multiple, at most 64 for each)")
+    table_p = _table(page_table, index)
     n = seq_rows.shape[0]
-    rows_p, start_p, len_p = (_i32(seq_rows, n, "seq_rows", dev), _i32(q_start, n + 1, "q_start", dev),
-                              _i32(kv_len, n, "kv_len", dev))
-    _need(sinks is None or (sinks.dtype == _BF16 and tuple(sinks.shape) == (Hq,) and sinks.is_contiguous()
-                            and sinks.device == dev), f"sinks must be a dense bfloat16 tensor [{Hq}] on {dev}")
+    rows_p, start_p, len_p = (_i32(seq_rows, n, "seq_rows", index), _i32(q_start, n + 1, "q_start", index),
+                              _i32(kv_len, n, "kv_len", index))
+    if sinks is not None and (sinks.dtype is not _BF16 or sinks.dim() != 1 or sinks.shape[0] != Hq
+                              or not sinks.is_contiguous() or sinks.get_device() != index):
+        _bad(f"sinks must be a dense bfloat16 tensor [{Hq}] on cuda:{index}")
     if out is None:
-        out = torch.empty(T, Hq, HEAD_DIM, dtype=_BF16, device=dev)
-    else:
-        _need(out.dtype == _BF16 and out.shape == q.shape and out.is_contiguous() and out.device == dev,
-              "out must be a dense bfloat16 tensor of q's shape")
-    lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
+        out = torch.empty((T, Hq, HEAD_DIM), dtype=_BF16, device=q.device)
+    elif out.dtype is not _BF16 or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index:
+        _bad("out must be a dense bfloat16 tensor of q's shape on its device")
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if T and n:
-        with torch.cuda.device(dev):
-            stream = torch.cuda.current_stream().cuda_stream
-            ws = workspace if workspace is not None else _workspace(dev, stream)
-            _need(ws.device.index in (None, dev.index), "the workspace is on another device")
-            _lib.call("gptoss_attn_chunk", q.data_ptr(), st[0] if T > 1 else Hq * HEAD_DIM, k_pages.data_ptr(),
-                      v_pages.data_ptr(), k_scale.data_ptr() if f8 else None, v_scale.data_ptr() if f8 else None,
-                      int(f8), pages, page_table.data_ptr(), page_table.shape[0], page_table.shape[1], rows_p,
-                      start_p, len_p, n, T, int(max_q), Hq, hkv, HEAD_DIM, int(window),
-                      sm_scale if sm_scale is not None else HEAD_DIM ** -0.5,
-                      sinks.data_ptr() if sinks is not None else None, ws.ptr, ws.nbytes, out.data_ptr(),
-                      lse.data_ptr() if return_lse else None, stream)
+        ws = workspace
+        if ws is None:
+            ws = _workspace(index, torch._C._cuda_getCurrentRawStream(index))
+        elif ws.buf.get_device() != index:
+            _bad("the workspace is on another device")
+        _run(index, "gptoss_attn_chunk", q.data_ptr(), st[0] if T > 1 else Hq * HEAD_DIM, k_pages.data_ptr(),
+             v_pages.data_ptr(), k_scale.data_ptr() if f8 else None, v_scale.data_ptr() if f8 else None, f8, pages,
+             table_p, page_table.shape[0], page_table.shape[1], rows_p, start_p, len_p, n, T, max_q, Hq, hkv,
+             HEAD_DIM, window, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
+             sinks.data_ptr() if sinks is not None else None, ws.ptr, ws.nbytes, out.data_ptr(),
+             lse.data_ptr() if return_lse else None)
     return (out, lse) if return_lse else out
 
 
@@ -153,50 +176,52 @@ def rope_append_f8(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tens
     positions [T], and quantises k and v into pool rows slots [T].  inv_freq:
     32 floats on the host (a CPU float32 tensor or a ctypes array).  Returns q
     [T, num_heads, 64] bf16, the bits that the bf16 cache's append gives."""
-    dev = qkv.device
-    hkv, pages, f8 = _pools(k_pages, v_pages, k_scale, v_scale, dev)
-    _need(f8, "rope_append_f8 writes 8-bit pools")
-    T = qkv.shape[0]
-    _need(qkv.is_cuda and qkv.dtype == _BF16 and qkv.is_contiguous()
-          and tuple(qkv.shape) == (T, (num_heads + 2 * hkv) * HEAD_DIM),
-          f"qkv must be a dense CUDA bfloat16 tensor [tokens, {(num_heads + 2 * hkv) * HEAD_DIM}]")
-    pos_p, slot_p = _i32(positions, T, "positions", dev), _i32(slots, T, "slots", dev)
+    if not qkv.is_cuda or qkv.dtype is not _BF16 or qkv.dim() != 2 or not qkv.is_contiguous():
+        _bad("qkv must be a dense CUDA bfloat16 tensor [tokens, (heads + 2 kv heads) * 64]")
+    index, T = qkv.get_device(), qkv.shape[0]
+    hkv, pages, f8 = _pools(k_pages, v_pages, k_scale, v_scale, index)
+    if not f8:
+        _bad("rope_append_f8 writes 8-bit pools")
+    if qkv.shape[1] != (num_heads + 2 * hkv) * HEAD_DIM:
+        _bad(f"qkv must have {(num_heads + 2 * hkv) * HEAD_DIM} columns for {num_heads} heads and {hkv} kv heads")
+    pos_p, slot_p = _i32(positions, T, "positions", index), _i32(slots, T, "slots", index)
     if isinstance(inv_freq, torch.Tensor):
-        _need(inv_freq.device.type == "cpu" and inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
-              and inv_freq.numel() == HEAD_DIM // 2, f"inv_freq must be {HEAD_DIM // 2} float32 values on the CPU")
+        if (inv_freq.is_cuda or inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous()
+                or inv_freq.numel() != HEAD_DIM // 2):
+            _bad(f"inv_freq must be {HEAD_DIM // 2} float32 values on the CPU")
         inv_p = inv_freq.data_ptr()
     else:
-        _need(len(inv_freq) == HEAD_DIM // 2, f"inv_freq must be {HEAD_DIM // 2} values")
+        if len(inv_freq) != HEAD_DIM // 2:
+            _bad(f"inv_freq must be {HEAD_DIM // 2} values")
         inv_p = ctypes.addressof(inv_freq)
     if q_out is None:
-        q_out = torch.empty(T, num_heads, HEAD_DIM, dtype=_BF16, device=dev)
-    else:
-        _need(q_out.dtype == _BF16 and tuple(q_out.shape) == (T, num_heads, HEAD_DIM) and q_out.is_contiguous()
-              and q_out.device == dev, f"q_out must be a dense bfloat16 tensor [{T}, {num_heads}, {HEAD_DIM}]")
+        q_out = torch.empty((T, num_heads, HEAD_DIM), dtype=_BF16, device=qkv.device)
+    elif (q_out.dtype is not _BF16 or q_out.shape != (T, num_heads, HEAD_DIM) or not q_out.is_contiguous()
+          or q_out.get_device() != index):
+        _bad(f"q_out must be a dense bfloat16 tensor [{T}, {num_heads}, {HEAD_DIM}] on cuda:{index}")
     if T:
-        with torch.cuda.device(dev):
-            _lib.call("gptoss_qkv_rope_append_f8", qkv.data_ptr(), pos_p, slot_p, T, pages, num_heads, hkv, HEAD_DIM,
-                      inv_p, concentration, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                      k_scale.data_ptr(), v_scale.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        _run(index, "gptoss_qkv_rope_append_f8", qkv.data_ptr(), pos_p, slot_p, T, pages, num_heads, hkv, HEAD_DIM,
+             inv_p, concentration, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(),
+             v_scale.data_ptr())
     return q_out
 
 
 def _copy_f8(k_pages, v_pages, k_scale, v_scale, page_table, seq, pos0, n, k_rows, v_rows, to_pages):
-    dev = k_pages.device
-    hkv, pages, f8 = _pools(k_pages, v_pages, k_scale, v_scale, dev)
-    _need(f8 and k_pages.is_cuda, "the pools must be 8-bit CUDA pools")
-    _need(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.is_contiguous()
-          and page_table.device == dev, f"page_table must be a dense int32 tensor [sequences, pages] on {dev}")
-    _need(0 <= seq < page_table.shape[0] and pos0 >= 0 and n >= 0, f"no rows {pos0}, {n} of sequence {seq}")
+    if not k_pages.is_cuda or k_pages.dtype is not _F8:
+        _bad("the pools must be 8-bit CUDA pools")
+    index = k_pages.get_device()
+    hkv, pages, _ = _pools(k_pages, v_pages, k_scale, v_scale, index)
+    table_p = _table(page_table, index)
+    if not 0 <= seq < page_table.shape[0] or pos0 < 0 or n < 0:
+        _bad(f"no rows {pos0}, {n} of sequence {seq}")
+    want = (n, hkv, HEAD_DIM)
     for t in (k_rows, v_rows):
-        _need(t.dtype == _BF16 and tuple(t.shape) == (n, hkv, HEAD_DIM) and t.is_contiguous() and t.device == dev,
-              f"rows must be dense bfloat16 tensors [{n}, {hkv}, {HEAD_DIM}] on {dev}")
+        if t.dtype is not _BF16 or t.shape != want or not t.is_contiguous() or t.get_device() != index:
+            _bad(f"rows must be dense bfloat16 tensors {want} on cuda:{index}")
     if n:
-        with torch.cuda.device(dev):
-            _lib.call("gptoss_kv_pages_copy_f8", k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(),
-                      v_scale.data_ptr(), pages, hkv, HEAD_DIM, page_table.data_ptr(), page_table.shape[1], seq, pos0,
-                      n, k_rows.data_ptr(), v_rows.data_ptr(), int(to_pages),
-                      torch.cuda.current_stream().cuda_stream)
+        _run(index, "gptoss_kv_pages_copy_f8", k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(),
+             v_scale.data_ptr(), pages, hkv, HEAD_DIM, table_p, page_table.shape[1], seq, pos0, n, k_rows.data_ptr(),
+             v_rows.data_ptr(), to_pages)
 
 
 def read_pages_f8(k_pages, v_pages, k_scale, v_scale, page_table, seq: int, pos0: int, n: int, k_out=None, v_out=None):

@@ -621,7 +621,9 @@ int gptoss_kv_pages_copy_f8(uint8_t* k_pages, uint8_t* v_pages, uint8_t* k_codes
                       "kv_pages_copy_f8");
 }
 
-int64_t gptoss_verify_drafts_scratch_bytes(int64_t T) { return T > 0 ? verify_scratch_bytes(T) : 64; }
+int64_t gptoss_verify_drafts_scratch_bytes(int64_t T, int64_t V) {
+  return T > 0 && V > 0 ? verify_scratch_bytes(T, V) : 64;
+}
 
 int gptoss_verify_drafts(const void* logits, int32_t logits_bf16, int64_t ld_logits, const int32_t* tokens,
                          const int32_t* row_start, int64_t T, int32_t N, int32_t V, double temperature,
@@ -639,7 +641,7 @@ int gptoss_verify_drafts(const void* logits, int32_t logits_bf16, int64_t ld_log
     return fail(-1, "gptoss_verify_drafts: random numbers are required above temperature 0");
   if (ld_logits < V || (draft_probs && ld_draft < V))
     return fail(-1, "gptoss_verify_drafts: a row stride is smaller than V");
-  if (scratch_bytes < gptoss_verify_drafts_scratch_bytes(T))
+  if (scratch_bytes < gptoss_verify_drafts_scratch_bytes(T, V))
     return fail(-1, "gptoss_verify_drafts: scratch smaller than gptoss_verify_drafts_scratch_bytes()");
   return check_launch(launch_verify(logits, logits_bf16, ld_logits, tokens, row_start, T, N, V, temperature, accept_u,
                                     next_u, draft_probs, ld_draft, scratch, accepted, next_tokens,

@@ -156,7 +156,7 @@ __device__ __forceinline__ float ch_norm(const ChunkParams& p, int h, float l, f
 // `rows` rows each per slot.
 __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg& sg, int heads, int rows, int tid,
                                            int nthreads) {
-  const int c0 = sg.c0, c1 = sg.c1, s0 = sg.first_slot;
+  const int c0 = sg.c0, c1 = sg.c1, s0 = 2 * sg.c0 + 1;
   const int64_t rs = (int64_t)heads * rows;
   for (int x = tid; x < heads * sg.nrows * 16; x += nthreads) {
     const int hr = x >> 4, d = (x & 15) * 4;
@@ -803,8 +803,10 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
 // (P_t bf16 in TMEM), tiles of 128 keys.  The tiles take turns: while one's
 // softmax runs the tensor core works for the other.  Bound by the exponentials:
 // 2 x 128 x 128 of them a key tile at 16 per cycle and SM are 2048 cycles, the
-// products 1024, K and V from L2 32 KB.  The reference of a row moves when a
-// score exceeds it by 8.
+// products 1024, K and V from L2 32 KB.  The reference of a row is the largest
+// score of its first tile; when a later one exceeds it by 8 it moves before the
+// next tile (P and l hold what 2^64 above it gives), so a tile's scores are read
+// once.
 //
 // 8-bit pages: a fourth warpgroup turns a tile's values into bf16 with their
 // power of two (exact) while the one before is used, about 450 issue cycles of
@@ -1110,7 +1112,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
       const int32_t lo = sg.lo, hi = sg.hi;
       const int32_t pos = row_ok ? sg.first_pos + tok : -1;
       const int32_t tile_first = sg.first_pos + t * tq1, tile_last = sg.first_pos + min(ntok, (t + 1) * tq1) - 1;
-      float m_ref = -INFINITY, l = 0.f;
+      float m_ref = -INFINITY, l = 0.f, pend = 1.0f;  // pend: what O_t is still to be multiplied by
       if (tile_on) {
         for (int i = 0; i < ntile; ++i) {
           const int32_t j0 = sg.j0 + i * kRowsKT;
@@ -1138,73 +1140,94 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
             continue;
           }
           const bool whole = j0 + kRowsKT - 1 <= tile_first && j0 >= lo && (p.window <= 0 || j0 > tile_last - p.window);
-          auto masked = [&](uint32_t bits, int e) -> uint32_t {
-            const int32_t kj = j0 + e;
-            const bool vis = kj <= pos && (p.window <= 0 || kj > pos - p.window);
-            return vis ? bits : __float_as_uint(-INFINITY);
-          };
-          // pass 1: the row's largest raw score (scale2 > 0)
-          float mx = -INFINITY;
+          auto masked = [&](uint32_t (&r)[32], int e0) {
 #pragma unroll
-          for (int hb = 0; hb < 2; ++hb) {
-            uint32_t r[64];
-            ch_ld32(s_col + 64 * hb, r);
-            ch_ld32(s_col + 64 * hb + 32, r + 32);
-            tmem_ld_wait();
-            if (whole) {
-#pragma unroll
-              for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 64; ++e) mx = fmaxf(mx, __uint_as_float(masked(r[e], 64 * hb + e)));
+            for (int e = 0; e < 32; ++e) {
+              const int32_t kj = j0 + e0 + e;
+              if (kj > pos || (p.window > 0 && kj <= pos - p.window)) r[e] = __float_as_uint(-INFINITY);
             }
+          };
+          if (__any_sync(0xffffffffu, m_ref == -INFINITY && row_ok)) {
+            // a row without a reference takes the largest score of its first tile (scale2 > 0)
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t r[32];
+              ch_ld32(s_col + 32 * q4, r);
+              tmem_ld_wait();
+              if (!whole) masked(r, 32 * q4);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+            }
+            if (m_ref == -INFINITY) m_ref = mx * p.scale2;  // nothing of it in O or l yet
           }
-          const float mxs = mx * p.scale2;
-          const bool move = mxs > m_ref + 8.0f;
-          const float m_new = move ? mxs : m_ref;
-          const float c = move ? ch_exp2(m_ref - m_new) : 1.0f;
-          const float m_eff = m_new == -INFINITY ? 0.f : m_new;  // nothing seen so far: every P is 0
           // P_t and O_t are free once the products of the tile before are done
           if (i > 0) {
             if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
             tc_fence_after();
           }
-          const ch_f2 sc2 = ch_pair(p.scale2, p.scale2), nm2 = ch_pair(-m_eff, -m_eff);
-          ch_f2 sum2 = 0ull;
+          float sum, mx;
+          for (;;) {
+            // P = 2^(s - m) two at a time, the next 32 scores on their way meanwhile
+            const float m_eff = m_ref == -INFINITY ? 0.f : m_ref;  // nothing seen so far: every P is 0
+            const ch_f2 sc2 = ch_pair(p.scale2, p.scale2), nm2 = ch_pair(-m_eff, -m_eff);
+            ch_f2 sum2 = 0ull;
+            mx = -INFINITY;
+            auto chunk = [&](uint32_t (&r)[32], int e0) {
+              if (!whole) masked(r, e0);
+              uint32_t pk[16];
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint32_t r[32], pk[16];
-            ch_ld32(s_col + 32 * q4, r);
-            tmem_ld_wait();
-            if (!whole) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = masked(r[e], 32 * q4 + e);
+              for (int e = 0; e < 16; ++e) {
+                const ch_f2 x = ch_fma2(((ch_f2)r[2 * e + 1] << 32) | r[2 * e], sc2, nm2);
+                mx = fmaxf(mx, fmaxf(ch_lo(x), ch_hi(x)));
+                const float p0 = ch_exp2(ch_lo(x)), p1 = ch_exp2(ch_hi(x));
+                sum2 = ch_add2(sum2, ch_pair(p0, p1));
+                pk[e] = ch_bf16x2(p0, p1);
+              }
+              ch_st16(p_col + e0 / 2, pk);
+            };
+            uint32_t ra[32], rb[32];
+            ch_ld32(s_col, ra);
+#pragma unroll 1
+            for (int e0 = 0; e0 < 128; e0 += 64) {
+              tmem_ld_wait();
+              ch_ld32(s_col + e0 + 32, rb);
+              chunk(ra, e0);
+              tmem_ld_wait();
+              if (e0 == 0) ch_ld32(s_col + 64, ra);
+              chunk(rb, e0 + 32);
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const ch_f2 x = ch_fma2(((ch_f2)r[2 * e + 1] << 32) | r[2 * e], sc2, nm2);
-              const float p0 = ch_exp2(ch_lo(x)), p1 = ch_exp2(ch_hi(x));
-              sum2 = ch_add2(sum2, ch_pair(p0, p1));
-              pk[e] = ch_bf16x2(p0, p1);
+            sum = ch_lo(sum2) + ch_hi(sum2);
+            // The reference follows a tile later, P and l have room: 2^64.  Beyond that, once more with a new one.
+            if (!__any_sync(0xffffffffu, mx > 64.0f)) break;
+            if (mx > 64.0f) {
+              const float c = ch_exp2(-mx);
+              pend *= c;
+              l *= c;
+              m_ref += mx;
             }
-            ch_st16(p_col + 16 * q4, pk);
           }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sfree[t]);  // S_t has been read
-          l = l * c + ch_lo(sum2) + ch_hi(sum2);
-          m_ref = m_new;
-          if (i > 0 && __any_sync(0xffffffffu, move)) {
+          if (i > 0 && __any_sync(0xffffffffu, pend != 1.0f)) {
             // O_t of the tiles before, before this one's product adds to it
-#pragma unroll
+#pragma unroll 1
             for (int hf = 0; hf < 2; ++hf) {
               uint32_t ov[32];
               tmem_ld_x32(o_col + 32 * hf, ov);
               tmem_ld_wait();
 #pragma unroll
-              for (int d = 0; d < 32; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * c);
+              for (int d = 0; d < 32; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * pend);
               tmem_st_x32(o_col + 32 * hf, ov);
             }
+          }
+          l += sum;
+          pend = 1.0f;
+          if (mx > 8.0f) {
+            pend = ch_exp2(-mx);
+            l *= pend;
+            m_ref += mx;
           }
           tmem_st_wait();
           tc_fence_before();
@@ -1224,6 +1247,8 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
         ch_ld32(o_col + 32, ov + 32);
         tmem_ld_wait();
         tc_fence_before();
+#pragma unroll
+        for (int d = 0; d < 64; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * pend);
       } else {
 #pragma unroll
         for (int d = 0; d < 64; ++d) ov[d] = 0u;
@@ -1291,7 +1316,7 @@ constexpr int kChunkSlotRows = 256;  // the most rows of a partial result
 // The line of key tiles is counted in 31 bits.
 bool chunk_fits(const ChunkParams& p, int kt) {
   const int64_t span = p.window > 0 ? (int64_t)p.window + p.TQ : (int64_t)p.tstride * kChunkPage;
-  return (p.T / p.TQ + p.N) * p.HG * (span / kt + 2) < (1ll << 31);
+  return (p.T / p.TQ + p.N) * p.HG * (span / kt + 2 + p.ov) < (1ll << 31);
 }
 
 template <bool F8, int N_>
@@ -1304,6 +1329,7 @@ int launch_keys(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
   p.TQ = N_ / p.G;
   p.HG = p.Hkv / HB;
   p.lg_kt = 7;
+  p.ov = 3;
   if (!chunk_fits(p, kKeysKT)) return -12;
   p.part_ml = p.part_o + (int64_t)2 * grid * HB * N_ * kChunkD;
   CUtensorMap tk, tv;
@@ -1332,6 +1358,7 @@ int launch_rows(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
   p.TQ = 2 * tq1;
   p.HG = p.Hkv;
   p.lg_kt = 7;
+  p.ov = 3;
   if (!chunk_fits(p, kRowsKT)) return -12;
   p.part_ml = p.part_o + (int64_t)2 * grid * 256 * kChunkD;
   CUtensorMap tq, tk, tv;

@@ -4,14 +4,16 @@
 // A unit is (sequence, group of its new tokens, kv head): the G = Hq / Hkv
 // query heads of the kv head times the tokens of the group are the rows of one
 // tile, so a key is read once for all of them.  A unit's work is its number of
-// key tiles; all units of the batch, one after another, form a line of key
-// tiles that is cut into equal parts, one per CTA, wherever the cut falls (the
-// lengths are only known on the device, and one long context beside many short
-// ones must not leave CTAs idle).  A unit cut between CTAs leaves partial
+// key tiles, plus `ov` for its beginning and end (in key tiles, measured); all
+// units of the batch, one after another, form a line that is cut into equal
+// parts, one per CTA, wherever the cut falls (the lengths are only known on the
+// device, and one long context beside many short ones must not leave CTAs
+// idle).  A unit cut between CTAs leaves partial
 // results (unnormalised output, maximum, sum) in the workspace; whichever CTA
 // finishes last joins them in the order of the keys, so the result does not
-// depend on which one that was.  A CTA has at most two partial results (its
-// first and its last unit), and nobody waits for another CTA.
+// depend on which one that was.  A CTA has at most two partial results (slot
+// 2 c: of a unit that others began; 2 c + 1: of one that it began and others go
+// on with), and nobody waits for another CTA.
 #pragma once
 #include "common.cuh"
 
@@ -44,7 +46,7 @@ struct ChunkParams {
   float* part_ml;      // [2 * grid][rows][2]
   int32_t HG;          // groups of kv heads: units per group of tokens
   int32_t lg_kt;       // log2 of the keys of a tile
-  int32_t stages;      // ring stages
+  int32_t ov;          // a unit's beginning and end, in key tiles
 };
 
 struct ChunkSeq {
@@ -92,7 +94,6 @@ struct ChunkSeg {
   int32_t ntile;       // key tiles of the part (0: a unit that sees nothing)
   int32_t slot;        // -1: the whole unit; else where the partial result goes
   int32_t c0, c1;      // CTAs that share the unit
-  int32_t first_slot;  // slot of CTA c0's part (the others': 2 c)
   int32_t row;         // page-table row
 };
 
@@ -107,7 +108,7 @@ __device__ __forceinline__ void chunk_plan(const ChunkParams& p, int32_t* pre, i
     int32_t w = 0;
     for (int t = lane; t < nt; t += 32) {
       int32_t lo, hi;
-      w += max(1, chunk_tiles(p, s, t, lo, hi));
+      w += max(1, chunk_tiles(p, s, t, lo, hi)) + p.ov;
     }
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     if (lane == 0) pre[b + 1] = w * p.HG;
@@ -167,7 +168,7 @@ struct ChunkWalk {
     for (t = 0;; t += 32) {
       int32_t l_, h_;
       const int nt = (s.ql + p.TQ - 1) / p.TQ;
-      int32_t w = t + lane < nt ? max(1, chunk_tiles(p, s, t + lane, l_, h_)) * p.HG : 0;
+      int32_t w = t + lane < nt ? (max(1, chunk_tiles(p, s, t + lane, l_, h_)) + p.ov) * p.HG : 0;
       for (int o = 1; o < 32; o <<= 1) {
         const int32_t u = __shfl_up_sync(0xffffffffu, w, o);
         if (lane >= o) w += u;
@@ -183,49 +184,52 @@ struct ChunkWalk {
       if (t + 32 >= nt) break;  // not reached: pos lies in this sequence
     }
     n = chunk_tiles(p, s, t, lo, hi);
-    hg = (int)((uint32_t)(pos - ubase) / (uint32_t)max(1, n));
-    ubase += hg * max(1, n);
+    const int32_t c = max(1, n) + p.ov;
+    hg = (int)((uint32_t)(pos - ubase) / (uint32_t)c);
+    ubase += hg * c;
   }
 
-  // The next part; false at the end.
+  // The next part with a key tile (or the one empty step of a unit that sees nothing); false at the end.
   __device__ __forceinline__ bool next(const ChunkParams& p, ChunkSeg& x) {
-    if (pos >= end) return false;
-    const int32_t c = max(1, n);
-    const int32_t uend = ubase + c;
-    const int32_t i0 = pos - ubase, i1 = min(c, end - ubase);
-    x.tok0 = s.q0 + (int64_t)t * p.TQ;
-    x.ntok = min(p.TQ, s.ql - t * p.TQ);
-    x.nrows = x.ntok * p.G;
-    x.first_pos = s.off + t * p.TQ;
-    x.hg = hg;
-    x.lo = lo;
-    x.hi = hi;
-    x.j0 = ((lo >> p.lg_kt) + i0) << p.lg_kt;
-    x.ntile = n == 0 ? 0 : i1 - i0;
-    x.row = s.row;
-    x.slot = -1;
-    x.c0 = x.c1 = x.first_slot = 0;
-    if (i0 > 0 || i1 < c) {
-      x.slot = 2 * cta + (pos == cut(cta) ? 0 : 1);
-      x.c0 = owner(ubase);
-      x.c1 = owner(uend - 1);
-      x.first_slot = cut(x.c0) == ubase ? 2 * x.c0 : 2 * x.c0 + 1;
-    }
-    pos = min(end, uend);
-    if (pos >= end) return true;
-    ubase = uend;
-    if (++hg == p.HG) {
-      hg = 0;
-      if (++t * p.TQ >= s.ql) {
-        t = 0;
-        do {
-          ++b;
-          s = chunk_seq(p, b);
-        } while (s.ql == 0);
+    while (pos < end) {
+      const int32_t c = max(1, n), ub = ubase + p.ov, uend = ub + c;  // the unit's tiles are [ub, uend)
+      const int32_t i0 = max(0, pos - ub), i1 = min(c, end - ub);
+      x.tok0 = s.q0 + (int64_t)t * p.TQ;
+      x.ntok = min(p.TQ, s.ql - t * p.TQ);
+      x.nrows = x.ntok * p.G;
+      x.first_pos = s.off + t * p.TQ;
+      x.hg = hg;
+      x.lo = lo;
+      x.hi = hi;
+      x.j0 = ((lo >> p.lg_kt) + i0) << p.lg_kt;
+      x.ntile = n == 0 ? 0 : i1 - i0;
+      x.row = s.row;
+      x.slot = -1;
+      x.c0 = x.c1 = 0;
+      if (i0 > 0 || i1 < c) {
+        x.slot = 2 * cta + (i0 > 0 ? 0 : 1);
+        x.c0 = owner(ub);
+        x.c1 = owner(uend - 1);
       }
-      n = chunk_tiles(p, s, t, lo, hi);
+      pos = min(end, uend);
+      if (pos < end) {
+        // on to the next unit
+        ubase = uend;
+        if (++hg == p.HG) {
+          hg = 0;
+          if (++t * p.TQ >= s.ql) {
+            t = 0;
+            do {
+              ++b;
+              s = chunk_seq(p, b);
+            } while (s.ql == 0);
+          }
+          n = chunk_tiles(p, s, t, lo, hi);
+        }
+      }
+      if (i1 > i0) return true;
     }
-    return true;
+    return false;
   }
 };
 

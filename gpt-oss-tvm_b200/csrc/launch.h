@@ -176,7 +176,7 @@ int launch_kv_pages_f8(uint8_t* kp, uint8_t* vp, uint8_t* kcode, uint8_t* vcode,
                        const int32_t* table, int32_t tstride, int64_t pos0, int64_t n, int32_t Hkv, uint16_t* kb,
                        uint16_t* vb, int32_t to_pages, cudaStream_t s);
 // verify.cu: drafted tokens against the target's logits
-int64_t verify_scratch_bytes(int64_t T);
+int64_t verify_scratch_bytes(int64_t T, int64_t V);
 int launch_verify(const void* logits, int32_t bf16, int64_t ld, const int32_t* tokens, const int32_t* row_start,
                   int64_t T, int32_t N, int32_t V, double temperature, const float* accept_u, const float* next_u,
                   const float* draft, int64_t ld_draft, void* scratch, int32_t* accepted, int32_t* next,

@@ -17,22 +17,26 @@
 // over threads and CTAs cannot change a token: the kernels and any other
 // evaluation of the formulas above agree bit for bit.
 //
-// verify_rows_kernel    one cluster of 8 CTAs per row: its slice of the row
-//                       stays in shared memory between the maximum and the
-//                       sum, so the logits are read once
-// verify_next_kernel    one cluster per sequence: the first rejected row, the
-//                       sum of its weights by 1024-value pieces, then the one
-//                       piece that holds the draw
+// verify_rows_kernel    one cluster of CTAs per row: a CTA's slice stays in
+//                       shared memory between the maximum and the sums, so the
+//                       logits are read once; the sums of pieces of 256 values
+//                       go to the scratch buffer
+// verify_next_kernel    one CTA per sequence: the first rejected row, the piece
+//                       that holds the draw from the stored sums, and the
+//                       token in it.  Only with draft distributions the
+//                       residual needs the whole row again: then a cluster per
+//                       sequence sums its pieces first
 #include "common.cuh"
 #include "launch.h"
 
 namespace gptoss {
 
-constexpr int kVerCluster = 8;
 constexpr int kVerThreads = 512;
-constexpr int kVerPiece = 1024;          // values per piece of the running sum
-constexpr float kVerFix = 1099511627776.0f;  // 2^40
-constexpr int64_t kVerMaxVocab = 1 << 22;    // 2^22 weights of at most 2^40 stay below 2^63
+constexpr int kVerWarps = kVerThreads / 32;
+constexpr int kVerPiece = 256;            // values per piece of the running sum: 8 a lane
+constexpr int kVerNextCluster = 8;
+constexpr int64_t kVerMaxVocab = 1 << 22;  // 2^22 weights of at most 2^40 stay below 2^63
+constexpr int kVerStash = 110 * 1024;      // bytes of a slice kept on chip: two CTAs per SM
 
 struct VerifyParams {
   const void* logits;
@@ -40,16 +44,17 @@ struct VerifyParams {
   const int32_t* tokens;
   const int32_t* row_start;
   int64_t T;
-  int32_t N, V;
+  int32_t N, V, pieces;
   float inv_temp;
   int greedy;
   const float* accept_u;
   const float* next_u;
   const float* draft;  // [T, V] rows of stride ld_draft, or NULL
   int64_t ld_draft;
-  // per row: max, sum of the weights, lowest index of the max, accepted
-  float* row_max;
+  // per row: sums of the pieces and of all weights, max, lowest index of the max, accepted
+  long long* piece_sum;
   long long* row_sum;
+  float* row_max;
   int32_t* row_top;
   int32_t* row_ok;
   int32_t* accepted;
@@ -70,11 +75,28 @@ __device__ __forceinline__ float ver_value<uint16_t>(uint16_t x) {
 __device__ __forceinline__ float ver_exp(float z, float m, float inv_temp) {
   return z == m ? 1.0f : expf(__fmul_rn(__fsub_rn(z, m), inv_temp));
 }
-__device__ __forceinline__ long long ver_fix(float w) { return __float2ll_rz(w * kVerFix); }
-__device__ __forceinline__ float ver_total(long long z) { return __ll2float_rn(z) * (1.0f / kVerFix); }
+__device__ __forceinline__ float ver_total(long long z) { return __ll2float_rn(z) * (1.0f / 1099511627776.0f); }
+
+// floor(w * 2^40) of 0 <= w <= 1 as hi * 2^20 + lo, both below 2^21: an
+// addition of 2^23 that rounds towards zero leaves the whole part in the low
+// bits (a conversion to 64 bits runs at a quarter of the rate).
+__device__ __forceinline__ void ver_fix(float w, uint32_t& hi, uint32_t& lo) {
+  const float a = w * 1048576.0f;
+  const float t = __fadd_rz(a, 8388608.0f);
+  hi = __float_as_uint(t) - 0x4B000000u;
+  lo = __float_as_uint(__fmaf_rz(__fsub_rn(a, __fsub_rn(t, 8388608.0f)), 1048576.0f, 8388608.0f)) - 0x4B000000u;
+}
+__device__ __forceinline__ long long ver_join(uint32_t hi, uint32_t lo) { return ((long long)hi << 20) + lo; }
 
 __device__ __forceinline__ long long warp_sum64(long long v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ long long warp_scan64(long long v) {
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += t;
+  }
   return v;
 }
 __device__ __forceinline__ void better(float& m, int& i, float m2, int i2) {
@@ -95,16 +117,16 @@ __device__ __forceinline__ long long ld_cluster_s64(const void* p, uint32_t rank
   return v;
 }
 
-// The slice [lo, hi) of a row that CTA `rank` takes: whole pieces.
-__device__ __forceinline__ void ver_slice(int V, uint32_t rank, int& lo, int& hi) {
-  const int pieces = (V + kVerPiece - 1) / kVerPiece;
-  const int per = (pieces + kVerCluster - 1) / kVerCluster;
-  lo = min(V, (int)rank * per * kVerPiece);
-  hi = min(V, lo + per * kVerPiece);
+// The pieces [lo, hi) of a row that CTA `rank` of `n` takes.
+__device__ __forceinline__ void ver_slice(int pieces, uint32_t rank, uint32_t n, int& lo, int& hi) {
+  const int per = (pieces + (int)n - 1) / (int)n;
+  lo = min(pieces, (int)rank * per);
+  hi = min(pieces, lo + per);
 }
 
-// Calls f(index, value) for this thread's values of [lo, hi); 16-byte loads
-// over the aligned middle (a row of an odd vocabulary starts anywhere).
+// Calls f(index, value) for this thread's values of [lo, hi): 16-byte loads
+// over the aligned middle (a row of an odd vocabulary starts anywhere), eight
+// of them in flight.
 template <typename T, typename F>
 __device__ __forceinline__ void ver_each(const T* __restrict__ row, int lo, int hi, F f) {
   constexpr int kVec = 16 / (int)sizeof(T);
@@ -113,46 +135,54 @@ __device__ __forceinline__ void ver_each(const T* __restrict__ row, int lo, int 
   const int nv = (hi - a0) / kVec;
   const int tail = a0 + nv * kVec;
   if (threadIdx.x < (unsigned)(a0 - lo)) f(lo + (int)threadIdx.x, row[lo + threadIdx.x]);
-#pragma unroll 4
-  for (int v = threadIdx.x; v < nv; v += kVerThreads) {
-    const uint4 x = ldg_nc_v4(row + a0 + v * kVec);
-    const T* e = (const T*)&x;
+  for (int v0 = threadIdx.x; v0 < nv; v0 += 8 * kVerThreads) {
+    uint4 x[8];
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) f(a0 + v * kVec + k, e[k]);
+    for (int k = 0; k < 8; ++k)
+      if (v0 + k * kVerThreads < nv) x[k] = ldg_nc_v4(row + a0 + (v0 + k * kVerThreads) * kVec);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (v0 + k * kVerThreads < nv) {
+        const T* e = (const T*)&x[k];
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) f(a0 + (v0 + k * kVerThreads) * kVec + y, e[y]);
+      }
+    }
   }
   if (threadIdx.x < (unsigned)(hi - tail)) f(tail + (int)threadIdx.x, row[tail + threadIdx.x]);
 }
 
+// One cluster of `C` CTAs per row.
 template <typename T>
-__global__ void __cluster_dims__(kVerCluster, 1, 1) __launch_bounds__(kVerThreads)
-    verify_rows_kernel(const VerifyParams p, int stash) {
+__global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyParams p, int C, int stash) {
   extern __shared__ __align__(16) uint8_t ver_smem[];
   T* keep = (T*)ver_smem;  // this CTA's slice, when `stash`
-  __shared__ float wm[kVerThreads / 32];
-  __shared__ int wi[kVerThreads / 32];
-  __shared__ long long ws[kVerThreads / 32];
+  __shared__ float wm[kVerWarps];
+  __shared__ int wi[kVerWarps];
+  __shared__ long long ws[kVerWarps];
   __shared__ float cta_m;
   __shared__ int cta_i;
   __shared__ long long cta_s;
+  cudaTriggerProgrammaticLaunchCompletion();  // the next kernel may take its place and wait
   const uint32_t rank = cluster_ctarank();
-  const int64_t r = blockIdx.x / kVerCluster;
+  const int64_t r = blockIdx.x / (unsigned)C;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* row = (const T*)p.logits + r * p.ld;
-  int lo, hi;
-  ver_slice(p.V, rank, lo, hi);
+  int plo, phi;
+  ver_slice(p.pieces, rank, (uint32_t)C, plo, phi);
+  const int lo = plo * kVerPiece, hi = min(p.V, phi * kVerPiece);
   // pass 1: maximum and its lowest index
   float m = -INFINITY;
   int mi = 0x7FFFFFFF;
-  ver_each<T>(row, lo, hi, [&](int i, T x) {
-    if (stash) keep[i - lo] = x;
-    const float z = ver_value<T>(x);
-    if (z > m || mi == 0x7FFFFFFF) {  // a thread's indices rise, but for its head and tail values
-      m = z;
-      mi = i;
-    } else if (z == m && i < mi) {
-      mi = i;
-    }
-  });
+  if (lo < hi)
+    ver_each<T>(row, lo, hi, [&](int i, T x) {
+      if (stash) keep[i - lo] = x;
+      const float z = ver_value<T>(x);
+      if (z > m || mi == 0x7FFFFFFF) {  // a thread's indices rise, but for its tail value, which is its last
+        m = z;
+        mi = i;
+      }
+    });
   for (int o = 16; o > 0; o >>= 1)
     better(m, mi, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, mi, o));
   if (lane == 0) {
@@ -160,70 +190,90 @@ __global__ void __cluster_dims__(kVerCluster, 1, 1) __launch_bounds__(kVerThread
     wi[warp] = mi;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kVerThreads / 32; ++w) better(m, mi, wm[w], wi[w]);
-    cta_m = m;
-    cta_i = mi;
+  if (warp == 0) {
+    m = lane < kVerWarps ? wm[lane] : -INFINITY;
+    mi = lane < kVerWarps ? wi[lane] : 0x7FFFFFFF;
+    for (int o = 16; o > 0; o >>= 1)
+      better(m, mi, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, mi, o));
+    if (lane == 0) {
+      cta_m = m;
+      cta_i = mi;
+    }
   }
   cluster_sync_all();
   m = -INFINITY;
   mi = 0x7FFFFFFF;
-  for (uint32_t c = 0; c < kVerCluster; ++c)
-    better(m, mi, __uint_as_float(ld_cluster_u32(&cta_m, c)), (int)ld_cluster_u32(&cta_i, c));
-  // pass 2: the sum of the weights
-  long long sum = 0;
+  if (lane < C) {
+    m = __uint_as_float(ld_cluster_u32(&cta_m, lane));
+    mi = (int)ld_cluster_u32(&cta_i, lane);
+  }
+  for (int o = 16; o > 0; o >>= 1)
+    better(m, mi, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, mi, o));
+  // pass 2: the sums of the pieces' weights
   if (!p.greedy) {
-    if (stash) {
-      for (int i = threadIdx.x; i < hi - lo; i += kVerThreads)
-        sum += ver_fix(ver_exp(ver_value<T>(keep[i]), m, p.inv_temp));
-    } else {
-      ver_each<T>(row, lo, hi, [&](int i, T x) { sum += ver_fix(ver_exp(ver_value<T>(x), m, p.inv_temp)); });
+    long long sum = 0;
+    for (int c = plo + warp; c < phi; c += kVerWarps) {
+      uint32_t h = 0, l = 0;
+      const int i0 = c * kVerPiece + lane;
+#pragma unroll
+      for (int k = 0; k < kVerPiece / 32; ++k) {
+        const int i = i0 + 32 * k;
+        if (i < hi) {
+          uint32_t h1, l1;
+          ver_fix(ver_exp(ver_value<T>(stash ? keep[i - lo] : row[i]), m, p.inv_temp), h1, l1);
+          h += h1;
+          l += l1;
+        }
+      }
+      const long long s = ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
+      if (lane == 0) p.piece_sum[r * p.pieces + c] = s;
+      sum += s;
     }
-    sum = warp_sum64(sum);
     if (lane == 0) ws[warp] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      sum = 0;
-      for (int w = 0; w < kVerThreads / 32; ++w) sum += ws[w];
-      cta_s = sum;
+    if (warp == 0) {
+      sum = warp_sum64(lane < kVerWarps ? ws[lane] : 0);
+      if (lane == 0) cta_s = sum;
     }
   }
   cluster_sync_all();
-  if (rank == 0 && threadIdx.x == 0) {
-    long long z = 0;
-    if (!p.greedy)
-      for (uint32_t c = 0; c < kVerCluster; ++c) z += ld_cluster_s64(&cta_s, c);
-    int ok = 0;
-    if (r + 1 < p.T) {  // the draft of this row, if the row is not its sequence's last (then nobody looks)
-      const int x = p.tokens[r + 1];
-      if (x >= 0 && x < p.V) {
-        if (p.greedy) {
-          ok = x == mi;
-        } else {
-          const float px = __fdiv_rn(ver_exp(ver_value<T>(row[x]), m, p.inv_temp), ver_total(z));
-          const float qx = p.draft ? p.draft[r * p.ld_draft + x] : 1.0f;
-          ok = __fmul_rn(p.accept_u[r], qx) < px;
+  if (rank == 0 && warp == 0) {
+    const long long z = p.greedy ? 0 : warp_sum64(lane < C ? ld_cluster_s64(&cta_s, lane) : 0);
+    if (lane == 0) {
+      int ok = 0;
+      if (r + 1 < p.T) {  // the draft of this row, if the row is not its sequence's last (then nobody looks)
+        const int x = p.tokens[r + 1];
+        if (x >= 0 && x < p.V) {
+          if (p.greedy) {
+            ok = x == mi;
+          } else {
+            const float px = __fdiv_rn(ver_exp(ver_value<T>(row[x]), m, p.inv_temp), ver_total(z));
+            const float qx = p.draft ? p.draft[r * p.ld_draft + x] : 1.0f;
+            ok = __fmul_rn(p.accept_u[r], qx) < px;
+          }
         }
       }
+      p.row_max[r] = m;
+      p.row_sum[r] = z;
+      p.row_top[r] = mi;
+      p.row_ok[r] = ok;
     }
-    p.row_max[r] = m;
-    p.row_sum[r] = z;
-    p.row_top[r] = mi;
-    p.row_ok[r] = ok;
   }
   cluster_sync_all();  // nobody leaves while its shared memory may be read
 }
 
-// One cluster per sequence.
-template <typename T>
-__global__ void __cluster_dims__(kVerCluster, 1, 1) __launch_bounds__(kVerThreads)
-    verify_next_kernel(const VerifyParams p) {
+// One CTA per sequence, or with kDraft a cluster of kVerNextCluster.
+template <typename T, bool kDraft>
+__global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyParams p) {
   extern __shared__ __align__(16) uint8_t ver_smem[];
-  long long* piece = (long long*)ver_smem;  // sums of this CTA's pieces
-  __shared__ long long cta_s;
-  const uint32_t rank = cluster_ctarank();
-  const int b = blockIdx.x / kVerCluster;
+  long long* mine = (long long*)ver_smem;  // kDraft: sums of this CTA's pieces
+  __shared__ long long ws[kVerWarps];
+  __shared__ long long cta_s, found_run;
+  __shared__ int found;
+  const uint32_t rank = kDraft ? cluster_ctarank() : 0u;
+  const int b = blockIdx.x / (kDraft ? kVerNextCluster : 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  cudaGridDependencySynchronize();  // the rows' results
   const int64_t r0 = max64(0, min64(p.T, p.row_start[b])), r1 = max64(r0, min64(p.T, p.row_start[b + 1]));
   if (r1 <= r0) {  // no rows: nothing to answer
     if (rank == 0 && threadIdx.x == 0) {
@@ -248,91 +298,172 @@ __global__ void __cluster_dims__(kVerCluster, 1, 1) __launch_bounds__(kVerThread
   }
   if (p.greedy) return;
   const T* row = (const T*)p.logits + at * p.ld;
-  const float* qrow = p.draft ? p.draft + at * p.ld_draft : nullptr;
-  const float m = p.row_max[at], total = ver_total(p.row_sum[at]);
+  const float* qrow = kDraft ? p.draft + at * p.ld_draft : nullptr;
+  const float m = p.row_max[at];
+  const long long z = p.row_sum[at];
+  const float total = ver_total(z);
   const int x = last ? -1 : p.tokens[at + 1];
-  int lo, hi;
-  ver_slice(p.V, rank, lo, hi);
-  const int np = (hi - lo + kVerPiece - 1) / kVerPiece;
-  // mode 0: the residual (or the last row's weights); mode 1, when nothing is left of it: the row's own weights
-  for (int mode = 0; mode < 2; ++mode) {
-    auto weight = [&](int i) -> long long {
-      const float e = ver_exp(ver_value<T>(row[i]), m, p.inv_temp);
-      if (last || mode == 1) return ver_fix(e);
-      if (qrow) return ver_fix(fmaxf(__fsub_rn(__fdiv_rn(e, total), qrow[i]), 0.0f));
-      return i == x ? 0 : ver_fix(e);
-    };
-    for (int c = warp; c < np; c += kVerThreads / 32) {
-      const int p0 = lo + c * kVerPiece, p1 = min(hi, p0 + kVerPiece);
-      long long s = 0;
-#pragma unroll 8
-      for (int i = p0 + lane; i < p1; i += 32) s += weight(i);
-      s = warp_sum64(s);
-      if (lane == 0) piece[c] = s;
+  const long long* stored = p.piece_sum + at * p.pieces;
+  auto own = [&](int i) -> long long {
+    uint32_t h, l;
+    ver_fix(ver_exp(ver_value<T>(row[i]), m, p.inv_temp), h, l);
+    return ver_join(h, l);
+  };
+  // the first of pieces [lo, hi) whose running sum from `before` on exceeds u, then the first value in it; whole CTA
+  auto search = [&](int lo, int hi, long long before, long long u, auto sum_of, auto weight) {
+    if (threadIdx.x == 0) found = hi - 1;
+    __syncthreads();
+    long long run = before;
+    for (int c0 = lo; c0 < hi; c0 += kVerThreads) {
+      const int c = c0 + (int)threadIdx.x;
+      const long long v = c < hi ? sum_of(c) : 0;
+      const long long inc = warp_scan64(v);
+      if (lane == 31) ws[warp] = inc;
+      __syncthreads();
+      long long below = run, all = 0;
+      for (int w = 0; w < kVerWarps; ++w) {
+        if (w < warp) below += ws[w];
+        all += ws[w];
+      }
+      if (c < hi && below + inc > u && below + inc - v <= u) {  // one thread at most
+        found = c;
+        found_run = below + inc - v;
+      }
+      run += all;
+      __syncthreads();
+      if (run > u) break;
     }
+    const int c = found;
+    if (threadIdx.x < kVerPiece) {
+      const int i = c * kVerPiece + (int)threadIdx.x;
+      const long long v = i < p.V ? weight(i) : 0;
+      const long long inc = warp_scan64(v);
+      if (lane == 31) ws[warp] = inc;
+      asm volatile("bar.sync 1, %0;" ::"n"(kVerPiece) : "memory");
+      long long below = found_run;
+      for (int w = 0; w < warp; ++w) below += ws[w];
+      if (below + inc > u && below + inc - v <= u) p.next[b] = i;
+    }
+  };
+  // u in [0, S): the token is the first whose running sum is above it
+  auto draw = [&](long long s) {
+    const long long u = __double2ll_rd(__dmul_rn((double)p.next_u[b], __ll2double_rn(s)));
+    return max(0ll, min(u, s - 1));
+  };
+  if (kDraft && !last) {
+    auto left = [&](int i) -> long long {
+      const float e = ver_exp(ver_value<T>(row[i]), m, p.inv_temp);
+      uint32_t h, l;
+      ver_fix(fmaxf(__fsub_rn(__fdiv_rn(e, total), qrow[i]), 0.0f), h, l);
+      return ver_join(h, l);
+    };
+    int plo, phi;
+    ver_slice(p.pieces, rank, kVerNextCluster, plo, phi);
+    long long sum = 0;
+    for (int c = plo + warp; c < phi; c += kVerWarps) {
+      float zv[kVerPiece / 32], qv[kVerPiece / 32];
+#pragma unroll
+      for (int k = 0; k < kVerPiece / 32; ++k) {
+        const int i = c * kVerPiece + lane + 32 * k;
+        zv[k] = i < p.V ? ver_value<T>(row[i]) : -INFINITY;
+        qv[k] = i < p.V ? qrow[i] : 1.0f;
+      }
+      uint32_t h = 0, l = 0;
+#pragma unroll
+      for (int k = 0; k < kVerPiece / 32; ++k) {
+        uint32_t h1, l1;
+        ver_fix(fmaxf(__fsub_rn(__fdiv_rn(ver_exp(zv[k], m, p.inv_temp), total), qv[k]), 0.0f), h1, l1);
+        if (c * kVerPiece + lane + 32 * k < p.V) {
+          h += h1;
+          l += l1;
+        }
+      }
+      const long long s = ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
+      if (lane == 0) mine[c - plo] = s;
+      sum += s;
+    }
+    if (lane == 0) ws[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-      long long s = 0;
-      for (int c = lane; c < np; c += 32) s += piece[c];
-      s = warp_sum64(s);
-      if (lane == 0) cta_s = s;
+      sum = warp_sum64(lane < kVerWarps ? ws[lane] : 0);
+      if (lane == 0) cta_s = sum;
     }
     cluster_sync_all();
-    long long before = 0, all = 0, mine = 0;
-    for (uint32_t c = 0; c < kVerCluster; ++c) {
+    long long before = 0, all = 0, here = 0;
+    for (uint32_t c = 0; c < kVerNextCluster; ++c) {
       const long long s = ld_cluster_s64(&cta_s, c);
       if (c < rank) before += s;
-      if (c == rank) mine = s;
+      if (c == rank) here = s;
       all += s;
     }
-    cluster_sync_all();
-    if (all == 0 && mode == 0) continue;
-    // u in [0, S): the token is the first whose running sum is above it
-    const double sd = __ll2double_rn(all);
-    long long u = __double2ll_rd(__dmul_rn((double)p.next_u[b], sd));
-    u = max(0ll, min(u, all - 1));
-    if (warp == 0 && u >= before && u < before + mine) {
-      long long run = before;
-      int c = 0;
-      while (c < np - 1 && run + piece[c] <= u) run += piece[c++];
-      const int p0 = lo + c * kVerPiece, p1 = min(hi, p0 + kVerPiece);
-      for (int i0 = p0; i0 < p1; i0 += 32) {
-        const int i = i0 + lane;
-        long long s = i < p1 ? weight(i) : 0;
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long t = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += t;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, run + s > u);
-        if (hit) {
-          if (lane == 0) p.next[b] = i0 + __ffs(hit) - 1;
-          break;
-        }
-        run += __shfl_sync(0xffffffffu, s, 31);
-      }
+    cluster_sync_all();  // nobody leaves while its shared memory may be read
+    if (all > 0) {
+      const long long u = draw(all);
+      if (u >= before && u < before + here)
+        search(plo, phi, before, u, [&](int c) { return mine[c - plo]; }, left);
+      return;
     }
-    break;
   }
+  if (rank != 0) return;
+  // the row's own weights, without the draft when it was looked up and rejected (unless nothing else is left)
+  const bool drop = !kDraft && x >= 0 && x < p.V && own(x) < z;
+  const long long wx = drop ? own(x) : 0;
+  search(0, p.pieces, 0, draw(z - wx), [&](int c) { return stored[c] - (drop && x / kVerPiece == c ? wx : 0); },
+         [&](int i) { return drop && i == x ? 0ll : own(i); });
 }
 
 // --------------------------------------------------------------- launch --
-int64_t verify_scratch_bytes(int64_t T) { return T * (8 + 4 + 4 + 4) + 64; }
+static int64_t ver_pieces(int64_t V) { return (V + kVerPiece - 1) / kVerPiece; }
+int64_t verify_scratch_bytes(int64_t T, int64_t V) { return T * (8 * ver_pieces(V) + 8 + 4 + 4 + 4) + 64; }
 
 template <typename T>
 static int launch_verify_t(const VerifyParams& p, cudaStream_t s) {
-  const int pieces = (p.V + kVerPiece - 1) / kVerPiece;
-  const int per = (pieces + kVerCluster - 1) / kVerCluster;
-  // the slice stays in shared memory while two CTAs fit on an SM
-  int keep = per * kVerPiece * (int)sizeof(T);
-  const int stash = keep <= 110 * 1024;
-  if (!stash) keep = 0;
-  static FuncSmemAttr attr_rows, attr_next;
-  if (keep > 40 * 1024) ensure_dyn_smem(attr_rows, (const void*)verify_rows_kernel<T>, 110 * 1024);
-  verify_rows_kernel<T><<<(unsigned)(p.T * kVerCluster), kVerThreads, keep, s>>>(p, stash);
-  if (cudaGetLastError() != cudaSuccess) return -3;
-  verify_next_kernel<T><<<(unsigned)(p.N * kVerCluster), kVerThreads, per * 8, s>>>(p);
-  (void)attr_next;
-  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  cfg.blockDim = dim3(kVerThreads);
+  cfg.stream = s;
+  cfg.attrs = at;
+  if (p.T > 0) {
+    // CTAs of a row: 16 while the rows leave SMs free (a cluster's most), else 8
+    static std::atomic<int> wide[kMaxAttrDevices];  // 0: not asked yet, 1: clusters of 16 allowed, 2: not
+    static FuncSmemAttr attr;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxAttrDevices) dev = 0;
+    ensure_dyn_smem(attr, (const void*)verify_rows_kernel<T>, kVerStash);
+    if (wide[dev].load(std::memory_order_relaxed) == 0) {
+      const bool ok = cudaFuncSetAttribute((const void*)verify_rows_kernel<T>,
+                                           cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+      if (!ok) (void)cudaGetLastError();
+      wide[dev].store(ok ? 1 : 2, std::memory_order_relaxed);
+    }
+    const int C = p.T * 16 <= device_sm_count() && wide[dev].load(std::memory_order_relaxed) == 1 ? 16 : 8;
+    int keep = (p.pieces + C - 1) / C * kVerPiece * (int)sizeof(T);
+    const int stash = keep <= kVerStash;
+    if (!stash) keep = 0;
+    cfg.gridDim = dim3((unsigned)(p.T * C));
+    cfg.dynamicSmemBytes = (size_t)keep;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, verify_rows_kernel<T>, p, C, stash) != cudaSuccess) return -3;
+  }
+  // starts while the rows' kernel ends, and waits for its results
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  if (p.draft) {
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = kVerNextCluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+    cfg.gridDim = dim3((unsigned)(p.N * kVerNextCluster));
+    cfg.dynamicSmemBytes = (size_t)((p.pieces + kVerNextCluster - 1) / kVerNextCluster) * 8;
+    return cudaLaunchKernelEx(&cfg, verify_next_kernel<T, true>, p) == cudaSuccess ? 0 : -3;
+  }
+  cfg.gridDim = dim3((unsigned)p.N);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, verify_next_kernel<T, false>, p) == cudaSuccess ? 0 : -3;
 }
 
 int launch_verify(const void* logits, int32_t bf16, int64_t ld, const int32_t* tokens, const int32_t* row_start,
@@ -349,13 +480,15 @@ int launch_verify(const void* logits, int32_t bf16, int64_t ld, const int32_t* t
   p.T = T;
   p.N = N;
   p.V = V;
+  p.pieces = (int32_t)ver_pieces(V);
   p.greedy = temperature < 1e-6;
   p.inv_temp = p.greedy ? 1.0f : (float)(1.0 / temperature);
   p.accept_u = accept_u;
   p.next_u = next_u;
-  p.draft = draft;
+  p.draft = p.greedy ? nullptr : draft;
   p.ld_draft = ld_draft;
-  p.row_sum = (long long*)(((uintptr_t)scratch + 7) & ~(uintptr_t)7);
+  p.piece_sum = (long long*)(((uintptr_t)scratch + 7) & ~(uintptr_t)7);
+  p.row_sum = p.piece_sum + T * p.pieces;
   p.row_max = (float*)(p.row_sum + T);
   p.row_top = (int32_t*)(p.row_max + T);
   p.row_ok = p.row_top + T;

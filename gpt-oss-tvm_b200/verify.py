@@ -8,11 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-
-
-def _need(cond: bool, what: str):
-    if not cond:
-        raise ValueError(what)
+from .chunk import _bad, _i32, _run
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.Tensor,
@@ -27,37 +23,34 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.T
     accepted [N], the drafts before the first that is not, and next_token [N],
     drawn with next_draws [N] from what is left of p there, or from the last
     row's p.  temperature < 1e-6: greedy, no draws needed."""
-    dev = logits.device
-    _need(logits.is_cuda and logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16),
-          "logits must be a CUDA tensor [rows, vocabulary], float32 or bfloat16")
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        _bad("logits must be a CUDA tensor [rows, vocabulary], float32 or bfloat16")
+    index = logits.get_device()
     T, V = logits.shape
-    _need(T <= 1 or (logits.stride(1) == 1 and logits.stride(0) >= V), "the values of a row of logits must be dense")
+    if T > 1 and (logits.stride(1) != 1 or logits.stride(0) < V):
+        _bad("the values of a row of logits must be dense")
     n = row_start.shape[0] - 1
-    for t, m, name in ((tokens, T, "tokens"), (row_start, n + 1, "row_start")):
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == m and t.is_contiguous() and t.device == dev,
-              f"{name} must be a dense int32 tensor of {m} entries on {dev}")
-    _need(n >= 0, "row_start needs at least one entry")
+    if n < 0:
+        _bad("row_start needs at least one entry")
+    tokens_p, start_p = _i32(tokens, T, "tokens", index), _i32(row_start, n + 1, "row_start", index)
     greedy = temperature < 1e-6
     if not greedy:
         for t, m, name in ((accept_draws, T, "accept_draws"), (next_draws, n, "next_draws")):
-            _need(t is not None and t.dtype == torch.float32 and t.dim() == 1 and t.shape[0] == m
-                  and t.is_contiguous() and t.device == dev,
-                  f"{name} must be a dense float32 tensor of {m} entries on {dev}")
-    if draft_probs is not None:
-        _need(draft_probs.dtype == torch.float32 and tuple(draft_probs.shape) == (T, V) and draft_probs.device == dev
-              and (T <= 1 or (draft_probs.stride(1) == 1 and draft_probs.stride(0) >= V)),
-              f"draft_probs must be a float32 tensor [{T}, {V}] with dense rows on {dev}")
-    out = torch.empty(2, n, dtype=torch.int32, device=dev)
+            if (t is None or t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != m or not t.is_contiguous()
+                    or t.get_device() != index):
+                _bad(f"{name} must be a dense float32 tensor of {m} entries on cuda:{index}")
+    if draft_probs is not None and (draft_probs.dtype is not torch.float32 or draft_probs.shape != (T, V)
+                                    or draft_probs.get_device() != index
+                                    or (T > 1 and (draft_probs.stride(1) != 1 or draft_probs.stride(0) < V))):
+        _bad(f"draft_probs must be a float32 tensor [{T}, {V}] with dense rows on cuda:{index}")
+    # one allocation: the two answers, then the library's scratch
+    nbytes = _lib.load().gptoss_verify_drafts_scratch_bytes(T, V)
+    buf = torch.empty(2 * n + nbytes // 4 + 1, dtype=torch.int32, device=logits.device)
     if n:
-        lib = _lib.load()
-        nbytes = lib.gptoss_verify_drafts_scratch_bytes(T)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            _lib.call("gptoss_verify_drafts", logits.data_ptr(), int(logits.dtype == torch.bfloat16),
-                      logits.stride(0) if T > 1 else V, tokens.data_ptr(), row_start.data_ptr(), T, n, V,
-                      float(temperature), None if greedy else accept_draws.data_ptr(),
-                      None if greedy else next_draws.data_ptr(),
-                      draft_probs.data_ptr() if draft_probs is not None else None,
-                      draft_probs.stride(0) if draft_probs is not None and T > 1 else V, scratch.data_ptr(), nbytes,
-                      out[0].data_ptr(), out[1].data_ptr(), torch.cuda.current_stream().cuda_stream)
-    return out[0], out[1]
+        p = buf.data_ptr()
+        _run(index, "gptoss_verify_drafts", logits.data_ptr(), logits.dtype is torch.bfloat16,
+             logits.stride(0) if T > 1 else V, tokens_p, start_p, T, n, V, temperature,
+             None if greedy else accept_draws.data_ptr(), None if greedy else next_draws.data_ptr(),
+             draft_probs.data_ptr() if draft_probs is not None else None,
+             draft_probs.stride(0) if draft_probs is not None and T > 1 else V, p + 8 * n, nbytes, p, p + 4 * n)
+    return buf[:n], buf[n:2 * n]

@@ -358,7 +358,7 @@ int gptoss_sample_top_p_from_logits(const float* logits, int64_t B, int64_t V, d
  * and the next token is the argmax; the random numbers may be NULL.  A NaN
  * logit counts as -inf; a draft outside 0 .. V - 1 is not accepted; a sequence
  * without rows gives 0 and -1.  All memory on the device; V at most 2^22. */
-int64_t gptoss_verify_drafts_scratch_bytes(int64_t T);
+int64_t gptoss_verify_drafts_scratch_bytes(int64_t T, int64_t V);
 int gptoss_verify_drafts(const void* logits, int32_t logits_bf16, int64_t ld_logits, const int32_t* tokens,
                          const int32_t* row_start, int64_t T, int32_t N, int32_t V, double temperature,
                          const float* accept_u, const float* next_u, const float* draft_probs, int64_t ld_draft,
