@@ -31,12 +31,13 @@
 
 namespace gptoss {
 
-constexpr int kVerThreads = 512;
+constexpr int kVerThreads = 256;
 constexpr int kVerWarps = kVerThreads / 32;
 constexpr int kVerPiece = 256;            // values per piece of the running sum: 8 a lane
-constexpr int kVerNextCluster = 8;
+constexpr int kVerCluster = 16;           // CTAs of a row (the most a cluster takes)
+constexpr int kVerNextCluster = 16;
 constexpr int64_t kVerMaxVocab = 1 << 22;  // 2^22 weights of at most 2^40 stay below 2^63
-constexpr int kVerStash = 110 * 1024;      // bytes of a slice kept on chip: two CTAs per SM
+constexpr int kVerStash = 110 * 1024;      // the most bytes of a slice kept on chip
 
 struct VerifyParams {
   const void* logits;
@@ -65,29 +66,68 @@ template <typename T>
 __device__ __forceinline__ float ver_value(T x);
 template <>
 __device__ __forceinline__ float ver_value<float>(float x) {
-  return x != x ? -INFINITY : x;  // a NaN logit counts as -inf
+  return fmaxf(x, -INFINITY);  // a NaN logit counts as -inf
 }
 template <>
 __device__ __forceinline__ float ver_value<uint16_t>(uint16_t x) {
-  const float f = bf16_bits_to_f32(x);
-  return f != f ? -INFINITY : f;
+  return fmaxf(bf16_bits_to_f32(x), -INFINITY);
 }
+// e of a value; a maximum that is infinite needs the comparison (inf - inf is no number), for any other it says the
+// same without: exp(0) is 1
 __device__ __forceinline__ float ver_exp(float z, float m, float inv_temp) {
-  return z == m ? 1.0f : expf(__fmul_rn(__fsub_rn(z, m), inv_temp));
+  return isinf(m) && z == m ? 1.0f : expf(__fmul_rn(__fsub_rn(z, m), inv_temp));
 }
 __device__ __forceinline__ float ver_total(long long z) { return __ll2float_rn(z) * (1.0f / 1099511627776.0f); }
 
-// floor(w * 2^40) of 0 <= w <= 1 as hi * 2^20 + lo, both below 2^21: an
-// addition of 2^23 that rounds towards zero leaves the whole part in the low
-// bits (a conversion to 64 bits runs at a quarter of the rate).
-__device__ __forceinline__ void ver_fix(float w, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ long long ver_join(uint32_t hi, uint32_t lo) { return ((long long)hi << 20) + lo; }
+// floor(w * 2^40) of 0 <= w <= 1 as hi * 2^20 + lo, both below 2^21, each plus
+// kVerBias: an addition of 2^23 that rounds towards zero leaves the whole part
+// in the low bits (a conversion to 64 bits runs at a quarter of the rate).
+constexpr uint32_t kVerBias = 0x4B000000u;
+__device__ __forceinline__ void ver_fix_biased(float w, uint32_t& hi, uint32_t& lo) {
   const float a = w * 1048576.0f;
   const float t = __fadd_rz(a, 8388608.0f);
-  hi = __float_as_uint(t) - 0x4B000000u;
-  lo = __float_as_uint(__fmaf_rz(__fsub_rn(a, __fsub_rn(t, 8388608.0f)), 1048576.0f, 8388608.0f)) - 0x4B000000u;
+  hi = __float_as_uint(t);
+  lo = __float_as_uint(__fmaf_rz(__fsub_rn(a, __fsub_rn(t, 8388608.0f)), 1048576.0f, 8388608.0f));
 }
-__device__ __forceinline__ long long ver_join(uint32_t hi, uint32_t lo) { return ((long long)hi << 20) + lo; }
-
+__device__ __forceinline__ void ver_fix(float w, uint32_t& hi, uint32_t& lo) {
+  ver_fix_biased(w, hi, lo);
+  hi -= kVerBias;
+  lo -= kVerBias;
+}
+// Sum of a whole piece's weights over the warp, 8 values a lane.
+template <typename F>
+__device__ __forceinline__ long long ver_piece(const float (&z)[8], F weight) {
+  uint32_t h = 0u - 8u * kVerBias, l = h;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint32_t h1, l1;
+    ver_fix_biased(weight(z[k], k), h1, l1);
+    h += h1;
+    l += l1;
+  }
+  return ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
+}
+// Eight values of a lane: 4 lane .. 4 lane + 3 and 128 more of a piece at q
+// (`wide`: 16-byte aligned, or 8 for bf16), -inf from index n on.
+template <typename T>
+__device__ __forceinline__ void ver_load8(const T* q, int n, bool wide, float (&z)[8]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = 128 * h + 4 * lane;
+    T e[4];
+    if (wide && n >= 256) {
+      if (sizeof(T) == 4) *(uint4*)e = *(const uint4*)(q + i);
+      else *(uint2*)e = *(const uint2*)(q + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[4 * h + k] = ver_value<T>(e[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[4 * h + k] = i + k < n ? ver_value<T>(q[i + k]) : -INFINITY;
+    }
+  }
+}
 __device__ __forceinline__ long long warp_sum64(long long v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -98,12 +138,6 @@ __device__ __forceinline__ long long warp_scan64(long long v) {
     if ((int)(threadIdx.x & 31) >= o) v += t;
   }
   return v;
-}
-__device__ __forceinline__ void better(float& m, int& i, float m2, int i2) {
-  if (m2 > m || (m2 == m && i2 < i)) {
-    m = m2;
-    i = i2;
-  }
 }
 // Value of a shared variable in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t ld_cluster_u32(const void* p, uint32_t rank) {
@@ -124,17 +158,25 @@ __device__ __forceinline__ void ver_slice(int pieces, uint32_t rank, uint32_t n,
   hi = min(pieces, lo + per);
 }
 
-// Calls f(index, value) for this thread's values of [lo, hi): 16-byte loads
-// over the aligned middle (a row of an odd vocabulary starts anywhere), eight
-// of them in flight.
-template <typename T, typename F>
-__device__ __forceinline__ void ver_each(const T* __restrict__ row, int lo, int hi, F f) {
+// Largest value of row[lo, hi) over the calling threads (each its own), the
+// values copied to `keep` (from index `pad` on, so that both sides are aligned
+// alike) when it is given: 16-byte loads over the aligned middle, eight in
+// flight.
+template <typename T>
+__device__ __forceinline__ float ver_max(const T* __restrict__ row, int lo, int hi, T* keep, int& pad) {
   constexpr int kVec = 16 / (int)sizeof(T);
   const int mis = (int)((kVec - (((uintptr_t)(row + lo) / sizeof(T)) & (kVec - 1))) & (kVec - 1));
+  pad = (kVec - mis) & (kVec - 1);
   const int a0 = min(hi, lo + mis);
   const int nv = (hi - a0) / kVec;
   const int tail = a0 + nv * kVec;
-  if (threadIdx.x < (unsigned)(a0 - lo)) f(lo + (int)threadIdx.x, row[lo + threadIdx.x]);
+  float m = -INFINITY;
+  auto one = [&](int i) {
+    const T x = row[i];
+    if (keep) keep[i - lo + pad] = x;
+    m = fmaxf(m, ver_value<T>(x));
+  };
+  if (threadIdx.x < (unsigned)(a0 - lo)) one(lo + (int)threadIdx.x);
   for (int v0 = threadIdx.x; v0 < nv; v0 += 8 * kVerThreads) {
     uint4 x[8];
 #pragma unroll
@@ -142,14 +184,20 @@ __device__ __forceinline__ void ver_each(const T* __restrict__ row, int lo, int 
       if (v0 + k * kVerThreads < nv) x[k] = ldg_nc_v4(row + a0 + (v0 + k * kVerThreads) * kVec);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (v0 + k * kVerThreads < nv) {
-        const T* e = (const T*)&x[k];
+      const int v = v0 + k * kVerThreads;
+      if (v < nv) {
+        if (keep) *(uint4*)(keep + (a0 - lo + pad) + v * kVec) = x[k];
+        const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
-        for (int y = 0; y < kVec; ++y) f(a0 + (v0 + k * kVerThreads) * kVec + y, e[y]);
+        for (int y = 0; y < 4; ++y) {  // fmaxf drops a NaN
+          if (sizeof(T) == 4) m = fmaxf(m, __uint_as_float(w[y]));
+          else m = fmaxf(m, fmaxf(__uint_as_float(w[y] << 16), __uint_as_float(w[y] & 0xFFFF0000u)));
+        }
       }
     }
   }
-  if (threadIdx.x < (unsigned)(hi - tail)) f(tail + (int)threadIdx.x, row[tail + threadIdx.x]);
+  if (threadIdx.x < (unsigned)(hi - tail)) one(tail + (int)threadIdx.x);
+  return m;
 }
 
 // One cluster of `C` CTAs per row.
@@ -158,10 +206,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
   extern __shared__ __align__(16) uint8_t ver_smem[];
   T* keep = (T*)ver_smem;  // this CTA's slice, when `stash`
   __shared__ float wm[kVerWarps];
-  __shared__ int wi[kVerWarps];
   __shared__ long long ws[kVerWarps];
   __shared__ float cta_m;
-  __shared__ int cta_i;
   __shared__ long long cta_s;
   cudaTriggerProgrammaticLaunchCompletion();  // the next kernel may take its place and wait
   const uint32_t rank = cluster_ctarank();
@@ -171,74 +217,65 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
   int plo, phi;
   ver_slice(p.pieces, rank, (uint32_t)C, plo, phi);
   const int lo = plo * kVerPiece, hi = min(p.V, phi * kVerPiece);
-  // pass 1: maximum and its lowest index
-  float m = -INFINITY;
-  int mi = 0x7FFFFFFF;
-  if (lo < hi)
-    ver_each<T>(row, lo, hi, [&](int i, T x) {
-      if (stash) keep[i - lo] = x;
-      const float z = ver_value<T>(x);
-      if (z > m || mi == 0x7FFFFFFF) {  // a thread's indices rise, but for its tail value, which is its last
-        m = z;
-        mi = i;
-      }
-    });
-  for (int o = 16; o > 0; o >>= 1)
-    better(m, mi, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, mi, o));
-  if (lane == 0) {
-    wm[warp] = m;
-    wi[warp] = mi;
-  }
+  // pass 1: the maximum
+  int pad = 0;
+  float m = lo < hi ? ver_max<T>(row, lo, hi, stash ? keep : (T*)nullptr, pad) : -INFINITY;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) wm[warp] = m;
   __syncthreads();
   if (warp == 0) {
     m = lane < kVerWarps ? wm[lane] : -INFINITY;
-    mi = lane < kVerWarps ? wi[lane] : 0x7FFFFFFF;
-    for (int o = 16; o > 0; o >>= 1)
-      better(m, mi, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, mi, o));
-    if (lane == 0) {
-      cta_m = m;
-      cta_i = mi;
-    }
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) cta_m = m;
   }
   cluster_sync_all();
-  m = -INFINITY;
-  mi = 0x7FFFFFFF;
-  if (lane < C) {
-    m = __uint_as_float(ld_cluster_u32(&cta_m, lane));
-    mi = (int)ld_cluster_u32(&cta_i, lane);
-  }
-  for (int o = 16; o > 0; o >>= 1)
-    better(m, mi, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, mi, o));
-  // pass 2: the sums of the pieces' weights
+  m = lane < C ? __uint_as_float(ld_cluster_u32(&cta_m, lane)) : -INFINITY;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  // pass 2: the sums of the pieces' weights, or the lowest index of the maximum
+  const T* src = stash ? keep + pad : row + lo;
   if (!p.greedy) {
+    const bool wide = ((uintptr_t)src & (4 * sizeof(T) - 1)) == 0;
     long long sum = 0;
     for (int c = plo + warp; c < phi; c += kVerWarps) {
-      uint32_t h = 0, l = 0;
-      const int i0 = c * kVerPiece + lane;
-#pragma unroll
-      for (int k = 0; k < kVerPiece / 32; ++k) {
-        const int i = i0 + 32 * k;
-        if (i < hi) {
-          uint32_t h1, l1;
-          ver_fix(ver_exp(ver_value<T>(stash ? keep[i - lo] : row[i]), m, p.inv_temp), h1, l1);
-          h += h1;
-          l += l1;
-        }
-      }
-      const long long s = ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
+      float z[8];
+      ver_load8<T>(src + (c * kVerPiece - lo), hi - c * kVerPiece, wide, z);
+      // beyond the row's end z is -inf: e = 0, but for a row of nothing else
+      const int left = hi - c * kVerPiece;
+      const long long s =
+          isinf(m) ? ver_piece(z, [&](float v, int k) {
+            return 128 * (k >> 2) + 4 * lane + (k & 3) < left ? ver_exp(v, m, p.inv_temp) : 0.f;
+          })
+                   : ver_piece(z, [&](float v, int) { return expf(__fmul_rn(__fsub_rn(v, m), p.inv_temp)); });
       if (lane == 0) p.piece_sum[r * p.pieces + c] = s;
       sum += s;
     }
     if (lane == 0) ws[warp] = sum;
-    __syncthreads();
-    if (warp == 0) {
-      sum = warp_sum64(lane < kVerWarps ? ws[lane] : 0);
+  } else {
+    int mi = 0x7FFFFFFF;
+    for (int i = lo + (int)threadIdx.x; i < hi; i += kVerThreads)
+      if (ver_value<T>(src[i - lo]) == m) {
+        mi = i;
+        break;
+      }
+    ws[warp] = 0;
+    mi = __reduce_min_sync(0xffffffffu, mi);
+    if (lane == 0) ws[warp] = mi;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    if (!p.greedy) {
+      const long long sum = warp_sum64(lane < kVerWarps ? ws[lane] : 0);
       if (lane == 0) cta_s = sum;
+    } else {
+      const int mi = __reduce_min_sync(0xffffffffu, lane < kVerWarps ? (int)ws[lane] : 0x7FFFFFFF);
+      if (lane == 0) cta_s = mi;
     }
   }
   cluster_sync_all();
   if (rank == 0 && warp == 0) {
-    const long long z = p.greedy ? 0 : warp_sum64(lane < C ? ld_cluster_s64(&cta_s, lane) : 0);
+    const long long part = lane < C ? ld_cluster_s64(&cta_s, lane) : p.greedy ? 0x7FFFFFFF : 0;
+    const long long z = p.greedy ? 0 : warp_sum64(part);
+    const int mi = p.greedy ? __reduce_min_sync(0xffffffffu, (int)part) : -1;
     if (lane == 0) {
       int ok = 0;
       if (r + 1 < p.T) {  // the draft of this row, if the row is not its sequence's last (then nobody looks)
@@ -354,31 +391,34 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
     auto left = [&](int i) -> long long {
       const float e = ver_exp(ver_value<T>(row[i]), m, p.inv_temp);
       uint32_t h, l;
-      ver_fix(fmaxf(__fsub_rn(__fdiv_rn(e, total), qrow[i]), 0.0f), h, l);
+      ver_fix(fminf(fmaxf(__fsub_rn(__fdiv_rn(e, total), fmaxf(qrow[i], -INFINITY)), 0.0f), 1.0f), h, l);  // as in the sums
       return ver_join(h, l);
     };
+    const bool wide = ((uintptr_t)row & (4 * sizeof(T) - 1)) == 0, wide_q = ((uintptr_t)qrow & 15) == 0;
     int plo, phi;
     ver_slice(p.pieces, rank, kVerNextCluster, plo, phi);
     long long sum = 0;
+    float zn[8], qn[8];  // the next piece's values are on their way while one is summed
+    auto fetch = [&](int c) {
+      if (c < phi) {
+        ver_load8<T>(row + c * kVerPiece, p.V - c * kVerPiece, wide, zn);
+        ver_load8<float>(qrow + c * kVerPiece, p.V - c * kVerPiece, wide_q, qn);
+      }
+    };
+    fetch(plo + warp);
     for (int c = plo + warp; c < phi; c += kVerWarps) {
-      float zv[kVerPiece / 32], qv[kVerPiece / 32];
+      float z8[8], q8[8];
+      const int left_n = p.V - c * kVerPiece;
 #pragma unroll
-      for (int k = 0; k < kVerPiece / 32; ++k) {
-        const int i = c * kVerPiece + lane + 32 * k;
-        zv[k] = i < p.V ? ver_value<T>(row[i]) : -INFINITY;
-        qv[k] = i < p.V ? qrow[i] : 1.0f;
+      for (int k = 0; k < 8; ++k) {
+        z8[k] = zn[k];
+        q8[k] = qn[k];
       }
-      uint32_t h = 0, l = 0;
-#pragma unroll
-      for (int k = 0; k < kVerPiece / 32; ++k) {
-        uint32_t h1, l1;
-        ver_fix(fmaxf(__fsub_rn(__fdiv_rn(ver_exp(zv[k], m, p.inv_temp), total), qv[k]), 0.0f), h1, l1);
-        if (c * kVerPiece + lane + 32 * k < p.V) {
-          h += h1;
-          l += l1;
-        }
-      }
-      const long long s = ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
+      fetch(c + kVerWarps);
+      const long long s = ver_piece(z8, [&](float v, int k) {
+        const float d = fminf(fmaxf(__fsub_rn(__fdiv_rn(ver_exp(v, m, p.inv_temp), total), q8[k]), 0.0f), 1.0f);
+        return 128 * (k >> 2) + 4 * lane + (k & 3) < left_n ? d : 0.f;
+      });
       if (lane == 0) mine[c - plo] = s;
       sum += s;
     }
@@ -404,7 +444,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
       return;
     }
   }
-  if (rank != 0) return;
+  if (kDraft && rank != 0) return;
   // the row's own weights, without the draft when it was looked up and rejected (unless nothing else is left)
   const bool drop = !kDraft && x >= 0 && x < p.V && own(x) < z;
   const long long wx = drop ? own(x) : 0;
@@ -416,28 +456,33 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
 static int64_t ver_pieces(int64_t V) { return (V + kVerPiece - 1) / kVerPiece; }
 int64_t verify_scratch_bytes(int64_t T, int64_t V) { return T * (8 * ver_pieces(V) + 8 + 4 + 4 + 4) + 64; }
 
+// Clusters of 16 have to be asked for, once per kernel and device.
+struct VerWide {
+  std::atomic<bool> asked[kMaxAttrDevices] = {};
+};
+static bool ver_wide_clusters(const void* f, VerWide& w) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxAttrDevices) dev = 0;
+  if (w.asked[dev].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  w.asked[dev].store(true, std::memory_order_release);
+  return true;
+}
+
 template <typename T>
 static int launch_verify_t(const VerifyParams& p, cudaStream_t s) {
+  static VerWide wide_rows, wide_next;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.blockDim = dim3(kVerThreads);
   cfg.stream = s;
   cfg.attrs = at;
   if (p.T > 0) {
-    // CTAs of a row: 16 while the rows leave SMs free (a cluster's most), else 8
-    static std::atomic<int> wide[kMaxAttrDevices];  // 0: not asked yet, 1: clusters of 16 allowed, 2: not
     static FuncSmemAttr attr;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxAttrDevices) dev = 0;
-    ensure_dyn_smem(attr, (const void*)verify_rows_kernel<T>, kVerStash);
-    if (wide[dev].load(std::memory_order_relaxed) == 0) {
-      const bool ok = cudaFuncSetAttribute((const void*)verify_rows_kernel<T>,
-                                           cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
-      if (!ok) (void)cudaGetLastError();
-      wide[dev].store(ok ? 1 : 2, std::memory_order_relaxed);
-    }
-    const int C = p.T * 16 <= device_sm_count() && wide[dev].load(std::memory_order_relaxed) == 1 ? 16 : 8;
-    int keep = (p.pieces + C - 1) / C * kVerPiece * (int)sizeof(T);
+    ensure_dyn_smem(attr, (const void*)verify_rows_kernel<T>, kVerStash + 16);
+    const int C = kVerCluster;
+    if (!ver_wide_clusters((const void*)verify_rows_kernel<T>, wide_rows)) return -3;
+    int keep = (p.pieces + C - 1) / C * kVerPiece * (int)sizeof(T) + 16;
     const int stash = keep <= kVerStash;
     if (!stash) keep = 0;
     cfg.gridDim = dim3((unsigned)(p.T * C));
@@ -453,6 +498,7 @@ static int launch_verify_t(const VerifyParams& p, cudaStream_t s) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
   if (p.draft) {
+    if (!ver_wide_clusters((const void*)verify_next_kernel<T, true>, wide_next)) return -3;
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = kVerNextCluster;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
