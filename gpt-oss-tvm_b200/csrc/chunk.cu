@@ -205,12 +205,15 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 }
 
 // ---------------------------------------------------------- keys on M --
-// CTA = two streams of 4 softmax warps (a kv head each), one warp that loads
-// and one that issues the products.  A tile is 128 keys of both heads (8
-// pages); one TMA box brings a page's keys of both, in groups of 8 rows of 128
+// CTA = two streams of softmax warps (a kv head each), a warp each that loads K
+// and V, and one per stream that issues the products.  A tile is 128 keys of
+// both heads (up to 16 rows in 8 bits: 256; the chain from one tile's products
+// to the next takes about 2000 cycles whatever it holds).  From 32 rows on a
+// stream has 8 warps, two for the same keys with half of the rows each: a
+// thread's rows are unrolled, and past about 700 instructions a tile the
+// instruction cache, not the issue, sets the pace.  One TMA box brings a page's keys of both, in groups of 8 rows of 128
 // bytes (bf16: a head's, 8-bit: both heads' side by side), so that a head's 128
-// keys are one matrix operand with an even stride.  K and V have a loading
-// warp each: the copy engine takes 2 KB in about 97 cycles from two issuers,
+// keys are one matrix operand with an even stride.  Two warps load: the copy engine takes 2 KB in about 97 cycles from two issuers,
 // 135 from one.  Per tile and stream:
 //   S^T [128 keys x W] = K Q^T    A = the K tile as it lies, B = Q, in TMEM
 //   a thread owns a key: its W scores are registers, the key's mask, scale
@@ -224,48 +227,55 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 // tcgen05's, and each 8-bit value had to be widened.)
 //
 // 8-bit pages are operands as they are (kind::f8f6f4).  The other side is then
-// e4m3 too, as two terms in columns of their own, W = 2 N: Q is scaled by a
-// power of two per unit and head, hi = Q to 4 significant bits, lo = 16 times
-// the rest (S = hi + lo / 16, 2^-22 of the largest); P likewise (2^-16 of the
-// row's largest).  The key's power of two meets the
+// e4m3 too, as two terms.  Q is scaled by a power of two per unit and head; hi =
+// Q to 4 significant bits and lo = the rest are two products into the same
+// columns (2^-18 of the largest).  P's terms have columns of their own, W = 2 N,
+// lo = 16 times the rest (2^-16 of the row's largest).  The key's power of two meets the
 // score in fp32; the value's goes into the exponent, t = s + e_v, and the
 // softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
 //
 // The reference m of a row moves only when a score exceeds it by 8 (8-bit:
 // when P would pass 448), which one barrier of the stream's warps tells; then
 // O^T in TMEM is rescaled.
-constexpr int kKeysKT = 128;
-constexpr int kKeysThreads = 12 * 32;
-
 template <bool F8, int N_>
 struct KeysCfg {
-  static constexpr int N = N_;                            // rows of a unit
-  static constexpr int W = F8 ? 2 * N : N;                // columns of S^T and O^T
+  static constexpr int N = N_;                             // rows of a unit
+  static constexpr int W = F8 ? 2 * N : N;                 // columns of O^T
+  static constexpr bool kSplit = N >= 32;                  // two warps share 32 keys, half of the rows each
+  static constexpr int KT = F8 && !kSplit ? 256 : 128;     // keys of a tile
+  static constexpr int kWps = kSplit ? 8 : KT / 32;        // softmax warps of a stream
+  static constexpr int NR = kSplit ? N / 2 : N;            // rows of a thread
+  static constexpr int kSums = KT / 32;                    // warps that hold a part of a row's sum
+  static constexpr int kThreads = 2 * kWps * 32 + 128;
   static constexpr int kRowBytes = F8 ? 64 : 128;
-  static constexpr int kSide = 2 * kKeysKT * kRowBytes;   // K or V of a tile, two heads
-  static constexpr int kCodes = F8 ? 2 * 2 * kKeysKT : 0;  // [K, V][head][128]
-  static constexpr int kStages = F8 ? 4 : 2;
-  static constexpr int kQ = N * 128;                      // per stream: N rows of 128 bytes, or 2 N of 64
-  static constexpr int kP = kKeysKT * 128;                // per stream
-  static constexpr int kTmem = 4 * W <= 64 ? 64 : 4 * W <= 128 ? 128 : 4 * W <= 256 ? 256 : 512;
+  static constexpr int kSide = 2 * KT * kRowBytes;         // K or V of a tile, two heads
+  static constexpr int kCodes = F8 ? 2 * 2 * KT : 0;       // [K, V][head][KT]
+  static constexpr int kStages = 2;
+  static constexpr int kQ = N * 128;                       // per stream: N rows of 128 bytes, or 2 N of 64
+  static constexpr int kP = KT * 128;                      // per stream
+  static constexpr int kColO = 2 * (KT / 128) * N;         // S^T: N columns per stream and 128 keys, then O^T
+  static constexpr int kCols = kColO + 2 * W;
+  static constexpr int kTmem = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static constexpr int kOffP = kStages * 2 * kSide;
   static constexpr int kOffQ = kOffP + 2 * kP;
   static constexpr int kOffCodes = kOffQ + 2 * kQ;
-  static constexpr int kOffRed = kOffCodes + kStages * kCodes;      // per stream: [4][N] maxima or sums
-  static constexpr int kOffRef = kOffRed + 2 * 4 * N * 4;           // per stream: m [N], factor [N]
+  static constexpr int kOffRed = kOffCodes + kStages * kCodes;  // per stream: [kSums][N] maxima or sums
+  static constexpr int kOffRef = kOffRed + 2 * kSums * N * 4;   // per stream: -m [N], factor [N]
   static constexpr int kOffPre = kOffRef + 2 * 2 * N * 4;
   static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
   static constexpr int kOffBar = kOffSeg + 2 * (int)sizeof(ChunkSeg);
   static constexpr int kAlloc = kOffBar + (4 * kStages + 4 + 10) * 8 + 32 + 1024;
-  static_assert(kAlloc <= 227 * 1024, "shared memory");
+  static_assert(kAlloc <= 227 * 1024 && kCols <= 512, "shared memory, TMEM");
 };
 
 template <bool F8, int N_>
-__global__ void __launch_bounds__(kKeysThreads, 1)
+__global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
     chunk_keys_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const ChunkParams p, const int HB) {
   using C = KeysCfg<F8, N_>;
-  constexpr int N = C::N, W = C::W, RB = C::kRowBytes, NS = C::kStages;
+  constexpr int N = C::N, W = C::W, RB = C::kRowBytes, NS = C::kStages, KT = C::KT, kWps = C::kWps, NR = C::NR,
+                kSums = C::kSums, kParts = kWps / 4;
+  constexpr int kLoadK = 2 * kWps, kLoadV = kLoadK + 2, kMma0 = kLoadK + 1, kMma1 = kLoadK + 3;  // warps
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   int32_t* pre = (int32_t*)(smem + C::kOffPre);
@@ -294,29 +304,31 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&seg_full[s], 1);
-      mbar_init(&seg_empty[s], 9 + HB);
-      mbar_init(&qfull[s], 4);
+      mbar_init(&seg_empty[s], 2 * kWps + 1 + HB);
+      mbar_init(&qfull[s], kWps);
       mbar_init(&sfull[s], 1);
-      mbar_init(&sfree[s], 4);
-      mbar_init(&pfull[s], 4);
+      mbar_init(&sfree[s], kWps);
+      mbar_init(&pfull[s], kWps);
       mbar_init(&ofull[s], 1);
     }
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kMma0) {
     tmem_alloc((uint32_t*)tmem_slot, C::kTmem);
     tmem_relinquish();
   }
   tc_fence_before();
-  chunk_plan(p, pre, kKeysThreads);  // with a __syncthreads at its end
+  chunk_plan(p, pre, C::kThreads);  // with a __syncthreads at its end
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   int it = 0;  // key tiles so far
   bool bad = false;
 
-  if (warp == 8 || warp == 10) {
+  // 640 threads start with 96 registers each: 512 * 104 + 128 * 64 of them from here on
+  if (kWps == 8 && warp >= kLoadK) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if (warp == kLoadK || warp == kLoadV) {
     // ------------------------------------------------------------- loads
-    const bool is_v = warp == 10;  // V and the codes; warp 8: K, and the parts' descriptions
+    const bool is_v = warp == kLoadV;  // V and the codes; the other: K, and the parts' descriptions
     ChunkWalk walk;
     if (!is_v) walk.begin(p, pre, gridDim.x, blockIdx.x);
     const uint32_t box = (uint32_t)(HB * kChunkPage * RB);
@@ -345,27 +357,28 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
       const int32_t* trow = p.table + (int64_t)segs[sb].row * p.tstride;
       for (int i = 0; i < ntile; ++i, ++it) {
         const int st = it % NS;
-        // lanes 0..7: the pages of this tile that hold a key to look at
-        const int32_t j = j0 + i * kKeysKT + (lane & 7) * kChunkPage;
+        // the pages of this tile that hold a key to look at, one a lane (8 or 16)
+        constexpr int kPages = KT / kChunkPage;
+        const int32_t j = j0 + i * KT + (lane & (kPages - 1)) * kChunkPage;
         const bool on = j < hi && j + kChunkPage > lo;
         int32_t page = -1;
         if (on) page = __ldg(trow + (uint32_t)(j / kChunkPage) % (uint32_t)p.tstride);
         if (page >= p.pool_pages) page = -1;  // a page outside the pool is not read
-        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0 && lane < 8)) * box;
+        const uint32_t bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, page >= 0 && lane < kPages)) * box;
         if (!bad) bad = !mbar_wait(&empty[st], ((uint32_t)(it / NS) & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
         if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
         __syncwarp();
-        if (page >= 0 && lane < 8)
+        if (page >= 0 && lane < kPages)
           ch_tma_4d(smem + st * 2 * C::kSide + (is_v ? C::kSide : 0) + lane * box, tmap, F8 && HB == 2 ? head / 2 : head,
                     page * 2, &full[st]);
         if (F8 && is_v) {
-          // 16 bytes of codes per page and head: lane = [K, V][head][page]
-          const int half = lane >> 4, hb = (lane >> 3) & 1;
+          // 16 bytes of codes per page and head, [K, V][head][page]: lane = [head][page], K's and V's
+          const int hb = lane / kPages;
           if (page >= 0 && hb < HB) {
-            const uint8_t* src = (half ? p.v_code : p.k_code) + ((int64_t)page * p.Hkv + head + hb) * kChunkPage;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(
-                             smem_u32(smem + C::kOffCodes + st * C::kCodes + lane * kChunkPage)),
-                         "l"(src)
+            const int64_t src = ((int64_t)page * p.Hkv + head + hb) * kChunkPage;
+            uint8_t* dst = smem + C::kOffCodes + st * C::kCodes + lane * kChunkPage;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(p.k_code + src) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + 2 * KT)), "l"(p.v_code + src)
                          : "memory");
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
@@ -377,14 +390,14 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
         __syncwarp();
       }
     }
-  } else if (warp == 9 || warp == 11) {
+  } else if (warp == kMma0 || warp == kMma1) {
     // ---------------------------------------------------------- products
-    // one thread per stream: S^T, A = K (K-major, 128 keys), B = Q (K-major, W rows); O^T, A = V^T (dims-major),
-    // B = P^T (rows-major)
-    const int s = warp == 11;
+    // one thread per stream: S^T, A = K (K-major, 128 keys), B = Q (K-major, N rows; 8 bit: its two terms one after
+    // the other); O^T, A = V^T (dims-major), B = P^T (rows-major)
+    const int s = warp == kMma1;
     if (s < HB && elect_one()) {
       const uint32_t fmt = F8 ? (1u << 4) : ((1u << 4) | (1u << 7) | (1u << 10));
-      const uint32_t idesc_s = fmt | ((uint32_t)(W >> 3) << 17) | (8u << 24);
+      const uint32_t idesc_s = fmt | ((uint32_t)(N >> 3) << 17) | (8u << 24);
       const uint32_t idesc_o = fmt | (1u << 15) | (1u << 16) | ((uint32_t)(W >> 3) << 17) | (4u << 24);
       // bytes between groups of 8 keys, and from one head to the next
       const uint32_t group = (uint32_t)(HB * 8 * RB), to_head = F8 ? 64u : 1024u;
@@ -404,8 +417,11 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
         tc_fence_after();
         const uint64_t a = dk + (uint32_t)ks * (2 * C::kSide >> 4);
 #pragma unroll
-        for (int kk = 0; kk < (F8 ? 2 : 4); ++kk)
-          ch_mma_ss<F8>(tmem + s * W, a + 2 * kk, dq + 2 * kk, idesc_s, kk > 0 ? 1u : 0u);
+        for (int h = 0; h < KT / 128; ++h)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            ch_mma_ss<F8>(tmem + (s * (KT / 128) + h) * N, a + h * 16 * (group >> 4) + 2 * (F8 ? kk & 1 : kk),
+                          dq + (F8 ? (kk >> 1) * (N * 64 >> 4) + 2 * (kk & 1) : 2 * kk), idesc_s, kk > 0 ? 1u : 0u);
         tc_commit(&sfull[s]);
         tc_commit(&kempty[ks]);
         tp ^= 1u;
@@ -428,8 +444,8 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
           tc_fence_after();
           const uint64_t a = dv + (uint32_t)vs * (2 * C::kSide >> 4);
 #pragma unroll
-          for (int kk = 0; kk < kKeysKT / kStep; ++kk)
-            ch_mma_ss<F8>(tmem + (2 + s) * W, a + kk * v_step, dp + kk * (kStep / 8) * 64, idesc_o,
+          for (int kk = 0; kk < KT / kStep; ++kk)
+            ch_mma_ss<F8>(tmem + C::kColO + s * W, a + kk * v_step, dp + kk * (kStep / 8) * 64, idesc_o,
                           (i > 0 || kk > 0) ? 1u : 0u);
           tc_commit(&ofull[s]);
           tc_commit(&vempty[vs]);
@@ -445,11 +461,16 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
     __syncwarp();
   } else {
     // ----------------------------------------------------------- softmax
-    const int s = warp >> 2, wq = warp & 3, tid = threadIdx.x & 127;  // tid: key of the tile, TMEM lane
+    if (kWps == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    constexpr int kBar = kWps * 32;  // threads of a stream
+    // tid: thread of the stream; tid % KT: its key of the tile; part: which half of the rows (kSplit) or keys
+    const int s = warp / kWps, wq = warp % kWps, tid = threadIdx.x % kBar, key = tid % KT, part = wq >> 2;
+    const int rb = C::kSplit ? part * NR : 0;          // its first row
+    const int sum_at = C::kSplit ? wq & 3 : wq;        // its warp's place in `red`
     const bool mine = s < HB;
-    const uint32_t tl = tmem + ((uint32_t)(wq * 32) << 16);
-    const uint32_t t_s = tl + s * W, t_o = tl + (2 + s) * W;
-    float* red = (float*)(smem + C::kOffRed) + s * 4 * N;
+    const uint32_t tl = tmem + ((uint32_t)((wq & 3) * 32) << 16);
+    const uint32_t t_s = tl + (C::kSplit ? s * N + rb : (s * (KT / 128) + part) * N), t_o = tl + C::kColO + s * W;
+    float* red = (float*)(smem + C::kOffRed) + s * kSums * N;
     float* nref = (float*)(smem + C::kOffRef) + s * 2 * N;  // -m of a row
     float* fac = nref + N;
     uint8_t* qs = smem + C::kOffQ + s * C::kQ;
@@ -459,7 +480,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
     for (int sn = 0;; ++sn) {
       const int sb = sn & 1;
       if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
-      bad = ch_named_or(6, 256, bad);  // all eight warps leave together
+      bad = ch_named_or(6, 2 * kBar, bad);  // all softmax warps leave together
       const ChunkSeg& sg = segs[sb];
       const int nrows = sg.nrows;
       if (nrows < 0 || bad) break;
@@ -467,16 +488,18 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
       const int32_t lo = sg.lo, hi = sg.hi, first_pos = sg.first_pos;
       const int head0 = (sg.hg * HB + s) * p.G;
       float q_unit = 1.0f;
-      ch_f2 l[N / 2];
+      const int mine_rows = max(0, min(NR, nrows - rb));  // this thread's rows in use
+      ch_f2 l[NR / 2];
 #pragma unroll
-      for (int r = 0; r < N / 2; ++r) l[r] = 0ull;
+      for (int r = 0; r < NR / 2; ++r) l[r] = 0ull;
       if (mine && ntile > 0) {
-        // Q into shared memory: 8 threads per row, 16 rows at a time
-        uint4 x[N / 16];
+        // Q into shared memory: 8 threads per row
+        constexpr int kQRows = kBar / 8, kQIter = (N + kQRows - 1) / kQRows;
+        uint4 x[kQIter];
         uint32_t am = 0;
 #pragma unroll
-        for (int k = 0; k < N / 16; ++k) {
-          const int r = k * 16 + (tid >> 3);
+        for (int k = 0; k < kQIter; ++k) {
+          const int r = k * kQRows + (tid >> 3);
           x[k] = make_uint4(0, 0, 0, 0);
           if (r < nrows) {
             const int tk = r / p.G;
@@ -491,17 +514,18 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
         if (F8) {
           // largest magnitude of the unit's finite values into [128, 256)
           am = __reduce_max_sync(0xffffffffu, am >= 0x7F800000u ? 0u : am);
-          if (lane == 0) red[wq] = __uint_as_float(am);
-          ch_named_sync(1 + s, 128);
-          am = max(max(__float_as_uint(red[0]), __float_as_uint(red[1])),
-                   max(__float_as_uint(red[2]), __float_as_uint(red[3])));
+          if (lane == 0) fac[wq] = __uint_as_float(am);
+          ch_named_sync(1 + s, kBar);
+#pragma unroll
+          for (int w = 0; w < kWps; ++w) am = max(am, __float_as_uint(fac[w]));
           const int ex = max((int)(am >> 23), 14);
           up = __uint_as_float((uint32_t)min(261 - ex, 254) << 23);
           q_unit = 1.0f / up;
         }
 #pragma unroll
-        for (int k = 0; k < N / 16; ++k) {
-          const int r = k * 16 + (tid >> 3), c = tid & 7;
+        for (int k = 0; k < kQIter; ++k) {
+          const int r = k * kQRows + (tid >> 3), c = tid & 7;
+          if (r >= N) continue;
           if (!F8) {
             *(uint4*)(qs + r * 128 + ((c ^ (r & 7)) << 4)) = x[k];
           } else {
@@ -514,20 +538,20 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
                                   __uint_as_float(w[2 * e + 1] & 0xFFFF0000u) * up};
               float hh[4];
 #pragma unroll
-              // what is not finite stays: e4m3 makes it NaN, and with it the row
+              // what is not finite makes the row NaN
               for (int y = 0; y < 4; ++y) hh[y] = fabsf(v[y]) < 1e30f ? ch_round4(v[y]) : __uint_as_float(0x7FC00000u);
               h4[e] = ch_e4m3x2(hh[0], hh[1]) | (ch_e4m3x2(hh[2], hh[3]) << 16);
-              l4[e] = ch_e4m3x2(16.f * (v[0] - hh[0]), 16.f * (v[1] - hh[1])) |
-                      (ch_e4m3x2(16.f * (v[2] - hh[2]), 16.f * (v[3] - hh[3])) << 16);
+              l4[e] = ch_e4m3x2(v[0] - hh[0], v[1] - hh[1]) | (ch_e4m3x2(v[2] - hh[2], v[3] - hh[3]) << 16);
             }
-            const int r2 = N + r;
-            *(uint2*)(qs + r * 64 + (((c >> 1) ^ ((r >> 1) & 3)) << 4) + (c & 1) * 8) = make_uint2(h4[0], h4[1]);
-            *(uint2*)(qs + r2 * 64 + (((c >> 1) ^ ((r2 >> 1) & 3)) << 4) + (c & 1) * 8) = make_uint2(l4[0], l4[1]);
+            // rows of 64 bytes; the second term N rows further (a whole number of groups of 8)
+            const int at = r * 64 + (((c >> 1) ^ ((r >> 1) & 3)) << 4) + (c & 1) * 8;
+            *(uint2*)(qs + at) = make_uint2(h4[0], h4[1]);
+            *(uint2*)(qs + N * 64 + at) = make_uint2(l4[0], l4[1]);
           }
         }
         if (tid < N) nref[tid] = tid < nrows ? INFINITY : -INFINITY;  // unused rows: P = 0
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        ch_named_sync(1 + s, 128);
+        ch_named_sync(1 + s, kBar);
         if (lane == 0) mbar_arrive(&qfull[s]);
       } else if (!mine || ntile == 0) {
         // an idle stream keeps the barriers' count of segments
@@ -536,56 +560,50 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
       for (int i = 0; i < ntile; ++i, ++it) {
         const int st = it % NS;
         if (!mine) continue;
-        const int32_t j = sg.j0 + i * kKeysKT + tid;
-        // rows [r_lo, r_hi) see this key
-        int r_lo = 0, r_hi = nrows;
-        const int32_t jt = sg.j0 + i * kKeysKT;
-        const bool whole = jt + kKeysKT - 1 <= first_pos && jt >= lo &&
+        const int32_t j = sg.j0 + i * KT + key;
+        // of this thread's rows, [r_lo, r_hi) see its key
+        int r_lo = 0, r_hi = mine_rows;
+        const int32_t jt = sg.j0 + i * KT;
+        const bool whole = jt + KT - 1 <= first_pos && jt >= lo &&
                            (p.window <= 0 || jt > first_pos + sg.ntok - 1 - p.window);
         if (!whole) {
-          r_lo = max(0, min(j - first_pos, 1 << 16)) * p.G;
-          if (p.window > 0) r_hi = min(nrows, max(0, min(j + p.window - first_pos, 1 << 16)) * p.G);
+          r_lo = max(0, min(j - first_pos, 1 << 16)) * p.G - rb;
+          if (p.window > 0) r_hi = min(r_hi, max(0, min(j + p.window - first_pos, 1 << 16)) * p.G - rb);
         }
         float kf = p.scale2, ev = 0.f, einv = 1.f;
         if (F8 || !whole) {
           if (!bad) bad = !mbar_wait(&vfull[st], (uint32_t)(it / NS) & 1u, p.err, kErrTimeoutFull);
         }
         if (F8) {
-          const uint8_t* cc = smem + C::kOffCodes + st * C::kCodes + s * kKeysKT + tid;
-          const uint32_t kc = cc[0], vc = cc[2 * kKeysKT];
+          const uint8_t* cc = smem + C::kOffCodes + st * C::kCodes + s * KT + key;
+          const uint32_t kc = cc[0], vc = cc[2 * KT];
           const float nan = __uint_as_float(0x7FC00000u);
           kf = kc == 255u ? nan : p.scale2 * q_unit * __uint_as_float(kc << 23);
           ev = vc == 255u ? nan : (float)((int)vc - 127);
           einv = __uint_as_float((254u - min(vc, 253u)) << 23);
         }
-        if (!whole && (j < lo || j >= hi)) {
+        if (!whole && (j < lo || j >= hi) && (!C::kSplit || part == 0)) {
           // a key nobody may see: 0 times what its V row (or an earlier tile) holds must be 0
           // (swizzled within the row, but for two heads in one row: 16-byte piece c of head s is 4 s + c)
           uint8_t* vr = smem + st * 2 * C::kSide + C::kSide +
-                        (F8 ? tid * (HB * RB) : ((tid >> 3) * HB + s) * 8 * RB + (tid & 7) * RB);
+                        (F8 ? key * (HB * RB) : ((key >> 3) * HB + s) * 8 * RB + (key & 7) * RB);
 #pragma unroll
           for (int c = 0; c < RB / 16; ++c)
-            *(uint4*)(vr + (F8 && HB == 2 ? (4 * s + c) ^ (tid & 7) : c) * 16) = make_uint4(0, 0, 0, 0);
+            *(uint4*)(vr + (F8 && HB == 2 ? (4 * s + c) ^ (key & 7) : c) * 16) = make_uint4(0, 0, 0, 0);
         }
         if (!bad) bad = !mbar_wait(&sfull[s], (uint32_t)it & 1u, p.err, kErrTimeoutAccum);
         tc_fence_after();
-        ch_f2 x[N / 2];
+        ch_f2 x[NR / 2];
         const ch_f2 kf2 = ch_pair(kf, kf), ev2 = ch_pair(ev, ev);
-        // t - m (nm: -m of the rows) of 8 rows from TMEM; -inf where the key is hidden from the row
+        // t - m (nm: -m of the rows) of this thread's rows r0 .. + 7 from TMEM; -inf where the key is hidden from one
         auto scores = [&](int r0, ch_f2 (&t)[4], const ch_f2 (&nm)[4]) {
-          uint32_t a[8], b[8];
+          uint32_t a[8];
           ch_ld8(t_s + r0, a);
-          if (F8) ch_ld8(t_s + N + r0, b);
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            ch_f2 v = ((ch_f2)a[2 * e + 1] << 32) | a[2 * e];
-            if (F8) {
-              v = ch_fma2(((ch_f2)b[2 * e + 1] << 32) | b[2 * e], ch_pair(0.0625f, 0.0625f), v);
-              t[e] = ch_add2(ch_fma2(v, kf2, ev2), nm[e]);
-            } else {
-              t[e] = ch_fma2(v, kf2, nm[e]);
-            }
+            const ch_f2 v = ((ch_f2)a[2 * e + 1] << 32) | a[2 * e];
+            t[e] = F8 ? ch_add2(ch_fma2(v, kf2, ev2), nm[e]) : ch_fma2(v, kf2, nm[e]);
           }
           if (!whole) {
 #pragma unroll
@@ -596,18 +614,21 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
             }
           }
         };
+        auto refs = [&](int r0, ch_f2 (&nm)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const ulonglong2 y = *(const ulonglong2*)(nref + rb + r0 + 2 * e);
+            nm[e] = y.x;
+            nm[e + 1] = y.y;
+          }
+        };
         for (int again = 0;; ++again) {
           float mx = -INFINITY;
 #pragma unroll
-          for (int r0 = 0; r0 < N; r0 += 8) {
-            if (r0 < nrows) {
+          for (int r0 = 0; r0 < NR; r0 += 8) {
+            if (r0 < mine_rows) {
               ch_f2 t[4], nm[4];
-#pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                const ulonglong2 y = *(const ulonglong2*)(nref + r0 + 2 * e);
-                nm[e] = y.x;
-                nm[e + 1] = y.y;
-              }
+              refs(r0, nm);
               scores(r0, t, nm);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -617,35 +638,37 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
             }
           }
           // the second time round nothing is left above the reference's reach
-          if (!ch_named_or(1 + s, 128, mx > kUp) || again) break;
+          if (!ch_named_or(1 + s, kBar, mx > kUp) || again) break;
           const ch_f2 zero[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll 1
-          for (int r0 = 0; r0 < nrows; r0 += 8) {
+          for (int r0 = 0; r0 < mine_rows; r0 += 8) {
             ch_f2 t[4];
             scores(r0, t, zero);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float m0 = ch_warp_max(ch_lo(t[e])), m1 = ch_warp_max(ch_hi(t[e]));
-              if (lane == 0) *(float2*)(red + wq * N + r0 + 2 * e) = make_float2(m0, m1);
+              if (lane == 0) *(float2*)(red + sum_at * N + rb + r0 + 2 * e) = make_float2(m0, m1);
             }
           }
-          ch_named_sync(3 + s, 128);
+          ch_named_sync(3 + s, kBar);
           if (tid < nrows) {
-            const float m = fmaxf(fmaxf(red[tid], red[N + tid]), fmaxf(red[2 * N + tid], red[3 * N + tid]));
+            float m = red[tid];
+#pragma unroll
+            for (int w = 1; w < kSums; ++w) m = fmaxf(m, red[w * N + tid]);
             const float m0 = -nref[tid], m1 = m > m0 + kUp ? m - kBase : m0;
             fac[tid] = m1 == m0 ? 1.0f : ch_exp2(m0 - m1);
             nref[tid] = -m1;
           }
-          ch_named_sync(3 + s, 128);
+          ch_named_sync(3 + s, kBar);
 #pragma unroll
-          for (int r = 0; r < N; r += 2)
-            if (r < nrows) l[r / 2] = ch_mul2(l[r / 2], *(const ch_f2*)(fac + r));
+          for (int r = 0; r < NR; r += 2)
+            if (r < mine_rows) l[r / 2] = ch_mul2(l[r / 2], *(const ch_f2*)(fac + rb + r));
           if (i > 0) {
             // O^T of the tiles before, once their products are done
             if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
             tc_fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < W; c0 += 8) {
+            for (int c0 = part * 8; c0 < W; c0 += 8 * kParts) {
               const int r0 = F8 && c0 >= N ? c0 - N : c0;
               if (r0 >= nrows) continue;
               uint32_t o8[8];
@@ -665,41 +688,35 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
         if (i > 0) {
           if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
         }
-        uint8_t* pr = ps + tid * 128;
-        const int sw = tid & 7;
+        uint8_t* pr = ps + key * 128;
+        const int sw = (key & 7) << 4;
         const ch_f2 einv2 = ch_pair(einv, einv);
-        constexpr int kPer = F8 ? 16 : 8;  // rows of a 16-byte piece
 #pragma unroll
-        for (int r0 = 0; r0 < N; r0 += kPer) {
-          if (r0 >= nrows) break;  // columns of rows that are not there: whatever they hold, nobody reads their results
-          uint32_t w[4], w2[4];
+        for (int r0 = 0; r0 < NR; r0 += 8) {
+          if (r0 >= mine_rows) break;  // columns of rows that are not there: nobody reads their results
+          uint32_t w[4], hl[4];  // bf16: 16 bytes; 8 bit: 8 of each term
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            ch_f2 pe[kPer / 8];
-#pragma unroll
-            for (int y = 0; y < kPer / 8; ++y) {
-              const int k = r0 / 2 + e * (kPer / 8) + y;
-              pe[y] = ch_pair(ch_exp2(ch_lo(x[k])), ch_exp2(ch_hi(x[k])));
-              l[k] = F8 ? ch_fma2(pe[y], einv2, l[k]) : ch_add2(pe[y], l[k]);
-            }
+            const ch_f2 v = x[r0 / 2 + e], pe = ch_pair(ch_exp2(ch_lo(v)), ch_exp2(ch_hi(v)));
+            l[r0 / 2 + e] = F8 ? ch_fma2(pe, einv2, l[r0 / 2 + e]) : ch_add2(pe, l[r0 / 2 + e]);
             if (!F8) {
-              w[e] = ch_bf16x2(ch_lo(pe[0]), ch_hi(pe[0]));
+              w[e] = ch_bf16x2(ch_lo(pe), ch_hi(pe));
             } else {
               // hi: 4 significant bits; lo: 16 times the rest
-              uint32_t h4[2], l4[2];
-#pragma unroll
-              for (int y = 0; y < kPer / 8; ++y) {
-                const ch_f2 h = ch_pair(ch_round4(ch_lo(pe[y])), ch_round4(ch_hi(pe[y])));
-                const ch_f2 d = ch_mul2(ch_fma2(h, ch_pair(-1.f, -1.f), pe[y]), ch_pair(16.f, 16.f));
-                h4[y] = ch_e4m3x2(ch_lo(h), ch_hi(h));
-                l4[y] = ch_e4m3x2(ch_lo(d), ch_hi(d));
-              }
-              w[e] = h4[0] | (h4[kPer / 8 - 1] << 16);
-              w2[e] = l4[0] | (l4[kPer / 8 - 1] << 16);
+              const ch_f2 h = ch_pair(ch_round4(ch_lo(pe)), ch_round4(ch_hi(pe)));
+              const ch_f2 d = ch_mul2(ch_fma2(h, ch_pair(-1.f, -1.f), pe), ch_pair(16.f, 16.f));
+              w[e] = ch_e4m3x2(ch_lo(h), ch_hi(h));
+              hl[e] = ch_e4m3x2(ch_lo(d), ch_hi(d));
             }
           }
-          *(uint4*)(pr + (((r0 / kPer) ^ sw) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (F8) *(uint4*)(pr + ((((N + r0) / kPer) ^ sw) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+          const int b = (rb + r0) * (F8 ? 1 : 2);  // byte of the row's place
+          if (!F8) {
+            *(uint4*)(pr + (b ^ sw)) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+            *(uint2*)(pr + ((b & ~15) ^ sw) + (b & 8)) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+            const int b2 = N + b;
+            *(uint2*)(pr + ((b2 & ~15) ^ sw) + (b2 & 8)) = make_uint2(hl[0] | (hl[1] << 16), hl[2] | (hl[3] << 16));
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -713,21 +730,29 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
           if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
           tc_fence_after();
         }
-        // sums over the keys
+        // sums over the keys, 8 rows side by side
 #pragma unroll
-        for (int r = 0; r < N; ++r) {
-          if (r < nrows) {
-            float v = r & 1 ? ch_hi(l[r / 2]) : ch_lo(l[r / 2]);
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) red[wq * N + r] = v;
+        for (int r0 = 0; r0 < NR; r0 += 8) {
+          if (r0 < mine_rows) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e & 1 ? ch_hi(l[(r0 + e) / 2]) : ch_lo(l[(r0 + e) / 2]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], o);
+            if (lane == 0) {
+#pragma unroll
+              for (int e = 0; e < 8; e += 4) *(float4*)(red + sum_at * N + rb + r0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
           }
         }
-        // O^T from TMEM to rows of 64 floats in P's place: lane < 16 of warp wq holds dim 16 wq + lane
+        // O^T from TMEM to rows of 64 floats in P's place: a lane below 16 of warp wq holds dim 16 (wq mod 4) + lane
         float* os = (float*)ps;
         if (ntile > 0) {
 #pragma unroll
           for (int r0 = 0; r0 < N; r0 += 8) {
-            if (r0 < nrows) {
+            if (r0 < nrows && (kParts == 1 || (r0 >> 3 & 1) == part)) {
               uint32_t a[8], b[8];
               ch_ld8(t_o + r0, a);
               if (F8) ch_ld8(t_o + N + r0, b);
@@ -735,21 +760,23 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
               if (lane < 16) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  os[(r0 + e) * 64 + wq * 16 + lane] =
+                  os[(r0 + e) * 64 + (wq & 3) * 16 + lane] =
                       F8 ? fmaf(__uint_as_float(b[e]), 0.0625f, __uint_as_float(a[e])) : __uint_as_float(a[e]);
               }
             }
           }
         }
         tc_fence_before();
-        ch_named_sync(3 + s, 128);
-        for (int x = tid; x < nrows * 16; x += 128) {
+        ch_named_sync(3 + s, kBar);
+        for (int x = tid; x < nrows * 16; x += kBar) {
           const int r = x >> 4, d = (x & 15) * 4;
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
           float lr = 0.f, m = -INFINITY;
           if (ntile > 0) {
             y = *(const float4*)(os + r * 64 + d);
-            lr = red[r] + red[N + r] + red[2 * N + r] + red[3 * N + r];
+            lr = red[r];
+#pragma unroll
+            for (int w = 1; w < kSums; ++w) lr += red[w * N + r];
             m = -nref[r];
           }
           if (slot >= 0) {
@@ -765,23 +792,23 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
                 make_uint2(ch_bf16x2(y.x * inv, y.y * inv), ch_bf16x2(y.z * inv, y.w * inv));
           }
         }
-        ch_named_sync(3 + s, 128);  // red, nref and os are free again
+        ch_named_sync(3 + s, kBar);  // red, nref and os are free again
       }
       if (slot >= 0) {
         __threadfence();
-        ch_named_sync(5, 256);
+        ch_named_sync(5, 2 * kBar);
         if (threadIdx.x == 0) {
           const uint32_t old = atomicAdd(&p.counters[sg.c0], 1u);
           const uint32_t last = old == (uint32_t)(sg.c1 - sg.c0);
           if (last) p.counters[sg.c0] = 0u;
           *flag = last;
         }
-        ch_named_sync(6, 256);
+        ch_named_sync(6, 2 * kBar);
         if (*flag) {
           __threadfence();
-          chunk_join(p, sg, HB, N, threadIdx.x, 256);
+          chunk_join(p, sg, HB, N, threadIdx.x, 2 * kBar);
         }
-        ch_named_sync(5, 256);  // flag is free again
+        ch_named_sync(5, 2 * kBar);  // flag is free again
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[sb]);
@@ -789,7 +816,7 @@ __global__ void __launch_bounds__(kKeysThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMma0) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmem);
@@ -1328,9 +1355,9 @@ int launch_keys(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
   const int HB = p.Hkv % 2 ? 1 : 2;  // with an odd number of kv heads one stream idles
   p.TQ = N_ / p.G;
   p.HG = p.Hkv / HB;
-  p.lg_kt = 7;
-  p.ov = 3;
-  if (!chunk_fits(p, kKeysKT)) return -12;
+  p.lg_kt = C::KT == 256 ? 8 : 7;
+  p.ov = C::KT == 256 ? 2 : 3;
+  if (!chunk_fits(p, C::KT)) return -12;
   p.part_ml = p.part_o + (int64_t)2 * grid * HB * N_ * kChunkD;
   CUtensorMap tk, tv;
   const uint64_t rb = C::kRowBytes, tok = (uint64_t)p.Hkv * rb;
@@ -1344,7 +1371,7 @@ int launch_keys(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
   const uint32_t box[4] = {(uint32_t)width, 8, (uint32_t)(pair ? 1 : HB), 2};
   const CUtensorMapSwizzle sw = F8 && !pair ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   if (make_tmap_4d(&tk, k, dt, dims, strides, box, sw) || make_tmap_4d(&tv, v, dt, dims, strides, box, sw)) return -2;
-  chunk_keys_kernel<F8, N_><<<(unsigned)grid, kKeysThreads, C::kAlloc, s>>>(tk, tv, p, HB);
+  chunk_keys_kernel<F8, N_><<<(unsigned)grid, C::kThreads, C::kAlloc, s>>>(tk, tv, p, HB);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
