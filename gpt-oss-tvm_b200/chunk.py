@@ -150,10 +150,10 @@ def attend_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                               or not sinks.is_contiguous() or sinks.get_device() != index):
         _bad(f"sinks must be a dense bfloat16 tensor [{Hq}] on cuda:{index}")
     if out is None:
-        out = torch.empty((T, Hq, HEAD_DIM), dtype=_BF16, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, Hq, HEAD_DIM))
     elif out.dtype is not _BF16 or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index:
         _bad("out must be a dense bfloat16 tensor of q's shape on its device")
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and n:
         ws = workspace
         if ws is None:
@@ -195,7 +195,7 @@ def rope_append_f8(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tens
             _bad(f"inv_freq must be {HEAD_DIM // 2} values")
         inv_p = ctypes.addressof(inv_freq)
     if q_out is None:
-        q_out = torch.empty((T, num_heads, HEAD_DIM), dtype=_BF16, device=qkv.device)
+        q_out = qkv.new_empty((T, num_heads, HEAD_DIM))
     elif (q_out.dtype is not _BF16 or q_out.shape != (T, num_heads, HEAD_DIM) or not q_out.is_contiguous()
           or q_out.get_device() != index):
         _bad(f"q_out must be a dense bfloat16 tensor [{T}, {num_heads}, {HEAD_DIM}] on cuda:{index}")
@@ -228,8 +228,8 @@ def read_pages_f8(k_pages, v_pages, k_scale, v_scale, page_table, seq: int, pos0
     """Keys and values of positions pos0 .. pos0 + n - 1 of sequence ``seq`` as
     bf16 rows [n, kv heads, 64] (exact)."""
     shape = (n, k_pages.shape[1], HEAD_DIM)
-    k_out = torch.empty(shape, dtype=_BF16, device=k_pages.device) if k_out is None else k_out
-    v_out = torch.empty(shape, dtype=_BF16, device=k_pages.device) if v_out is None else v_out
+    k_out = k_pages.new_empty(shape, dtype=_BF16) if k_out is None else k_out
+    v_out = torch.empty_like(k_out) if v_out is None else v_out
     _copy_f8(k_pages, v_pages, k_scale, v_scale, page_table, seq, pos0, n, k_out, v_out, False)
     return k_out, v_out
 

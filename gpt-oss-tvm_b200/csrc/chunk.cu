@@ -250,7 +250,7 @@ struct KeysCfg {
   static constexpr int kRowBytes = F8 ? 64 : 128;
   static constexpr int kSide = 2 * KT * kRowBytes;         // K or V of a tile, two heads
   static constexpr int kCodes = F8 ? 2 * 2 * KT : 0;       // [K, V][head][KT]
-  static constexpr int kStages = 2;
+  static constexpr int kStages = F8 && kSplit ? 4 : 2;
   static constexpr int kQ = N * 128;                       // per stream: N rows of 128 bytes, or 2 N of 64
   static constexpr int kP = KT * 128;                      // per stream
   static constexpr int kColO = 2 * (KT / 128) * N;         // S^T: N columns per stream and 128 keys, then O^T

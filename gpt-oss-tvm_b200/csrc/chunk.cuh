@@ -102,16 +102,20 @@ struct ChunkSeg {
 // The host has made sure that the total fits 31 bits.
 __device__ __forceinline__ void chunk_plan(const ChunkParams& p, int32_t* pre, int nthreads) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = nthreads >> 5;
-  for (int b = warp; b < p.N; b += nw) {
+  // a warp per sequence while there are enough, its lanes over the groups of tokens; else a thread per sequence
+  const bool wide = p.N <= nw;
+  const int step = wide ? 32 : 1, first = wide ? lane : 0;
+  for (int b = wide ? warp : (int)threadIdx.x; b < p.N; b += wide ? nw : nthreads) {
     const ChunkSeq s = chunk_seq(p, b);
     const int nt = (s.ql + p.TQ - 1) / p.TQ;
     int32_t w = 0;
-    for (int t = lane; t < nt; t += 32) {
+    for (int t = first; t < nt; t += step) {
       int32_t lo, hi;
       w += max(1, chunk_tiles(p, s, t, lo, hi)) + p.ov;
     }
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    if (lane == 0) pre[b + 1] = w * p.HG;
+    if (wide)
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (!wide || lane == 0) pre[b + 1] = w * p.HG;
   }
   __syncthreads();
   if (warp == 0) {

@@ -45,7 +45,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.T
         _bad(f"draft_probs must be a float32 tensor [{T}, {V}] with dense rows on cuda:{index}")
     # one allocation: the two answers, then the library's scratch
     nbytes = _lib.load().gptoss_verify_drafts_scratch_bytes(T, V)
-    buf = torch.empty(2 * n + nbytes // 4 + 1, dtype=torch.int32, device=logits.device)
+    buf = tokens.new_empty(2 * n + nbytes // 4 + 1)
     if n:
         p = buf.data_ptr()
         _run(index, "gptoss_verify_drafts", logits.data_ptr(), logits.dtype is torch.bfloat16,
