@@ -21,6 +21,11 @@ only; the attention semantics (append before attention, window of the last W
 keys including the current token) are the reference's (tvm_fix.patch:35-47,
 :194-281).  A prefill / extend chunk attends over one contiguous buffer: the
 cached keys its window can reach, gathered from the pages, then its own.
+
+Beyond the reference: new tokens of several sequences at once
+(``forward_to="chunk"``, after ``KVCache.begin_chunks``) attend over the pages
+directly, and the pages may hold 8-bit values (``kv_dtype="float8_e4m3"``): see
+chunk.py.
 """
 from __future__ import annotations
 
@@ -29,7 +34,7 @@ import ctypes
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, chunk
 from .config import GPTOssConfig
 
 
@@ -64,10 +69,21 @@ class KVCache:
     the device (``begin_decode_on_device``) inside a CUDA graph; the
     decode-step buffers never move, so a captured graph keeps reading the
     current values.  ``check_decode`` makes sure every decoding sequence has a
-    page for its next token (host allocation, device table refreshed)."""
+    page for its next token (host allocation, device table refreshed).
+
+    kv_dtype: "bfloat16", or "float8_e4m3": e4m3 values with one power of two
+    per row and head (``k_scale`` / ``v_scale``, chunk.py), a little over half
+    the memory.  max_chunk: the most tokens of one sequence that
+    ``begin_chunks`` appends at a time; the window rings are that much longer,
+    since a chunk is appended before it attends (and a rejected draft is popped
+    without losing the window)."""
 
     def __init__(self, config: GPTOssConfig, max_batch: int, max_len: int, num_layers: int | None = None,
-                 device="cuda", window_pages: int | None = None):
+                 device="cuda", window_pages: int | None = None, kv_dtype: str = "bfloat16", max_chunk: int = 1):
+        if kv_dtype not in ("bfloat16", "float8_e4m3"):
+            raise ValueError(f"KVCache: kv_dtype {kv_dtype!r} is neither 'bfloat16' nor 'float8_e4m3'")
+        if max_chunk < 1:
+            raise ValueError("KVCache: max_chunk must be at least 1")
         if max_batch < 1 or max_len < 1 or max_batch * (max_len + PAGE_SIZE) >= 2 ** 31:
             raise ValueError(f"KVCache: max_batch x max_len = {max_batch} x {max_len} must fit int32 rows")
         self.config = config
@@ -76,7 +92,8 @@ class KVCache:
         Hkv, D = config.num_key_value_heads, config.head_dim
         self.window = int(config.sliding_window_size)
         self.pages_per_seq = -(-max_len // PAGE_SIZE)                    # table stride, full layers
-        self.window_pages = window_pages or (-(-self.window // PAGE_SIZE) + 1)
+        self.max_chunk = max_chunk
+        self.window_pages = window_pages or (-(-(self.window + max_chunk - 1) // PAGE_SIZE) + 1)
         if self.window_pages * PAGE_SIZE < self.window + PAGE_SIZE - 1:
             raise ValueError("window_pages must cover the window plus the page being filled")
         self.full_pool_pages = max_batch * self.pages_per_seq
@@ -85,10 +102,18 @@ class KVCache:
         bf = dict(dtype=torch.bfloat16, device=dev)
         self.windowed = [(i % config.sliding_window_pattern == 0) and self.window > 0 for i in range(L)]
         self.k, self.v = [], []
-        for w in self.windowed:
-            rows = (max_batch * self.window_pages if w else self.full_pool_pages) * PAGE_SIZE
-            self.k.append(torch.zeros(rows, Hkv, D, **bf))
-            self.v.append(torch.zeros(rows, Hkv, D, **bf))
+        self.f8 = kv_dtype == "float8_e4m3"
+        self.k_scale, self.v_scale = [None] * L, [None] * L
+        for i, w in enumerate(self.windowed):
+            pages = max_batch * self.window_pages if w else self.full_pool_pages
+            if self.f8:
+                if D != chunk.HEAD_DIM:
+                    raise ValueError(f"KVCache: 8-bit pages need head_dim {chunk.HEAD_DIM}")
+                (k, self.k_scale[i]), (v, self.v_scale[i]) = (chunk.f8_pool(pages, Hkv, dev) for _ in range(2))
+            else:
+                k, v = (torch.zeros(pages * PAGE_SIZE, Hkv, D, **bf) for _ in range(2))
+            self.k.append(k)
+            self.v.append(v)
         i32 = dict(dtype=torch.int32, device=dev)
         # full layers: page lists (host) and their device mirror; windowed layers: fixed rings
         self._free = list(range(self.full_pool_pages - 1, -1, -1))
@@ -113,6 +138,10 @@ class KVCache:
         self._slot = torch.zeros(max_batch, **i32)
         self._slot_win = torch.zeros(max_batch, **i32)
         self._cur = None
+        # one token for each of sequences 0..B-1, as chunks; and the chunks of begin_chunks
+        self._one_each = torch.arange(max_batch + 1, **i32)
+        self.q_start = self.seq_rows = None
+        self.max_q = 1
         self.start = 0  # first position of the current prefill / extend chunk
 
     # ------------------------------------------------------------- pages --
@@ -199,6 +228,31 @@ class KVCache:
         self.positions, self.kv_len = self._pos[:T], self._kv_len[:nb]
         self.slots, self.slots_win = self._slot[:T], self._slot_win[:T]
         return self.positions
+
+    def begin_chunks(self, seq_ids, append_lengths):
+        """begin_forward for new tokens of several sequences that attend over
+        the pages in one call (``forward_to="chunk"``): also the chunks' first
+        rows (``q_start``) and page-table rows (``seq_rows``) on the device."""
+        seq_ids, append_lengths = list(seq_ids), list(append_lengths)
+        if len(set(seq_ids)) != len(seq_ids) or len(seq_ids) != len(append_lengths) or not seq_ids:
+            raise ValueError("begin_chunks takes distinct sequences and one length for each")
+        if min(append_lengths) < 1:
+            raise ValueError("begin_chunks: every sequence needs a new token")
+        if self.window > 0 and any(self.windowed):
+            for s, n in zip(seq_ids, append_lengths):
+                start = int(self.lengths[s]) if 0 <= s < self.max_batch else 0
+                first = max(0, start - self.window + 1) // PAGE_SIZE
+                if (start + n - 1) // PAGE_SIZE - first + 1 > self.window_pages:
+                    raise ValueError(f"a chunk of {n} tokens does not fit the sliding-window rings of "
+                                     f"{self.window_pages} pages beside its window (KVCache max_chunk)")
+        positions = self.begin_forward(seq_ids, append_lengths)
+        starts = [0]
+        for n in append_lengths:
+            starts.append(starts[-1] + n)
+        both = torch.tensor(starts + seq_ids, dtype=torch.int32).to(self.device)
+        self.q_start, self.seq_rows = both[:len(starts)], both[len(starts):]
+        self.max_q = max(append_lengths)
+        return positions
 
     def slots_for(self, layer_idx: int):
         return self.slots_win if self.windowed[layer_idx] else self.slots
@@ -308,8 +362,14 @@ class KVCache:
                 a, b = src_rows.to(self.device), dst_rows.to(self.device)
             else:
                 continue
-            self.k[i].index_copy_(0, b, self.k[i].index_select(0, a))
-            self.v[i].index_copy_(0, b, self.v[i].index_select(0, a))
+            for t in (self.k[i], self.v[i]):
+                t = t.view(torch.uint8) if self.f8 else t
+                t.index_copy_(0, b, t.index_select(0, a))
+            if self.f8:  # whole pages: their first rows name them
+                pa, pb = a[::PAGE_SIZE] // PAGE_SIZE, b[::PAGE_SIZE] // PAGE_SIZE
+                for t in (self.k_scale[i], self.v_scale[i]):
+                    t = t.view(torch.uint8)
+                    t.index_copy_(0, pb, t.index_select(0, pa))
         self.lengths[dst] = n
         self._written[dst] = self._written[src]
         self._sync_dev_lengths()
@@ -325,10 +385,18 @@ class KVCache:
         else:
             rows = self.table_full_host[seq][p // PAGE_SIZE].long() * PAGE_SIZE + p % PAGE_SIZE
         rows = rows.to(self.k[layer_idx].device)
+        if self.f8:
+            out = []
+            for t, c in ((self.k, self.k_scale), (self.v, self.v_scale)):
+                x = t[layer_idx].view(torch.uint8).index_select(0, rows).view(torch.float8_e4m3fn).float()
+                c = c[layer_idx][rows // PAGE_SIZE, :, rows % PAGE_SIZE].float()
+                out.append((x * c.unsqueeze(-1)).to(torch.bfloat16))
+            return tuple(out)
         return self.k[layer_idx].index_select(0, rows), self.v[layer_idx].index_select(0, rows)
 
     def memory_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.k + self.v)
+        return sum(t.numel() * t.element_size() for t in self.k + self.v + self.k_scale + self.v_scale
+                   if t is not None)
 
 
 DENSE_GEMV = False  # decode-size projections through gptoss_dense_gemv instead of cuBLAS
@@ -369,6 +437,14 @@ class DecodeScratch:
     def __init__(self, device):
         self.device = torch.device(device)
         self.buf = None
+        self._chunk = None
+
+    def chunk(self) -> "chunk.ChunkWorkspace":
+        """The workspace of attend_chunks (made on its first use, before a
+        step is captured)."""
+        if self._chunk is None:
+            self._chunk = chunk.ChunkWorkspace(self.device)
+        return self._chunk
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf is None or self.buf.numel() * 4 < nbytes:
@@ -431,7 +507,9 @@ class AttentionBlock:
 
     def forward(self, x: torch.Tensor, kv_cache: KVCache, query_positions: torch.Tensor | None, forward_to: str):
         """x [b, s, hidden] bf16.  prefill / extend: one sequence (b = 1, the
-        reference's batch size); decode: one token per sequence of the batch."""
+        reference's batch size); decode: one token per sequence of the batch;
+        chunk: the tokens of the cache's begin_chunks, one sequence after
+        another."""
         H, D = self.config.hidden_size, self.head_dim
         Hq, Hkv = self.num_attention_heads, self.num_key_value_heads
         shape = x.shape
@@ -461,15 +539,41 @@ class AttentionBlock:
             vb = torch.empty_like(kb)
             _lib.call("gptoss_qkv_rope_append", _ptr(qkv), _ptr(pos), None, T, Hq, Hkv, D, self._inv_freq,
                       ctypes.c_float(self._conc), _ptr(q), _ptr(kb[ctx:]), _ptr(vb[ctx:]), S)
-            if ctx > 0:
+            if ctx > 0 and kv_cache.f8:
+                chunk.read_pages_f8(kc, vc, kv_cache.k_scale[L], kv_cache.v_scale[L], table, sid, g0, ctx, kb[:ctx],
+                                    vb[:ctx])
+            elif ctx > 0:
                 _lib.call("gptoss_kv_pages_copy", _ptr(kc), _ptr(vc), Hkv, D, _ptr(table), stride, sid, g0, ctx,
                           _ptr(kb), _ptr(vb), 0, S)
             # append_mha_kv: the chunk into the pages (a ring keeps its last rows only)
             keep = T if not kv_cache.windowed[L] else min(T, stride * PAGE_SIZE)
-            _lib.call("gptoss_kv_pages_copy", _ptr(kc), _ptr(vc), Hkv, D, _ptr(table), stride, sid,
-                      start + T - keep, keep, _ptr(kb[ctx + T - keep:]), _ptr(vb[ctx + T - keep:]), 1, S)
+            if kv_cache.f8:
+                chunk.write_pages_f8(kb[ctx + T - keep:], vb[ctx + T - keep:], kc, vc, kv_cache.k_scale[L],
+                                     kv_cache.v_scale[L], table, sid, start + T - keep)
+            else:
+                _lib.call("gptoss_kv_pages_copy", _ptr(kc), _ptr(vc), Hkv, D, _ptr(table), stride, sid,
+                          start + T - keep, keep, _ptr(kb[ctx + T - keep:]), _ptr(vb[ctx + T - keep:]), 1, S)
             _lib.call("gptoss_attn_prefill", _ptr(q), _ptr(kb), _ptr(vb), _ptr(self.sinks), T, ctx + T, Hq, Hkv, D,
                       self.sliding_window, ctypes.c_float(self.sm_scale), _ptr(o), None, S)
+        elif forward_to == "chunk" or (forward_to == "decode" and kv_cache.f8):
+            if forward_to == "decode":
+                if any(n != 1 for n in lens) or list(seq_ids) != list(range(len(seq_ids))):
+                    raise ValueError("decode takes one token for each of sequences 0..B-1")
+                q_start, seq_rows = kv_cache._one_each[:len(seq_ids) + 1], kv_cache._one_each[:len(seq_ids)]
+                max_q = 1
+            else:
+                if kv_cache.q_start is None or sum(lens) != T:
+                    raise ValueError("chunk takes the tokens that KVCache.begin_chunks planned")
+                q_start, seq_rows, max_q = kv_cache.q_start, kv_cache.seq_rows, kv_cache.max_q
+            ks, vs = kv_cache.k_scale[L], kv_cache.v_scale[L]
+            if kv_cache.f8:
+                chunk.rope_append_f8(qkv, pos, kv_cache.slots_for(L), Hq, self._inv_freq, self._conc, kc, vc, ks, vs, q)
+            else:
+                _lib.call("gptoss_qkv_rope_append", _ptr(qkv), _ptr(pos), _ptr(kv_cache.slots_for(L)), T, Hq, Hkv, D,
+                          self._inv_freq, ctypes.c_float(self._conc), _ptr(q), _ptr(kc), _ptr(vc), S)
+            chunk.attend_chunks(q, kc, vc, table, seq_rows, q_start, kv_cache.kv_len, max_q=max_q,
+                                window=self.sliding_window, sm_scale=self.sm_scale, sinks=self.sinks, k_scale=ks,
+                                v_scale=vs, out=o, workspace=self.scratch.chunk())
         elif forward_to == "decode":
             if any(n != 1 for n in lens) or min(seq_ids) != 0 or list(seq_ids) != list(range(len(seq_ids))):
                 raise ValueError("decode takes one token for each of sequences 0..B-1")

@@ -1139,7 +1139,9 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
       const int32_t lo = sg.lo, hi = sg.hi;
       const int32_t pos = row_ok ? sg.first_pos + tok : -1;
       const int32_t tile_first = sg.first_pos + t * tq1, tile_last = sg.first_pos + min(ntok, (t + 1) * tq1) - 1;
-      float m_ref = -INFINITY, l = 0.f, pend = 1.0f;  // pend: what O_t is still to be multiplied by
+      // a row that is not in use has whatever its place in shared memory held for a query: scale 0, reference 0
+      const float scale = row_ok ? p.scale2 : 0.f;
+      float m_ref = row_ok ? -INFINITY : 0.f, l = 0.f, pend = 1.0f;  // pend: what O_t is still to be multiplied by
       if (tile_on) {
         for (int i = 0; i < ntile; ++i) {
           const int32_t j0 = sg.j0 + i * kRowsKT;
@@ -1174,7 +1176,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
               if (kj > pos || (p.window > 0 && kj <= pos - p.window)) r[e] = __float_as_uint(-INFINITY);
             }
           };
-          if (__any_sync(0xffffffffu, m_ref == -INFINITY && row_ok)) {
+          if (__any_sync(0xffffffffu, m_ref == -INFINITY)) {
             // a row without a reference takes the largest score of its first tile (scale2 > 0)
             float mx = -INFINITY;
 #pragma unroll 1
@@ -1186,7 +1188,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
             }
-            if (m_ref == -INFINITY) m_ref = mx * p.scale2;  // nothing of it in O or l yet
+            if (m_ref == -INFINITY) m_ref = mx * scale;  // nothing of it in O or l yet
           }
           // P_t and O_t are free once the products of the tile before are done
           if (i > 0) {
@@ -1194,10 +1196,10 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
             tc_fence_after();
           }
           float sum, mx;
-          for (;;) {
+          for (int again = 0;; ++again) {
             // P = 2^(s - m) two at a time, the next 32 scores on their way meanwhile
             const float m_eff = m_ref == -INFINITY ? 0.f : m_ref;  // nothing seen so far: every P is 0
-            const ch_f2 sc2 = ch_pair(p.scale2, p.scale2), nm2 = ch_pair(-m_eff, -m_eff);
+            const ch_f2 sc2 = ch_pair(scale, scale), nm2 = ch_pair(-m_eff, -m_eff);
             ch_f2 sum2 = 0ull;
             mx = -INFINITY;
             auto chunk = [&](uint32_t (&r)[32], int e0) {
@@ -1225,8 +1227,9 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
               chunk(rb, e0 + 32);
             }
             sum = ch_lo(sum2) + ch_hi(sum2);
-            // The reference follows a tile later, P and l have room: 2^64.  Beyond that, once more with a new one.
-            if (!__any_sync(0xffffffffu, mx > 64.0f)) break;
+            // The reference follows a tile later, P and l have room: 2^64.  Beyond that, once more with a new one (once:
+            // scores so large that their own rounding passes 2^6 have no right answer in fp32).
+            if (again || !__any_sync(0xffffffffu, mx > 64.0f)) break;
             if (mx > 64.0f) {
               const float c = ch_exp2(-mx);
               pend *= c;

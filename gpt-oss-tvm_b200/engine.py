@@ -16,7 +16,10 @@ Added for batched serving and the benchmarks: ``Engine.random(config, seed)``
 (``max_batch_size``), and ``GreedyDecodeGraph``: one greedy decode step of
 sequences 0..B-1 (embedding, every layer, final norm, unembedding, argmax)
 captured as a single CUDA graph whose replays feed each step's tokens to the
-next on the device.
+next on the device.  ``extend_batch`` runs new tokens of several sequences in one
+forward over the paged cache (``max_chunk`` of them at most for each), ``verify``
+tests drafted tokens against its logits, ``kv_dtype="float8_e4m3"`` keeps the cache
+in 8 bits; speculative.py puts the three together.
 """
 from __future__ import annotations
 
@@ -30,6 +33,7 @@ from . import _lib
 from .attention import KVCache
 from .config import GPTOssConfig
 from .model import GPTOssForCausalLM, random_init
+from .verify import verify_drafts
 from .weights import checkpoint_file, load_checkpoint
 
 
@@ -48,7 +52,7 @@ class Engine:
 
     def __init__(self, model_path: str | Path | None, target: str = "cuda", *, config: GPTOssConfig | None = None,
                  seed: int | None = None, max_batch_size: int = 1, max_total_seq_len: int | None = None,
-                 warmup: bool = True):
+                 warmup: bool = True, kv_dtype: str = "bfloat16", max_chunk: int = 1):
         self.device = _device_of(target)
         torch.cuda.set_device(self.device)
         self.model_path = Path(model_path) if model_path is not None else None
@@ -67,7 +71,8 @@ class Engine:
             load_checkpoint(self.model, checkpoint_file(self.model_path))
         self.max_batch_size = max_batch_size
         self.max_total_seq_len = max_total_seq_len or config.context_window_size
-        self.model.reserve(max(config.prefill_chunk_size, max_batch_size))
+        self.kv_dtype, self.max_chunk = kv_dtype, max_chunk
+        self.model.reserve(max(config.prefill_chunk_size, max_batch_size * max_chunk))
         self.sample_parameters = {"temperature": 0.7, "top_p": 0.9, "random_seed": 0.5}
         self.paged_kv_cache = self._create_paged_kv_cache()
         if warmup:
@@ -80,7 +85,8 @@ class Engine:
 
     # KV cache ---------------------------------------------------------------
     def _create_paged_kv_cache(self) -> KVCache:
-        return self.model.create_paged_kv_cache(self.max_batch_size, self.max_total_seq_len)
+        return self.model.create_paged_kv_cache(self.max_batch_size, self.max_total_seq_len, self.kv_dtype,
+                                                self.max_chunk)
 
     def clear_kv_cache(self):
         self.paged_kv_cache.clear()
@@ -162,6 +168,29 @@ class Engine:
         self.paged_kv_cache.begin_forward(list(range(B)), [1] * B)
         logits, self.paged_kv_cache = self.model.decode(self.model.embed(ids), self.paged_kv_cache)
         return logits
+
+    def extend_batch(self, input_tokens, sequence_ids):
+        """New tokens of several sequences in one forward over their pages:
+        input_tokens a list of token lists, at most max_chunk each.  Returns
+        (logits [T, vocab] of every token, ids [T] int32, row_start [N + 1]
+        int32), all on the device and the sequences one after another -- what
+        ``verify`` takes."""
+        lens = [len(t) for t in input_tokens]
+        if lens and max(lens) > self.max_chunk:
+            raise ValueError(f"extend_batch takes up to max_chunk = {self.max_chunk} tokens of a sequence")
+        ids = self._ids([int(t) for seq in input_tokens for t in seq])
+        self.paged_kv_cache.begin_chunks(sequence_ids, lens)
+        logits, self.paged_kv_cache = self.model.chunk(self.model.embed(ids), self.paged_kv_cache)
+        self.paged_kv_cache.end_forward()
+        return logits[0], ids.to(torch.int32), self.paged_kv_cache.q_start
+
+    def verify(self, logits: torch.Tensor, ids: torch.Tensor, row_start: torch.Tensor,
+               accept_draws: torch.Tensor | None = None, next_draws: torch.Tensor | None = None, *,
+               temperature: float = 0.0, draft_probs: torch.Tensor | None = None):
+        """Of each sequence's drafts (its tokens of ``extend_batch`` but the
+        first): how many stand, and the token after them (verify.py)."""
+        return verify_drafts(logits, ids, row_start, accept_draws, next_draws, temperature=temperature,
+                             draft_probs=draft_probs)
 
     # sampling -------------------------------------------------------------------
     @staticmethod

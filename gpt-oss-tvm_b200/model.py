@@ -237,8 +237,10 @@ class GPTOssForCausalLM:
                 b.moe = None
         self.model.block[0].mlp.free_workspace()
 
-    def create_paged_kv_cache(self, max_batch_size: int, max_total_seq_len: int) -> KVCache:
-        return KVCache(self.config, max_batch_size, max_total_seq_len, self.num_hidden_layers, self.device)
+    def create_paged_kv_cache(self, max_batch_size: int, max_total_seq_len: int, kv_dtype: str = "bfloat16",
+                              max_chunk: int = 1) -> KVCache:
+        return KVCache(self.config, max_batch_size, max_total_seq_len, self.num_hidden_layers, self.device,
+                       kv_dtype=kv_dtype, max_chunk=max_chunk)
 
     # forward passes ------------------------------------------------------------
     def _get_logits(self, hidden_states: torch.Tensor) -> torch.Tensor:
@@ -266,6 +268,14 @@ class GPTOssForCausalLM:
         (model/transformer.py:127-132; the batch sits on the first axis)."""
         x = input_embed.reshape(-1, 1, self.hidden_size)
         hidden_states, paged_kv_cache = self.model(x, paged_kv_cache, "decode")
+        return self._get_logits(hidden_states), paged_kv_cache
+
+    def chunk(self, input_embed: torch.Tensor, paged_kv_cache: KVCache):
+        """The tokens of the cache's begin_chunks, several sequences' one after
+        another: logits [1, T, vocab] fp32 of every token (no counterpart in
+        the reference)."""
+        x = input_embed.reshape(1, -1, self.hidden_size)
+        hidden_states, paged_kv_cache = self.model(x, paged_kv_cache, "chunk")
         return self._get_logits(hidden_states), paged_kv_cache
 
 
