@@ -571,6 +571,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
           if (p.window > 0) r_hi = min(r_hi, max(0, min(j + p.window - first_pos, 1 << 16)) * p.G - rb);
         }
         float kf = p.scale2, ev = 0.f, einv = 1.f;
+        bool v_nan = false;
         if (F8 || !whole) {
           if (!bad) bad = !mbar_wait(&vfull[st], (uint32_t)(it / NS) & 1u, p.err, kErrTimeoutFull);
         }
@@ -579,17 +580,35 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
           const uint32_t kc = cc[0], vc = cc[2 * KT];
           const float nan = __uint_as_float(0x7FC00000u);
           kf = kc == 255u ? nan : p.scale2 * q_unit * __uint_as_float(kc << 23);
-          ev = vc == 255u ? nan : (float)((int)vc - 127);
-          einv = __uint_as_float((254u - min(vc, 253u)) << 23);
+          v_nan = vc == 255u;
+          ev = v_nan ? 0.f : (float)((int)vc - 127);
+          einv = v_nan ? 1.f : __uint_as_float((254u - min(vc, 253u)) << 23);
         }
-        if (!whole && (j < lo || j >= hi) && (!C::kSplit || part == 0)) {
-          // a key nobody may see: 0 times what its V row (or an earlier tile) holds must be 0
-          // (swizzled within the row, but for two heads in one row: 16-byte piece c of head s is 4 s + c)
-          uint8_t* vr = smem + st * 2 * C::kSide + C::kSide +
-                        (F8 ? key * (HB * RB) : ((key >> 3) * HB + s) * 8 * RB + (key & 7) * RB);
+        // Rows that do not see a key have P = 0 there, and 0 times its V row must be 0: where some row does not, the V
+        // rows of keys nobody sees (whatever their page, or an earlier tile, holds) and those that are not finite
+        // become zeros, and the latter's P NaN for the rows that do see them.
+        // (Swizzled within the row, but for two heads in one row: 16-byte piece c of head s is 4 s + c.)
+        uint8_t* vr = smem + st * 2 * C::kSide + C::kSide +
+                      (F8 ? key * (HB * RB) : ((key >> 3) * HB + s) * 8 * RB + (key & 7) * RB);
+        auto v_piece = [&](int c) { return (uint4*)(vr + (F8 && HB == 2 ? (4 * s + c) ^ (key & 7) : c) * 16); };
+        bool v_zero = false;
+        if (!whole) {
+          if (j < lo || j >= hi) {
+            v_zero = true;
+          } else {
+            uint32_t most = 0;
+#pragma unroll 1
+            for (int c = 0; c < RB / 16; ++c) {
+              const uint4 y = *v_piece(c);
+              const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int c = 0; c < RB / 16; ++c)
-            *(uint4*)(vr + (F8 && HB == 2 ? (4 * s + c) ^ (key & 7) : c) * 16) = make_uint4(0, 0, 0, 0);
+              for (int e = 0; e < 4; ++e)
+                most = F8 ? most | (((w[e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u)
+                          : max(most, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
+            }
+            if (F8 ? most != 0u : most >= 0x7F800000u) v_nan = true;
+            v_zero = v_nan;
+          }
         }
         if (!bad) bad = !mbar_wait(&sfull[s], (uint32_t)it & 1u, p.err, kErrTimeoutAccum);
         tc_fence_after();
@@ -684,6 +703,11 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sfree[s]);  // S^T is in registers
+        if (v_zero && (!C::kSplit || part == 0)) {  // both halves have looked, before the vote
+#pragma unroll
+          for (int c = 0; c < RB / 16; ++c) *v_piece(c) = make_uint4(0, 0, 0, 0);
+        }
+        const bool some_nan = __any_sync(0xffffffffu, v_nan);
         // P^T of the tile before has been used
         if (i > 0) {
           if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
@@ -708,6 +732,14 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
               w[e] = ch_e4m3x2(ch_lo(h), ch_hi(h));
               hl[e] = ch_e4m3x2(ch_lo(d), ch_hi(d));
             }
+          }
+          if (some_nan && v_nan) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (r0 + e >= r_lo && r0 + e < r_hi) {
+                const int at = (e & 1) * (F8 ? 8 : 16);
+                w[e >> 1] = (w[e >> 1] & ~((F8 ? 0xFFu : 0xFFFFu) << at)) | ((F8 ? 0x7Fu : 0x7FC0u) << at);
+              }
           }
           const int b = (rb + r0) * (F8 ? 1 : 2);  // byte of the row's place
           if (!F8) {
@@ -849,10 +881,11 @@ struct RowsCfg {
   static constexpr int kRawSide = kRowsKT * 64;
   static constexpr int kOffRaw = 2 * 128 * 128 + kStages * 2 * kSide;
   static constexpr int kOffCodes = kOffRaw + kRaw * 2 * kRawSide;
-  static constexpr int kOffPre = kOffCodes + kRaw * 2 * kRowsKT;
+  static constexpr int kOffNan = kOffCodes + kRaw * 2 * kRowsKT;  // per stage: a bit for each key whose V row is not finite
+  static constexpr int kOffPre = kOffNan + kStages * 16;
   static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
   static constexpr int kOffBar = kOffSeg + 2 * (int)sizeof(ChunkSeg);
-  static constexpr int kAlloc = kOffBar + (2 * kStages + 4 + 4 + 2 + 8) * 8 + 16 + 1024;
+  static constexpr int kAlloc = kOffBar + (3 * kStages + 4 + 4 + 2 + 8) * 8 + 16 + 1024;
   static_assert(kAlloc <= 227 * 1024, "shared memory");
 };
 
@@ -891,7 +924,8 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
   ChunkSeg* segs = (ChunkSeg*)(smem + C::kOffSeg);
   uint64_t* kvfull = (uint64_t*)(smem + C::kOffBar);
   uint64_t* kvempty = kvfull + NS;
-  uint64_t* rawfull = kvempty + NS;  // [2]
+  uint64_t* vready = kvempty + NS;  // bf16: V has been looked at
+  uint64_t* rawfull = vready + NS;  // [2]
   uint64_t* rawempty = rawfull + 2;  // [2]
   uint64_t* seg_full = rawempty + 2;
   uint64_t* seg_empty = seg_full + 2;
@@ -910,12 +944,13 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
     for (int s = 0; s < NS; ++s) {
       mbar_init(&kvfull[s], F8 ? 4 : 1);
       mbar_init(&kvempty[s], 1);
+      mbar_init(&vready[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&rawfull[s], 33);  // the loading warp's lanes arrive with their copies of the codes
       mbar_init(&rawempty[s], 4);
       mbar_init(&seg_full[s], 1);
-      mbar_init(&seg_empty[s], 9 + (F8 ? 4 : 0));
+      mbar_init(&seg_empty[s], 9 + (F8 ? 4 : 2));
       mbar_init(&sfull[s], 1);
       mbar_init(&sfree[s], 4);
       mbar_init(&pfull[s], 4);
@@ -1086,10 +1121,26 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
               const int idx = x * 128 + tid, key = idx >> 2, c = idx & 3;
               const int32_t j = j0 + i * kRowsKT + key;
               uint32_t o[8];
-              // a key nobody may see: zeros, whatever its page (or an earlier tile) holds
-              if (j >= lo && j < hi) {
-                const uint4 w = *(const uint4*)(raw + side * C::kRawSide + idx * 16);
-                const uint32_t mul = ch_code_mul(codes[side * kRowsKT + key]);
+              bool on = j >= lo && j < hi;  // a key nobody may see: zeros, whatever its page (or an earlier tile) holds
+              const uint4 w = *(const uint4*)(raw + side * C::kRawSide + idx * 16);
+              const uint32_t code = codes[side * kRowsKT + key];
+              if (side) {
+                // V rows that are not finite: zeros and a mark, see the softmax
+                uint32_t n = 0;
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int y = 0; y < 4; ++y) n |= ((ww[y] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                const uint32_t bad4 = __ballot_sync(0xffffffffu, on && (n != 0u || code == 255u));
+                if (bad4 >> (lane & 28) & 15u) on = false;
+                if (lane == 0) {
+                  uint32_t bits = 0;
+#pragma unroll
+                  for (int y = 0; y < 8; ++y) bits |= (bad4 >> (4 * y) & 15u) ? 1u << y : 0u;
+                  smem[C::kOffNan + st * 16 + x * 4 + (warp & 3)] = (uint8_t)bits;
+                }
+              }
+              if (on) {
+                const uint32_t mul = ch_code_mul(code);
                 ch_e4m3_to_bf16(w.x, mul, o[0], o[1]);
                 ch_e4m3_to_bf16(w.y, mul, o[2], o[3]);
                 ch_e4m3_to_bf16(w.z, mul, o[4], o[5]);
@@ -1115,6 +1166,53 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
     }
   } else if (warp >= 10) {
     if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (!F8) {
+      // ---------------------------------------------------- V rows at the edges
+      // Rows that do not see a key have P = 0 there, and 0 times its V row must be 0: in tiles where some row does not,
+      // the V rows of keys nobody sees and those that are not finite become zeros, the latter with a mark.
+      const int half = warp - 10;
+      for (int sn = 0;; ++sn) {
+        const int sb = sn & 1;
+        if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
+        if (bad || segs[sb].nrows < 0) break;
+        const int nt = segs[sb].ntile;
+        const int32_t j0 = segs[sb].j0, lo = segs[sb].lo, hi = segs[sb].hi, first = segs[sb].first_pos;
+        const int32_t last = first + segs[sb].ntok - 1;
+        for (int i = 0; i < nt; ++i, ++it) {
+          const int st = it % NS;
+          const int32_t jt = j0 + i * kRowsKT;
+          if (!bad) bad = !mbar_wait(&kvfull[st], (uint32_t)(it / NS) & 1u, p.err, kErrTimeoutFull);
+          if (jt + kRowsKT - 1 > first || jt < lo || (p.window > 0 && jt <= last - p.window)) {
+#pragma unroll 1
+            for (int x = 0; x < 2; ++x) {
+              const int key = half * 64 + x * 32 + lane;
+              uint4* vr = (uint4*)(kv0 + st * 2 * C::kSide + C::kSide + key * 128);
+              const bool seen = jt + key >= lo && jt + key < hi;
+              uint32_t most = 0;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const uint4 y = vr[c];
+                const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = max(most, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
+              }
+              const bool is_nan = seen && most >= 0x7F800000u;
+              if (!seen || is_nan) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) vr[c] = make_uint4(0, 0, 0, 0);
+              }
+              const uint32_t bits = __ballot_sync(0xffffffffu, is_nan);
+              if (lane == 0) *(uint32_t*)(smem + C::kOffNan + st * 16 + (half * 2 + x) * 4) = bits;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&vready[st]);
+        }
+        if (lane == 0) mbar_arrive(&seg_empty[sb]);
+        __syncwarp();
+      }
+    }
   } else {
     // ----------------------------------------------------------- softmax
     if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
@@ -1136,7 +1234,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
       const int tok = t * tq1 + tok_r;
       const bool row_ok = tok_r < tq1 && tok < ntok;
       const bool warp_on = __any_sync(0xffffffffu, row_ok);
-      const int32_t lo = sg.lo, hi = sg.hi;
+      const int32_t lo = sg.lo;
       const int32_t pos = row_ok ? sg.first_pos + tok : -1;
       const int32_t tile_first = sg.first_pos + t * tq1, tile_last = sg.first_pos + min(ntok, (t + 1) * tq1) - 1;
       // a row that is not in use has whatever its place in shared memory held for a query: scale 0, reference 0
@@ -1145,21 +1243,11 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
       if (tile_on) {
         for (int i = 0; i < ntile; ++i) {
           const int32_t j0 = sg.j0 + i * kRowsKT;
-          if (!F8 && t == 0 && (j0 < lo || j0 + kRowsKT > hi)) {
-            // keys nobody may see: 0 times what their V rows (or an earlier tile) hold must be 0; both tiles' products
-            // with V come after this tile's warps have arrived
-            const int st = (it + i) % NS;
-            if (!bad) bad = !mbar_wait(&kvfull[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
-            if (j0 + row < lo || j0 + row >= hi) {
-              uint8_t* vr = kv0 + st * 2 * C::kSide + C::kSide + row * 128;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) *(uint4*)(vr + c * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          }
           if (!bad) bad = !mbar_wait(&sfull[t], par, p.err, kErrTimeoutAccum);
           tc_fence_after();
           if (!warp_on) {  // no row of this warp is in use
+            if (!F8 && t == 0 && !bad)
+              bad = !mbar_wait(&vready[(it + i) % NS], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
             tc_fence_before();
             if (lane == 0) {
               mbar_arrive(&sfree[t]);
@@ -1190,6 +1278,16 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
             }
             if (m_ref == -INFINITY) m_ref = mx * scale;  // nothing of it in O or l yet
           }
+          // keys whose V row is not finite
+          uint4 nans = make_uint4(0, 0, 0, 0);
+          const bool edge = j0 + kRowsKT - 1 > sg.first_pos || j0 < lo ||
+                            (p.window > 0 && j0 <= sg.first_pos + ntok - 1 - p.window);
+          const int st = (it + i) % NS;
+          if (F8 || edge) {
+            if (!F8 && !bad) bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
+            nans = *(const uint4*)(smem + C::kOffNan + st * 16);
+          }
+          const bool some_nan = (nans.x | nans.y | nans.z | nans.w) != 0u;
           // P_t and O_t are free once the products of the tile before are done
           if (i > 0) {
             if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
@@ -1212,6 +1310,14 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
                 const float p0 = ch_exp2(ch_lo(x)), p1 = ch_exp2(ch_hi(x));
                 sum2 = ch_add2(sum2, ch_pair(p0, p1));
                 pk[e] = ch_bf16x2(p0, p1);
+              }
+              if (some_nan) {  // a row that sees such a key is NaN; its sum is not
+                const uint32_t bits = e0 == 0 ? nans.x : e0 == 32 ? nans.y : e0 == 64 ? nans.z : nans.w;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  if ((bits >> (2 * e) & 1u) && r[2 * e] != 0xFF800000u) pk[e] = (pk[e] & 0xFFFF0000u) | 0x7FC0u;
+                  if ((bits >> (2 * e + 1) & 1u) && r[2 * e + 1] != 0xFF800000u) pk[e] = (pk[e] & 0xFFFFu) | 0x7FC00000u;
+                }
               }
               ch_st16(p_col + e0 / 2, pk);
             };

@@ -14,7 +14,7 @@
 // A power of two loses nothing against a finer scale: e4m3 is a floating
 // format, its relative precision does not depend on where a lies in the
 // binade, and value * 2^e is then exact in bf16.  A row that holds a NaN gets
-// code 255 and reads back as NaN; magnitudes above 448 * 2^60 (infinities too)
+// code 255 and values 0 and reads back as NaN; magnitudes above 448 * 2^60 (infinities too)
 // saturate.
 #include "common.cuh"
 #include "launch.h"
@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t kv8_code(uint32_t amax_bits) {
   e = max(kKv8MinExp, min(kKv8MaxExp, e));
   return (uint32_t)(e + 127);
 }
-// 2^-(code - 127) (any value for the NaN code: the row reads back as NaN).
+// 2^-(code - 127)
 __device__ __forceinline__ float kv8_inv_scale(uint32_t code) { return __uint_as_float((254u - min(code, 253u)) << 23); }
 
 // lo -> byte 0, hi -> byte 1
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(256)
           r[k] = e4m3x2(a[4 * k] * inv, a[4 * k + 1] * inv) | (e4m3x2(a[4 * k + 2] * inv, a[4 * k + 3] * inv) << 16);
           r[2 + k] = e4m3x2(b[4 * k] * inv, b[4 * k + 1] * inv) | (e4m3x2(b[4 * k + 2] * inv, b[4 * k + 3] * inv) << 16);
         }
+        if (code == 255u) r[0] = r[1] = r[2] = r[3] = 0u;
         uint8_t* p = (h < Hq + Hkv ? kp : vp) + (row * Hkv + hk) * kKv8D + 8 * l;
         *(uint2*)p = make_uint2(r[0], r[1]);
         *(uint2*)(p + 32) = make_uint2(r[2], r[3]);
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(256)
           o[k] = e4m3x2(__uint_as_float(u << 16) * inv, __uint_as_float(u & 0xFFFF0000u) * inv) |
                  (e4m3x2(__uint_as_float(t << 16) * inv, __uint_as_float(t & 0xFFFF0000u) * inv) << 16);
         }
+        if (code == 255u) o[0] = o[1] = o[2] = o[3] = 0u;
         if (on) {
           *(uint4*)((side ? vp : kp) + at) = make_uint4(o[0], o[1], o[2], o[3]);
           if (l == 0) (side ? vcode : kcode)[ca] = (uint8_t)code;

@@ -209,6 +209,34 @@ def test_a_nan_key_stays_with_those_who_see_it(f8):
 
 
 @pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("q,window", [(1, 0), (4, 0), (7, 0), (40, 0), (100, 0), (5, 20), (40, 20)])
+def test_a_value_that_is_not_finite_stays_with_those_who_see_it(q, window, value, f8):
+    """Also when it is a later token's of the same chunk: the rows before it
+    keep their bits, the rows from it on are NaN (in the window), sums and
+    other heads are untouched."""
+    L = 150 + q
+    c = Case([q, 2], [L, 60], f8=f8, window=window, seed=q).gpu()
+    o, lse = c.run()
+    for at in (q // 2, q - 1):
+        pos = L - q + at
+        row = int(c.table[0, pos // PAGE]) * PAGE + pos % PAGE
+        keep = [t.clone() if t is not None else None for t in (c.v, c.vs)]
+        if f8:
+            c.vs.view(torch.uint8)[row // PAGE, 2, row % PAGE] = 255
+            c.v.view(torch.uint8)[row, 2] = 0x7F
+        else:
+            c.v[row, 2, 7] = value
+        o2, lse2 = c.run()
+        c.v, c.vs = keep
+        sees = torch.zeros(q + 2, 64, dtype=torch.bool, device="cuda")
+        sees[at:(min(q, at + window) if window else q), 16:24] = True
+        assert bool(((lse - lse2).abs() <= 1e-4).all())
+        assert torch.equal(o[~sees], o2[~sees])
+        assert not bool(torch.isfinite(o2[sees][:, 7]).any())
+
+
+@pytest.mark.parametrize("f8", [False, True])
 @pytest.mark.parametrize("q", [1, 5, 40])
 def test_large_scores_and_moving_reference(q, f8):
     """Scores that rise along the keys by hundreds (the reference of a row
