@@ -704,10 +704,9 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sfree[s]);  // S^T is in registers
         if (v_zero && (!C::kSplit || part == 0)) {  // both halves have looked, before the vote
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < RB / 16; ++c) *v_piece(c) = make_uint4(0, 0, 0, 0);
         }
-        const bool some_nan = __any_sync(0xffffffffu, v_nan);
         // P^T of the tile before has been used
         if (i > 0) {
           if (!bad) bad = !mbar_wait(&ofull[s], ((uint32_t)it & 1u) ^ 1u, p.err, kErrTimeoutAccum);
@@ -733,14 +732,6 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
               hl[e] = ch_e4m3x2(ch_lo(d), ch_hi(d));
             }
           }
-          if (some_nan && v_nan) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (r0 + e >= r_lo && r0 + e < r_hi) {
-                const int at = (e & 1) * (F8 ? 8 : 16);
-                w[e >> 1] = (w[e >> 1] & ~((F8 ? 0xFFu : 0xFFFFu) << at)) | ((F8 ? 0x7Fu : 0x7FC0u) << at);
-              }
-          }
           const int b = (rb + r0) * (F8 ? 1 : 2);  // byte of the row's place
           if (!F8) {
             *(uint4*)(pr + (b ^ sw)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -748,6 +739,14 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
             *(uint2*)(pr + ((b & ~15) ^ sw) + (b & 8)) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
             const int b2 = N + b;
             *(uint2*)(pr + ((b2 & ~15) ^ sw) + (b2 & 8)) = make_uint2(hl[0] | (hl[1] << 16), hl[2] | (hl[3] << 16));
+          }
+        }
+        if (v_nan) {
+#pragma unroll 1
+          for (int r = max(0, r_lo); r < r_hi; ++r) {
+            const int b = (rb + r) * (F8 ? 1 : 2), at = ((b & ~15) ^ sw) + (b & 15);
+            if (F8) pr[at] = 0x7F;
+            else *(uint16_t*)(pr + at) = 0x7FC0;
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1105,9 +1104,12 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
         if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
         if (bad || segs[sb].nrows < 0) break;
         const int nt = segs[sb].ntile;
-        const int32_t j0 = segs[sb].j0, lo = segs[sb].lo, hi = segs[sb].hi;
+        const int32_t j0 = segs[sb].j0, lo = segs[sb].lo, hi = segs[sb].hi, first = segs[sb].first_pos;
+        const int32_t last = first + segs[sb].ntok - 1;
         for (int i = 0; i < nt; ++i, ++it) {
           const int rs = it & 1, st = it % NS;
+          const int32_t jt = j0 + i * kRowsKT;
+          const bool edge = jt + kRowsKT - 1 > first || jt < lo || (p.window > 0 && jt <= last - p.window);
           if (!bad) bad = !mbar_wait(&rawfull[rs], (uint32_t)(it >> 1) & 1u, p.err, kErrTimeoutFull);
           if (!bad) bad = !mbar_wait(&kvempty[st], ((uint32_t)(it / NS) & 1u) ^ 1u, p.err, kErrTimeoutEmpty);
           const uint8_t* raw = smem + C::kOffRaw + rs * 2 * C::kRawSide;
@@ -1124,8 +1126,8 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
               bool on = j >= lo && j < hi;  // a key nobody may see: zeros, whatever its page (or an earlier tile) holds
               const uint4 w = *(const uint4*)(raw + side * C::kRawSide + idx * 16);
               const uint32_t code = codes[side * kRowsKT + key];
-              if (side) {
-                // V rows that are not finite: zeros and a mark, see the softmax
+              if (side && edge) {
+                // V rows that are not finite, where some row does not see them: zeros and a mark, see the softmax
                 uint32_t n = 0;
                 const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -1283,11 +1285,10 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
           const bool edge = j0 + kRowsKT - 1 > sg.first_pos || j0 < lo ||
                             (p.window > 0 && j0 <= sg.first_pos + ntok - 1 - p.window);
           const int st = (it + i) % NS;
-          if (F8 || edge) {
+          if (edge) {
             if (!F8 && !bad) bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
             nans = *(const uint4*)(smem + C::kOffNan + st * 16);
           }
-          const bool some_nan = (nans.x | nans.y | nans.z | nans.w) != 0u;
           // P_t and O_t are free once the products of the tile before are done
           if (i > 0) {
             if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
@@ -1311,14 +1312,6 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
                 sum2 = ch_add2(sum2, ch_pair(p0, p1));
                 pk[e] = ch_bf16x2(p0, p1);
               }
-              if (some_nan) {  // a row that sees such a key is NaN; its sum is not
-                const uint32_t bits = e0 == 0 ? nans.x : e0 == 32 ? nans.y : e0 == 64 ? nans.z : nans.w;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  if ((bits >> (2 * e) & 1u) && r[2 * e] != 0xFF800000u) pk[e] = (pk[e] & 0xFFFF0000u) | 0x7FC0u;
-                  if ((bits >> (2 * e + 1) & 1u) && r[2 * e + 1] != 0xFF800000u) pk[e] = (pk[e] & 0xFFFFu) | 0x7FC00000u;
-                }
-              }
               ch_st16(p_col + e0 / 2, pk);
             };
             uint32_t ra[32], rb[32];
@@ -1341,6 +1334,23 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
               pend *= c;
               l *= c;
               m_ref += mx;
+            }
+          }
+          if ((nans.x | nans.y | nans.z | nans.w) != 0u) {
+            // P of the rows that see a key whose V row is not finite; the sum keeps its own
+            tmem_st_wait();
+#pragma unroll 1
+            for (int e = 0; e < 128; ++e) {
+              const uint32_t bits = e < 32 ? nans.x : e < 64 ? nans.y : e < 96 ? nans.z : nans.w;
+              if (!(bits >> (e & 31) & 1u)) continue;
+              const int32_t kj = j0 + e;
+              uint32_t w;
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(w) : "r"(p_col + e / 2) : "memory");
+              tmem_ld_wait();
+              if (kj <= pos && (p.window <= 0 || kj > pos - p.window))
+                w = e & 1 ? (w & 0xFFFFu) | 0x7FC00000u : (w & 0xFFFF0000u) | 0x7FC0u;
+              asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(p_col + e / 2), "r"(w) : "memory");
+              tmem_st_wait();
             }
           }
           tc_fence_before();
