@@ -47,18 +47,22 @@ __device__ __forceinline__ uint32_t ch_e4m3x2(float lo, float hi) {
 __device__ __forceinline__ float ch_round4(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x80000u) & 0xFFF00000u);
 }
-// Four e4m3 bytes as two bf16 pairs (b0, b1), (b2, b3) times 2^e, exactly: the
-// bits moved into a bf16 read 2^-120 of the value, then come 2^60 and `mul`
-// (ch_code_mul: 2^(e + 60), NaN for the code of a row that held one).
+// Four e4m3 bytes as two bf16 pairs (b0, b1), (b2, b3) times `mul`, exactly: a
+// byte below eight copies of its sign, moved up by four bits, is a bf16 that
+// reads 2^-120 of the value.  ch_code_mul is 2^(e + 120) for the code 127 + e,
+// NaN for that of a row that held one; beyond e = 7, which bf16 does not hold,
+// it is 2^127 and ch_code_rest the factor that is left.
 __device__ __forceinline__ void ch_e4m3_to_bf16(uint32_t w, uint32_t mul, uint32_t& p01, uint32_t& p23) {
-  const uint32_t ev = ((w << 4) & 0x07F007F0u) | ((w << 8) & 0x80008000u);  // (b0, b2)
-  const uint32_t od = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);         // (b1, b3)
-  const uint32_t e2 = bf16x2_mul(bf16x2_mul(ev, 0x5D805D80u), mul), o2 = bf16x2_mul(bf16x2_mul(od, 0x5D805D80u), mul);
-  p01 = prmt(e2, o2, 0x5410u);
-  p23 = prmt(e2, o2, 0x7632u);
+  p01 = bf16x2_mul((prmt(w, 0u, 0x9180u) << 4) & 0x87F087F0u, mul);
+  p23 = bf16x2_mul((prmt(w, 0u, 0xB3A2u) << 4) & 0x87F087F0u, mul);
 }
+constexpr uint32_t kCodeOne = 134;  // the largest code that takes one factor
 __device__ __forceinline__ uint32_t ch_code_mul(uint32_t code) {
-  const uint32_t h = code == 255u ? 0x7FC0u : ((min(code, 194u) + 60u) << 7);
+  const uint32_t h = code == 255u ? 0x7FC0u : ((min(code, kCodeOne) + 120u) << 7);
+  return h | (h << 16);
+}
+__device__ __forceinline__ uint32_t ch_code_rest(uint32_t code) {
+  const uint32_t h = (min(code, 194u) - kCodeOne + 127u) << 7;
   return h | (h << 16);
 }
 // Two fp32 at a time.
@@ -856,35 +860,78 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
 
 // ---------------------------------------------------------- rows on M --
 // CTA = two tiles of 128 rows (128 / G tokens times the G heads of a kv head),
-// a softmax warpgroup each (thread = row = TMEM lane), one warp that loads, one
-// that issues the products: S_t = Q_t K^T (both in shared memory), O_t += P_t V
-// (P_t bf16 in TMEM), tiles of 128 keys.  The tiles take turns: while one's
-// softmax runs the tensor core works for the other.  Bound by the exponentials:
-// 2 x 128 x 128 of them a key tile at 16 per cycle and SM are 2048 cycles, the
-// products 1024, K and V from L2 32 KB.  The reference of a row is the largest
-// score of its first tile; when a later one exceeds it by 8 it moves before the
-// next tile (P and l hold what 2^64 above it gives), so a tile's scores are read
-// once.
+// two softmax warpgroups each (thread = row = TMEM lane, half of a tile's 128
+// keys), one warp that loads, one that issues the products: S_t = Q_t K^T (both
+// in shared memory), O_t += P_t V (P_t bf16 in TMEM, in the place of S_t).  S has
+// three buffers: the scores of three (key tile, tile) steps are ahead of their
+// softmax, so a warp that ends a step finds the next one's ready.
 //
-// 8-bit pages: a fourth warpgroup turns a tile's values into bf16 with their
-// power of two (exact) while the one before is used, about 450 issue cycles of
-// the 2048 a tile takes; the rest of the kernel is the same.
+// Bound by the exponentials and what stands around them: 2 x 128 x 128 a key
+// tile at 16 per cycle and SM are 2048 cycles, the products 1024, K and V from
+// L2 32 KB; a step of a warp is 405 instructions for its 32 x 64 scores, 64 of
+// them exponentials, and every operation that passes the same queue (barriers,
+// shared memory, TMEM) waits behind those.  So a step has few: the row's two
+// warps agree by one barrier whether a reference has to move (they exchange
+// maxima only then), and wait for O_t only then.  Measured, 2048 tokens on a
+// sequence of 32768: 1338 us in bf16, 800 TFLOP/s, 3000 cycles a key tile.  One
+// softmax warpgroup a tile took 1718, two that exchange every maximum 1504,
+// turns between the tiles by a barrier 1480; without the polynomial below 1421.
+//
+// 8-bit pages: two more warpgroups turn a tile's values into bf16 with their
+// power of two (exact) while those before are used: 60 instructions for 32 x 16
+// values; the rest of the kernel is the same.  1867 us for the same call: a key
+// tile's conversion is a third of the instructions that its softmax is.  (One
+// converting warpgroup: 3121.)
 constexpr int kRowsKT = 128;
+__device__ __forceinline__ float ch_max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+__device__ __forceinline__ float ch_max3_nan(float a, float b, float c) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+// 2^x of two values without the exponential unit: x = n + f with n its floor, 2^f a polynomial of degree 4 with value 1
+// at 0 that is nowhere on [0, 1] further than 2^-17 of 2^f (its coefficients solve that minimax problem), n added to the
+// exponent.  Below 2^-127 it is 0: f is 0 there.  P has 8 bits.
+__device__ __forceinline__ void ch_exp2_poly(ch_f2 x, float& p0, float& p1) {
+  const float kMagic = 12582912.0f;  // 1.5 * 2^23: a sum with it has its integer part in the low bits
+  x = ch_pair(fmaxf(ch_lo(x), -127.0f), fmaxf(ch_hi(x), -127.0f));
+  ch_f2 t;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(ch_pair(kMagic, kMagic)));
+  const ch_f2 n = ch_add2(t, ch_pair(-kMagic, -kMagic));
+  const ch_f2 f = ch_fma2(n, ch_pair(-1.0f, -1.0f), x);
+  ch_f2 q = ch_fma2(f, ch_pair(0.0134266838f, 0.0134266838f), ch_pair(0.0522424765f, 0.0522424765f));
+  q = ch_fma2(q, f, ch_pair(0.241280198f, 0.241280198f));
+  q = ch_fma2(q, f, ch_pair(0.693044841f, 0.693044841f));
+  q = ch_fma2(q, f, ch_pair(1.0f, 1.0f));
+  p0 = __uint_as_float((uint32_t)q + ((uint32_t)t << 23));
+  p1 = __uint_as_float((uint32_t)(q >> 32) + ((uint32_t)(t >> 32) << 23));
+}
 
 template <bool F8>
 struct RowsCfg {
-  static constexpr int kThreads = F8 ? 512 : 384;
-  static constexpr int kStages = F8 ? 3 : 4;
+  static constexpr int kSoftmax = 16;        // softmax warps; then 4 that load, issue and check
+  static constexpr int kConv = F8 ? 8 : 0;   // and those that turn 8-bit tiles into bf16
+  static constexpr int kThreads = 32 * (kSoftmax + 4 + kConv);
+  // registers: all have the same at first, then the softmax warps get what the others do without
+  static constexpr int kRegs = (65536 / kThreads) & ~7;
+  static constexpr int kRegAux = F8 ? 40 : 64, kRegConv = 56;
+  static constexpr int kRegSoftmax = ((kRegs * kThreads - 128 * kRegAux - 32 * kConv * kRegConv) / (32 * kSoftmax)) & ~7;
+  static constexpr int kStages = 4;
   static constexpr int kSide = kRowsKT * 128;            // K or V of a tile, bf16
   static constexpr int kRaw = F8 ? 2 : 0;                // stages of 8-bit tiles
   static constexpr int kRawSide = kRowsKT * 64;
   static constexpr int kOffRaw = 2 * 128 * 128 + kStages * 2 * kSide;
   static constexpr int kOffCodes = kOffRaw + kRaw * 2 * kRawSide;
   static constexpr int kOffNan = kOffCodes + kRaw * 2 * kRowsKT;  // per stage: a bit for each key whose V row is not finite
-  static constexpr int kOffPre = kOffNan + kStages * 16;
+  static constexpr int kOffMax = kOffNan + kStages * 16;  // [tile][half][128]: maxima, at the end sums
+  static constexpr int kOffPre = kOffMax + 2 * 2 * 128 * 4;
   static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
   static constexpr int kOffBar = kOffSeg + 2 * (int)sizeof(ChunkSeg);
-  static constexpr int kAlloc = kOffBar + (3 * kStages + 4 + 4 + 2 + 8) * 8 + 16 + 1024;
+  static constexpr int kAlloc = kOffBar + (3 * kStages + 4 + 4 + 2 + 4 + 4 + 2) * 8 + 16 + 1024;
   static_assert(kAlloc <= 227 * 1024, "shared memory");
 };
 
@@ -915,7 +962,8 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
                       const __grid_constant__ CUtensorMap tmap_v, const ChunkParams p) {
   using C = RowsCfg<F8>;
   constexpr int NS = C::kStages, RB = F8 ? 64 : 128;
-  constexpr uint32_t kColO = 256, kColP = 384;
+  constexpr int SW = C::kSoftmax, CV = C::kConv, KW = 64, DW = 32;  // a warp's share of a tile's keys, of the dims
+  constexpr uint32_t kColO = 384;  // after three buffers of 128 columns for S
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* kv0 = smem + 2 * 128 * 128;
@@ -930,10 +978,9 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
   uint64_t* seg_empty = seg_full + 2;
   uint64_t* qfull = seg_empty + 2;
   uint64_t* qempty = qfull + 1;
-  uint64_t* sfull = qempty + 1;  // per tile from here on
-  uint64_t* sfree = sfull + 2;
-  uint64_t* pfull = sfree + 2;
-  uint64_t* ofull = pfull + 2;
+  uint64_t* sfull = qempty + 1;  // [tile][key tile & 1]
+  uint64_t* pfull = sfull + 4;   // [tile][key tile & 1]
+  uint64_t* ofull = pfull + 4;   // [tile]
   volatile uint32_t* flag = (volatile uint32_t*)(ofull + 2);
   volatile uint32_t* tmem_slot = flag + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -941,25 +988,26 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&kvfull[s], F8 ? 4 : 1);
+      mbar_init(&kvfull[s], F8 ? CV : 1);
       mbar_init(&kvempty[s], 1);
       mbar_init(&vready[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&rawfull[s], 33);  // the loading warp's lanes arrive with their copies of the codes
-      mbar_init(&rawempty[s], 4);
+      mbar_init(&rawempty[s], CV);
       mbar_init(&seg_full[s], 1);
-      mbar_init(&seg_empty[s], 9 + (F8 ? 4 : 2));
-      mbar_init(&sfull[s], 1);
-      mbar_init(&sfree[s], 4);
-      mbar_init(&pfull[s], 4);
+      mbar_init(&seg_empty[s], SW + 1 + (F8 ? CV : 2));
+      mbar_init(&sfull[2 * s], 1);
+      mbar_init(&sfull[2 * s + 1], 1);
+      mbar_init(&pfull[2 * s], SW / 2);
+      mbar_init(&pfull[2 * s + 1], SW / 2);
       mbar_init(&ofull[s], 1);
     }
     mbar_init(qfull, 1);
     mbar_init(qempty, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == SW + 1) {
     tmem_alloc((uint32_t*)tmem_slot, 512);
     tmem_relinquish();
   }
@@ -969,11 +1017,10 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   int it = 0;  // key tiles so far
   bool bad = false;
-  // 8 bit: 512 threads start with 128 registers each: 256 * 176 + 128 * 64 + 128 * 80 of them from here on
-
-  if (warp == 8) {
+  if (warp >= SW + 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegConv));
+  if (warp >= SW && warp < SW + 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegAux));
+  if (warp == SW) {
     // ------------------------------------------------------------- loads
-    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     ChunkWalk walk;
     walk.begin(p, pre, gridDim.x, blockIdx.x);
     for (int sn = 0;; ++sn) {
@@ -1033,72 +1080,71 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
         __syncwarp();
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == SW + 1) {
     // ---------------------------------------------------------- products
-    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (elect_one()) {
       const uint32_t idesc_s = make_idesc_bf16(128, kRowsKT);
       const uint32_t idesc_o = make_idesc_bf16(128, 64) | (1u << 16);  // B (V) read dims-major
       const uint64_t dq = make_sdesc_sw128(smem_u32(smem)), dk = make_sdesc_sw128(smem_u32(kv0)),
                      dv = make_sdesc_sw128(smem_u32(kv0 + C::kSide));
-      int ks = 0, vs = 0;
-      uint32_t kp = 0, tp = 0, op = 0;  // parity of the stage; bit t: parities of S_t and P_t (a tile may sit out)
+      int ks = 0, vs = 0, sbuf = 0, pbuf = 0;
+      uint32_t kp = 0, op = 0, sp = 0;  // parity of the stage; P_t and S_t so far, 2 and 1 bits each (a tile may sit out)
       for (int sn = 0; !bad; ++sn) {
         const int sb = sn & 1;
         bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
         if (bad || segs[sb].nrows < 0) break;
-        const int nt = segs[sb].ntile, tiles = segs[sb].ntok > tq1 ? 2 : 1;
+        const int nt = segs[sb].ntile, tiles = segs[sb].ntok > tq1 ? 2 : 1, total = nt * tiles;
         bad = !mbar_wait(qfull, (uint32_t)sn & 1u, p.err, kErrTimeoutFull);
-        auto issue_s = [&](int t, bool last) {
-          if (!bad) bad = !mbar_wait(&sfree[t], (tp >> t & 1u) ^ 1u, p.err, kErrTimeoutAccum);  // S_t has been read
-          tp ^= 1u << t;
+        // Products in the order (key tile, tile).  The scores go three ahead of P V (two with one tile, so that the
+        // wait for a tile's output cannot meet the one two before): the buffer they go to is the one whose P V was
+        // issued last, and the tensor core keeps the order.
+        auto issue_s = [&](int n) {
+          const int t = tiles == 2 ? n & 1 : 0;
+          if (t == 0 && !bad) bad = !mbar_wait(&kvfull[ks], kp, p.err, kErrTimeoutFull);
           tc_fence_after();
           const uint64_t a = dq + t * (128 * 128 >> 4), b = dk + (uint32_t)ks * (2 * C::kSide >> 4);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) tc_mma_ss(tmem + t * 128, a + 2 * kk, b + 2 * kk, idesc_s, kk > 0 ? 1u : 0u);
-          tc_commit(&sfull[t]);
-          if (last && t == tiles - 1) tc_commit(qempty);
-        };
-        auto next_k = [&]() {
-          if (++ks == NS) {
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_ss(tmem + sbuf * 128, a + 2 * kk, b + 2 * kk, idesc_s, kk > 0 ? 1u : 0u);
+          tc_commit(&sfull[2 * t + (sp >> t & 1u)]);
+          sp ^= 1u << t;
+          if (++sbuf == 3) sbuf = 0;
+          if (t == tiles - 1 && ++ks == NS) {
             ks = 0;
             kp ^= 1u;
           }
+          if (n == total - 1) tc_commit(qempty);
         };
         if (nt == 0) mbar_arrive(qempty);
-        if (nt > 0) {
-          if (!bad) bad = !mbar_wait(&kvfull[ks], kp, p.err, kErrTimeoutFull);
-          for (int t = 0; t < tiles; ++t) issue_s(t, nt == 1);
-          next_k();
-        }
-        for (int i = 0; i < nt; ++i) {
-          const bool more = i + 1 < nt;
-          if (more && !bad) bad = !mbar_wait(&kvfull[ks], kp, p.err, kErrTimeoutFull);
-          for (int t = 0; t < tiles; ++t) {
-            if (more) issue_s(t, i + 2 == nt);
-            if (!bad) bad = !mbar_wait(&pfull[t], op >> t & 1u, p.err, kErrTimeoutAccum);
-            op ^= 1u << t;
-            tc_fence_after();
-            const uint64_t b = dv + (uint32_t)vs * (2 * C::kSide >> 4);
+        const int ahead = min(tiles + 1, total);
+        for (int n = 0; n < ahead; ++n) issue_s(n);
+        for (int n = 0; n < total; ++n) {
+          const int t = tiles == 2 ? n & 1 : 0;
+          // t's tiles so far: bit 0 picks the barrier, bit 1 is its parity
+          if (!bad) bad = !mbar_wait(&pfull[2 * t + (op >> 2 * t & 1u)], op >> (2 * t + 1) & 1u, p.err, kErrTimeoutAccum);
+          op = t ? (op & 3u) | ((op + 4u) & 12u) : (op & 12u) | ((op + 1u) & 3u);
+          tc_fence_after();
+          const uint64_t b = dv + (uint32_t)vs * (2 * C::kSide >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              tc_mma_ts(tmem + kColO + 64 * t, tmem + kColP + 64 * t + kk * 8, b + 128 * kk, idesc_o,
-                        (i > 0 || kk > 0) ? 1u : 0u);
-            tc_commit(&ofull[t]);
+          for (int kk = 0; kk < 8; ++kk)
+            tc_mma_ts(tmem + kColO + 64 * t, tmem + pbuf * 128 + (kk >> 2) * KW + (kk & 3) * 8, b + 128 * kk, idesc_o,
+                      (n >= tiles || kk > 0) ? 1u : 0u);
+          tc_commit(&ofull[t]);
+          if (++pbuf == 3) pbuf = 0;
+          if (t == tiles - 1) {
+            tc_commit(&kvempty[vs]);
+            if (++vs == NS) vs = 0;
           }
-          tc_commit(&kvempty[vs]);
-          if (more) next_k();
-          if (++vs == NS) vs = 0;
+          if (n + ahead < total) issue_s(n + ahead);
         }
         mbar_arrive(&seg_empty[sb]);
       }
     }
     __syncwarp();
-  } else if (warp >= 12) {
+  } else if (warp >= SW + 4) {
     // ------------------------------------------- 8-bit tiles to bf16 tiles
     if (F8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-      const int tid = threadIdx.x & 127;
+      const int cw = warp - (SW + 4), tid = cw * 32 + lane;
       for (int sn = 0;; ++sn) {
         const int sb = sn & 1;
         if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
@@ -1115,17 +1161,25 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
           const uint8_t* raw = smem + C::kOffRaw + rs * 2 * C::kRawSide;
           const uint8_t* codes = smem + C::kOffCodes + rs * 2 * kRowsKT;
           uint8_t* dst = kv0 + st * 2 * C::kSide;
+          // 4 threads a key, 16 values each
+          constexpr int X = 512 / (CV * 32 + !F8);
+          uint4 w4[2 * X];
+          uint32_t code4[2 * X];
+#pragma unroll
+          for (int y = 0; y < 2 * X; ++y) {
+            w4[y] = *(const uint4*)(raw + (y * CV * 32 + tid) * 16);
+            code4[y] = codes[(y * CV * 32 + tid) >> 2];
+          }
 #pragma unroll
           for (int side = 0; side < 2; ++side)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              // 4 threads a key, 16 values each
-              const int idx = x * 128 + tid, key = idx >> 2, c = idx & 3;
-              const int32_t j = j0 + i * kRowsKT + key;
+            for (int x = 0; x < X; ++x) {
+              const int idx = x * CV * 32 + tid, key = idx >> 2, c = idx & 3;
+              const int32_t j = jt + key;
               uint32_t o[8];
               bool on = j >= lo && j < hi;  // a key nobody may see: zeros, whatever its page (or an earlier tile) holds
-              const uint4 w = *(const uint4*)(raw + side * C::kRawSide + idx * 16);
-              const uint32_t code = codes[side * kRowsKT + key];
+              const uint4 w = w4[side * X + x];
+              const uint32_t code = code4[side * X + x];
               if (side && edge) {
                 // V rows that are not finite, where some row does not see them: zeros and a mark, see the softmax
                 uint32_t n = 0;
@@ -1138,7 +1192,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
                   uint32_t bits = 0;
 #pragma unroll
                   for (int y = 0; y < 8; ++y) bits |= (bad4 >> (4 * y) & 15u) ? 1u << y : 0u;
-                  smem[C::kOffNan + st * 16 + x * 4 + (warp & 3)] = (uint8_t)bits;
+                  smem[C::kOffNan + st * 16 + x * CV + cw] = (uint8_t)bits;
                 }
               }
               if (on) {
@@ -1147,6 +1201,11 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
                 ch_e4m3_to_bf16(w.y, mul, o[2], o[3]);
                 ch_e4m3_to_bf16(w.z, mul, o[4], o[5]);
                 ch_e4m3_to_bf16(w.w, mul, o[6], o[7]);
+                if (code > kCodeOne) {
+                  const uint32_t rest = ch_code_rest(code);
+#pragma unroll
+                  for (int y = 0; y < 8; ++y) o[y] = bf16x2_mul(o[y], rest);
+                }
               } else {
 #pragma unroll
                 for (int y = 0; y < 8; ++y) o[y] = 0u;
@@ -1166,13 +1225,12 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
         __syncwarp();
       }
     }
-  } else if (warp >= 10) {
-    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  } else if (warp >= SW + 2) {
     if (!F8) {
       // ---------------------------------------------------- V rows at the edges
       // Rows that do not see a key have P = 0 there, and 0 times its V row must be 0: in tiles where some row does not,
       // the V rows of keys nobody sees and those that are not finite become zeros, the latter with a mark.
-      const int half = warp - 10;
+      const int half = warp - (SW + 2);
       for (int sn = 0;; ++sn) {
         const int sb = sn & 1;
         if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
@@ -1217,204 +1275,189 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
     }
   } else {
     // ----------------------------------------------------------- softmax
-    if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane;  // tile; row = TMEM lane
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegSoftmax));
+    // tile, half of its keys (and of the output's dims), row = TMEM lane
+    const int t = warp / (SW / 2), half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+    const int pair = 8 + t * 4 + (warp & 3);  // barrier of the two warps that share 32 rows
+    float* const own_max = (float*)(smem + C::kOffMax) + t * 256 + half * 128 + row;
+    const float* const other_max = (const float*)(smem + C::kOffMax) + t * 256 + (half ^ 1) * 128 + row;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_col = tmem + lane_base + (uint32_t)t * 128;
-    const uint32_t o_col = tmem + lane_base + kColO + 64 * t;
-    const uint32_t p_col = tmem + lane_base + kColP + 64 * t;
+    const uint32_t o_col = tmem + lane_base + kColO + 64 * t + DW * half;
     const int tok_r = row / p.G;  // token of the row within the tile
-    uint32_t par = 0;             // parity of the tile's products
+    uint32_t c = 0;               // key tiles of this tile so far
+    int buf0 = 0;                 // buffer of the part's first scores
     for (int sn = 0;; ++sn) {
       const int sb = sn & 1;
       if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
-      bad = ch_named_or(6, 256, bad);  // all eight warps leave together
+      bad = ch_named_or(6, SW * 32, bad);  // all softmax warps leave together
       const ChunkSeg& sg = segs[sb];
       if (sg.nrows < 0 || bad) break;
       const int ntile = sg.ntile, ntok = sg.ntok;
-      const bool tile_on = t == 0 || ntok > tq1;
+      const int32_t jbase = sg.j0, first = sg.first_pos;
+      const int tiles = ntok > tq1 ? 2 : 1;
+      const bool tile_on = t < tiles;
       const int tok = t * tq1 + tok_r;
       const bool row_ok = tok_r < tq1 && tok < ntok;
       const bool warp_on = __any_sync(0xffffffffu, row_ok);
       const int32_t lo = sg.lo;
-      const int32_t pos = row_ok ? sg.first_pos + tok : -1;
-      const int32_t tile_first = sg.first_pos + t * tq1, tile_last = sg.first_pos + min(ntok, (t + 1) * tq1) - 1;
+      const int32_t pos = row_ok ? first + tok : -1;
+      const int32_t tile_first = first + t * tq1, tile_last = first + min(ntok, (t + 1) * tq1) - 1;
       // a row that is not in use has whatever its place in shared memory held for a query: scale 0, reference 0
       const float scale = row_ok ? p.scale2 : 0.f;
-      float m_ref = row_ok ? -INFINITY : 0.f, l = 0.f, pend = 1.0f;  // pend: what O_t is still to be multiplied by
+      float m_ref = row_ok ? -INFINITY : 0.f, l = 0.f;
+      int buf = (buf0 + (tile_on ? t : 0)) % 3;
+      buf0 = (buf0 + ntile * tiles) % 3;
       if (tile_on) {
-        for (int i = 0; i < ntile; ++i) {
-          const int32_t j0 = sg.j0 + i * kRowsKT;
-          if (!bad) bad = !mbar_wait(&sfull[t], par, p.err, kErrTimeoutAccum);
+        for (int i = 0; i < ntile; ++i, ++c) {
+          const int32_t j0 = jbase + i * kRowsKT;
+          const uint32_t s_col = tmem + lane_base + (uint32_t)(buf * 128 + KW * half);  // P takes the place of S
+          buf = (buf + tiles) % 3;
+          const int st = (it + i) % NS;
+          if (!bad) bad = !mbar_wait(&sfull[2 * t + (c & 1)], c >> 1 & 1u, p.err, kErrTimeoutAccum);
           tc_fence_after();
           if (!warp_on) {  // no row of this warp is in use
-            if (!F8 && t == 0 && !bad)
-              bad = !mbar_wait(&vready[(it + i) % NS], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
+            if (!F8 && t == 0 && !bad) bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
             tc_fence_before();
-            if (lane == 0) {
-              mbar_arrive(&sfree[t]);
-              mbar_arrive(&pfull[t]);
-            }
-            par ^= 1u;
+            if (lane == 0) mbar_arrive(&pfull[2 * t + (c & 1)]);
             continue;
           }
           const bool whole = j0 + kRowsKT - 1 <= tile_first && j0 >= lo && (p.window <= 0 || j0 > tile_last - p.window);
-          auto masked = [&](uint32_t (&r)[32], int e0) {
+          uint32_t r[KW];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int32_t kj = j0 + e0 + e;
+          for (int e = 0; e < KW; e += 32) ch_ld32(s_col + e, r + e);
+          tmem_ld_wait();
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < KW; ++e) {
+              const int32_t kj = j0 + KW * half + e;
               if (kj > pos || (p.window > 0 && kj <= pos - p.window)) r[e] = __float_as_uint(-INFINITY);
             }
-          };
-          if (__any_sync(0xffffffffu, m_ref == -INFINITY)) {
-            // a row without a reference takes the largest score of its first tile (scale2 > 0)
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint32_t r[32];
-              ch_ld32(s_col + 32 * q4, r);
-              tmem_ld_wait();
-              if (!whole) masked(r, 32 * q4);
+          }
+          // the largest score of the row: both halves'
+          float mx0 = __uint_as_float(r[0]), mx1 = __uint_as_float(r[1]);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+          for (int e = 2; e + 2 < KW; e += 4) {
+            mx0 = ch_max3_nan(mx0, __uint_as_float(r[e]), __uint_as_float(r[e + 2]));
+            mx1 = ch_max3_nan(mx1, __uint_as_float(r[e + 1]), __uint_as_float(r[e + 3]));
+          }
+          mx0 = ch_max3_nan(mx0, __uint_as_float(r[KW - 2]), ch_max_nan(mx1, __uint_as_float(r[KW - 1])));
+          // The reference moves when the row's first scores come and when it falls 2^8 behind: P is at most 2^8, and a
+          // row's output is multiplied rarely.  The two warps of a row agree by one barrier whether any has to, and
+          // exchange their maxima only then.
+          float pend = 1.0f;
+          const bool over = row_ok && !(mx0 * scale <= m_ref + 8.0f);
+          const bool move = ch_named_or(pair, 64, over);
+          if (move) {
+            *own_max = mx0;
+            ch_named_sync(pair, 64);
+            mx0 = ch_max_nan(mx0, *other_max) * scale;
+            ch_named_sync(pair, 64);  // read before it is written again
+            if (row_ok && !(mx0 <= m_ref + 8.0f)) {
+              // NaN and infinity make the row NaN
+              if (mx0 == INFINITY) mx0 = __int_as_float(0x7FC00000);
+              pend = ch_exp2(m_ref - mx0);  // 0 for the first scores
+              l *= pend;
+              m_ref = mx0;
             }
-            if (m_ref == -INFINITY) m_ref = mx * scale;  // nothing of it in O or l yet
           }
-          // keys whose V row is not finite
-          uint4 nans = make_uint4(0, 0, 0, 0);
-          const bool edge = j0 + kRowsKT - 1 > sg.first_pos || j0 < lo ||
-                            (p.window > 0 && j0 <= sg.first_pos + ntok - 1 - p.window);
-          const int st = (it + i) % NS;
-          if (edge) {
-            if (!F8 && !bad) bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
-            nans = *(const uint4*)(smem + C::kOffNan + st * 16);
-          }
-          // P_t and O_t are free once the products of the tile before are done
-          if (i > 0) {
-            if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
-            tc_fence_after();
-          }
-          float sum, mx;
-          for (int again = 0;; ++again) {
-            // P = 2^(s - m) two at a time, the next 32 scores on their way meanwhile
+          {
             const float m_eff = m_ref == -INFINITY ? 0.f : m_ref;  // nothing seen so far: every P is 0
             const ch_f2 sc2 = ch_pair(scale, scale), nm2 = ch_pair(-m_eff, -m_eff);
             ch_f2 sum2 = 0ull;
-            mx = -INFINITY;
-            auto chunk = [&](uint32_t (&r)[32], int e0) {
-              if (!whole) masked(r, e0);
+#pragma unroll
+            for (int e0 = 0; e0 < KW; e0 += 32) {
               uint32_t pk[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                const ch_f2 x = ch_fma2(((ch_f2)r[2 * e + 1] << 32) | r[2 * e], sc2, nm2);
-                mx = fmaxf(mx, fmaxf(ch_lo(x), ch_hi(x)));
-                const float p0 = ch_exp2(ch_lo(x)), p1 = ch_exp2(ch_hi(x));
+                const ch_f2 x = ch_fma2(((ch_f2)r[e0 + 2 * e + 1] << 32) | r[e0 + 2 * e], sc2, nm2);
+                float p0, p1;
+                if (!F8 && (e & 7) == 7) {  // an eighth by the polynomial; 8 bit: the converters need those instructions
+                  ch_exp2_poly(x, p0, p1);
+                } else {
+                  p0 = ch_exp2(ch_lo(x));
+                  p1 = ch_exp2(ch_hi(x));
+                }
                 sum2 = ch_add2(sum2, ch_pair(p0, p1));
                 pk[e] = ch_bf16x2(p0, p1);
               }
-              ch_st16(p_col + e0 / 2, pk);
-            };
-            uint32_t ra[32], rb[32];
-            ch_ld32(s_col, ra);
-#pragma unroll 1
-            for (int e0 = 0; e0 < 128; e0 += 64) {
-              tmem_ld_wait();
-              ch_ld32(s_col + e0 + 32, rb);
-              chunk(ra, e0);
-              tmem_ld_wait();
-              if (e0 == 0) ch_ld32(s_col + 64, ra);
-              chunk(rb, e0 + 32);
+              ch_st16(s_col + e0 / 2, pk);
             }
-            sum = ch_lo(sum2) + ch_hi(sum2);
-            // The reference follows a tile later, P and l have room: 2^64.  Beyond that, once more with a new one (once:
-            // scores so large that their own rounding passes 2^6 have no right answer in fp32).
-            if (again || !__any_sync(0xffffffffu, mx > 64.0f)) break;
-            if (mx > 64.0f) {
-              const float c = ch_exp2(-mx);
-              pend *= c;
-              l *= c;
-              m_ref += mx;
-            }
+            l += ch_lo(sum2) + ch_hi(sum2);
           }
-          if ((nans.x | nans.y | nans.z | nans.w) != 0u) {
+          if (j0 + kRowsKT - 1 > first || j0 < lo || (p.window > 0 && j0 <= first + ntok - 1 - p.window)) {
             // P of the rows that see a key whose V row is not finite; the sum keeps its own
-            tmem_st_wait();
-#pragma unroll 1
-            for (int e = 0; e < 128; ++e) {
-              const uint32_t bits = e < 32 ? nans.x : e < 64 ? nans.y : e < 96 ? nans.z : nans.w;
-              if (!(bits >> (e & 31) & 1u)) continue;
-              const int32_t kj = j0 + e;
-              uint32_t w;
-              asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(w) : "r"(p_col + e / 2) : "memory");
-              tmem_ld_wait();
-              if (kj <= pos && (p.window <= 0 || kj > pos - p.window))
-                w = e & 1 ? (w & 0xFFFFu) | 0x7FC00000u : (w & 0xFFFF0000u) | 0x7FC0u;
-              asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(p_col + e / 2), "r"(w) : "memory");
+            if (!F8 && !bad) bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
+            const uint2 nans = *(const uint2*)(smem + C::kOffNan + st * 16 + 8 * half);
+            if ((nans.x | nans.y) != 0u) {
               tmem_st_wait();
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sfree[t]);  // S_t has been read
-          if (i > 0 && __any_sync(0xffffffffu, pend != 1.0f)) {
-            // O_t of the tiles before, before this one's product adds to it
 #pragma unroll 1
-            for (int hf = 0; hf < 2; ++hf) {
-              uint32_t ov[32];
-              tmem_ld_x32(o_col + 32 * hf, ov);
-              tmem_ld_wait();
-#pragma unroll
-              for (int d = 0; d < 32; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * pend);
-              tmem_st_x32(o_col + 32 * hf, ov);
+              for (int e = 0; e < KW; ++e) {
+                if (!((e < 32 ? nans.x : nans.y) >> (e & 31) & 1u)) continue;
+                const int32_t kj = j0 + KW * half + e;
+                uint32_t w;
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(w) : "r"(s_col + e / 2) : "memory");
+                tmem_ld_wait();
+                if (kj <= pos && (p.window <= 0 || kj > pos - p.window))
+                  w = e & 1 ? (w & 0xFFFFu) | 0x7FC00000u : (w & 0xFFFF0000u) | 0x7FC0u;
+                asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(s_col + e / 2), "r"(w) : "memory");
+                tmem_st_wait();
+              }
             }
           }
-          l += sum;
-          pend = 1.0f;
-          if (mx > 8.0f) {
-            pend = ch_exp2(-mx);
-            l *= pend;
-            m_ref += mx;
+          if (move && i > 0) {
+            // O_t has the tiles before.  (The wait cannot meet the product two before: this tile's scores were issued
+            // after it.)
+            if (!bad) bad = !mbar_wait(&ofull[t], (c & 1) ^ 1u, p.err, kErrTimeoutAccum);
+            tc_fence_after();
+            uint32_t ov[DW];
+            tmem_ld_x32(o_col, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int d = 0; d < DW; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * pend);
+            tmem_st_x32(o_col, ov);
           }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pfull[t]);
-          par ^= 1u;
+          if (lane == 0) mbar_arrive(&pfull[2 * t + (c & 1)]);
         }
       }
       it += ntile;
       // ------------------------------------------------- end of a part
       const int slot = sg.slot;
-      uint32_t ov[64];
+      uint32_t ov[DW];
+      if (tile_on) {  // the row's sum: the two halves' in their order
+        *own_max = l;
+        ch_named_sync(pair, 64);
+        l = half ? *other_max + l : l + *other_max;
+        ch_named_sync(pair, 64);
+      }
       if (tile_on && ntile > 0) {
-        if (!bad) bad = !mbar_wait(&ofull[t], par ^ 1u, p.err, kErrTimeoutAccum);
+        if (!bad) bad = !mbar_wait(&ofull[t], (c & 1) ^ 1u, p.err, kErrTimeoutAccum);
         tc_fence_after();
         ch_ld32(o_col, ov);
-        ch_ld32(o_col + 32, ov + 32);
         tmem_ld_wait();
         tc_fence_before();
-#pragma unroll
-        for (int d = 0; d < 64; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * pend);
       } else {
 #pragma unroll
-        for (int d = 0; d < 64; ++d) ov[d] = 0u;
+        for (int d = 0; d < DW; ++d) ov[d] = 0u;
       }
       if (row_ok) {
         const int hh = row - tok_r * p.G;
         if (slot >= 0) {
           const int64_t prow = (int64_t)slot * 256 + tok * p.G + hh;
-          *(float2*)(p.part_ml + prow * 2) = make_float2(m_ref, l);
+          if (half == 0) *(float2*)(p.part_ml + prow * 2) = make_float2(m_ref, l);
 #pragma unroll
-          for (int d = 0; d < 16; ++d)
-            *(uint4*)(p.part_o + prow * kChunkD + 4 * d) = make_uint4(ov[4 * d], ov[4 * d + 1], ov[4 * d + 2], ov[4 * d + 3]);
+          for (int d = 0; d < DW / 4; ++d)
+            *(uint4*)(p.part_o + prow * kChunkD + DW * half + 4 * d) = make_uint4(ov[4 * d], ov[4 * d + 1], ov[4 * d + 2], ov[4 * d + 3]);
         } else {
           const int h = sg.hg * p.G + hh;
           const int64_t tg = sg.tok0 + tok;
-          if (p.lse) p.lse[tg * p.Hq + h] = m_ref + log2f(l);
+          if (p.lse && half == 0) p.lse[tg * p.Hq + h] = m_ref + log2f(l);
           const float inv = ch_norm(p, h, l, m_ref);
-          uint4* orow = (uint4*)(p.o + (tg * p.Hq + h) * kChunkD);
+          uint4* orow = (uint4*)(p.o + (tg * p.Hq + h) * kChunkD + DW * half);
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
+          for (int d = 0; d < DW / 8; ++d) {
             uint32_t w[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y)
@@ -1425,19 +1468,19 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
       }
       if (slot >= 0) {
         __threadfence();
-        ch_named_sync(5, 256);
+        ch_named_sync(5, SW * 32);
         if (threadIdx.x == 0) {
           const uint32_t old = atomicAdd(&p.counters[sg.c0], 1u);
           const uint32_t last = old == (uint32_t)(sg.c1 - sg.c0);
           if (last) p.counters[sg.c0] = 0u;
           *flag = last;
         }
-        ch_named_sync(6, 256);
+        ch_named_sync(6, SW * 32);
         if (*flag) {
           __threadfence();
-          chunk_join(p, sg, 1, 256, threadIdx.x, 256);
+          chunk_join(p, sg, 1, 256, threadIdx.x, SW * 32);
         }
-        ch_named_sync(5, 256);  // flag is free again
+        ch_named_sync(5, SW * 32);  // flag is free again
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[sb]);
@@ -1445,7 +1488,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == SW + 1) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
