@@ -215,17 +215,18 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 // to the next takes about 2000 cycles whatever it holds).  From 32 rows on a
 // stream has 8 warps, two for the same keys with half of the rows each: a
 // thread's rows are unrolled, and past about 700 instructions a tile the
-// instruction cache, not the issue, sets the pace.  One TMA box brings a page's keys of both, in groups of 8 rows of 128
-// bytes (bf16: a head's, 8-bit: both heads' side by side), so that a head's 128
-// keys are one matrix operand with an even stride.  Two warps load: the copy engine takes 2 KB in about 97 cycles from two issuers,
-// 135 from one.  Per tile and stream:
-//   S^T [128 keys x W] = K Q^T    A = the K tile as it lies, B = Q, in TMEM
-//   a thread owns a key: its W scores are registers, the key's mask, scale
-//     and V exponent are its own constants
+// instruction cache, not the issue, sets the pace.  One TMA box brings a page's
+// keys of both, in groups of 8 rows of 128 bytes (bf16: a head's, 8-bit: both
+// heads' side by side), so that a head's 128 keys are one matrix operand with an
+// even stride.  Two warps load: the copy engine takes 2 KB in about 97 cycles
+// from two issuers, 135 from one.  Per tile and stream, N rows:
+//   S^T [128 keys x N] = K Q^T    A = the K tile as it lies, B = Q
+//   a thread owns a key: its N scores (or N / 2) are registers, the key's mask,
+//     scale and V exponent are its own constants
 //   O^T [64 dims x W] += V^T P^T  A = the V tile read dims-major, B = P^T,
-//     which the threads wrote to shared memory row by key
+//     which the threads wrote to shared memory row by key; W = N, 8-bit 2 N
 // With the keys on the 128-row side nothing is padded to 128 queries: 8 rows
-// (one token's group of heads) cost W = 16 columns.  (An mma.sync form of this
+// (one token's group of heads) cost N = 16 columns.  (An mma.sync form of this
 // kernel, rows on M, ran 32 x 5 tokens over 8191 8-bit keys in 317 us: legacy
 // mma.sync reaches 1009 multiply-adds per cycle and SM here, a quarter of
 // tcgen05's, and each 8-bit value had to be widened.)
@@ -234,13 +235,18 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 // e4m3 too, as two terms.  Q is scaled by a power of two per unit and head; hi =
 // Q to 4 significant bits and lo = the rest are two products into the same
 // columns (2^-18 of the largest).  P's terms have columns of their own, W = 2 N,
-// lo = 16 times the rest (2^-16 of the row's largest).  The key's power of two meets the
-// score in fp32; the value's goes into the exponent, t = s + e_v, and the
-// softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
+// lo = 16 times the rest (2^-16 of the row's largest).  The key's power of two
+// meets the score in fp32; the value's goes into the exponent, t = s + e_v, and
+// the softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
 //
 // The reference m of a row moves only when a score exceeds it by 8 (8-bit:
 // when P would pass 448), which one barrier of the stream's warps tells; then
 // O^T in TMEM is rescaled.
+//
+// Measured, 32 sequences of 8192 keys, 8 kv heads: one token 91 us in bf16 (5.9
+// TB/s, the bytes bound it), 68 us in 8 bits (4.0 TB/s: a tile's chain of barrier
+// waits, products and softmax, not the bytes, bounds it); five tokens 118 and 136
+// us (the softmax: 5 times the exponentials and, in 8 bits, P as two terms).
 template <bool F8, int N_>
 struct KeysCfg {
   static constexpr int N = N_;                             // rows of a unit
@@ -1581,11 +1587,28 @@ int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, i
   p.counters = (uint32_t*)((uint8_t*)workspace + 256);
   p.part_o = (float*)((uint8_t*)workspace + chunk_parts_at());
   const int64_t rows = (int64_t)max_q * p.G;
-  // the smallest tile that holds the longest chunk's rows
-  if (rows <= 16 && p.G <= 16) return f8 ? launch_keys<true, 16>(k, v, p, s) : launch_keys<false, 16>(k, v, p, s);
-  if (rows <= 32 && p.G <= 32) return f8 ? launch_keys<true, 32>(k, v, p, s) : launch_keys<false, 32>(k, v, p, s);
-  if (rows <= 48 && p.G <= 48) return f8 ? launch_keys<true, 48>(k, v, p, s) : launch_keys<false, 48>(k, v, p, s);
-  if (rows <= 64) return f8 ? launch_keys<true, 64>(k, v, p, s) : launch_keys<false, 64>(k, v, p, s);
+  // Rows of the longest chunk: up to 64 on the short side of the keys kernel, the smallest tile that holds them (32
+  // sequences of 8192 8-bit keys, one token: 68 us with 16 rows, 80 with 32, 90 with 48, 109 with 64; five tokens: 136
+  // with 48, 171 with 64).  The rows kernel pads them to 128 but takes a key tile in less time and has cheaper ends, so
+  // it is ahead with few (sequence, kv head) units, whose tiles are few per SM, and in bf16 with 64 rows always.  Keys /
+  // rows kernel in us, 8 kv heads, sequences x tokens on keys:
+  //   bf16  64 rows     64x8 on 512 67 / 44, on 8192 301 / 300;  16x8 on 8192 100 / 84;  1x8 on 8192 68 / 29
+  //   bf16  17..48      4x4 on 2048 23 / 17, on 8192 32 / 30;  1x6 on 8192 54 / 29;  but 16x4 on 8192 61 / 81
+  //   bf16  9..16       1x2 on 512 15 / 13, on 8192 34 / 21;  but 4x2 on 8192 26 / 29
+  //   8 bit 64 rows     16x8 on 2048 53 / 46, on 8192 114 / 122;  1x8 on 8192 76 / 35;  but 64x8 on 8192 363 / 446
+  //   8 bit 17..48      1x4 on 512 17 / 19, on 8192 42 / 27;  1x6 on 8192 59 / 36;  but 4x4 on 8192 33 / 41
+  // and with up to 8 rows the keys kernel, 4x1 on 8192: 20 / 29, 8 bit 19 / 38.
+  const int64_t units = (int64_t)p.N * p.Hkv, sms = device_sm_count();
+  const bool few = rows <= 8    ? false
+                   : rows <= 16 ? !f8 && 16 * units <= sms
+                   : rows <= 48 ? (f8 ? 16 : 4) * units <= sms
+                                : !f8 || units <= sms;
+  if (!few) {
+    if (rows <= 16 && p.G <= 16) return f8 ? launch_keys<true, 16>(k, v, p, s) : launch_keys<false, 16>(k, v, p, s);
+    if (rows <= 32 && p.G <= 32) return f8 ? launch_keys<true, 32>(k, v, p, s) : launch_keys<false, 32>(k, v, p, s);
+    if (rows <= 48 && p.G <= 48) return f8 ? launch_keys<true, 48>(k, v, p, s) : launch_keys<false, 48>(k, v, p, s);
+    if (rows <= 64 && f8) return launch_keys<true, 64>(k, v, p, s);
+  }
   return f8 ? launch_rows<true>(k, v, p, s) : launch_rows<false>(k, v, p, s);
 }
 

