@@ -390,3 +390,73 @@ def test_no_sequences_and_no_tokens():
     e = torch.zeros(0, dtype=torch.int32, device="cuda")
     o = chunk.attend_chunks(c.q[:0], c.k, c.v, c.table, e, c.q_start[:1], e, max_q=1)
     assert o.shape == (0, 64, 64)
+
+
+# Few short chunks share a kernel with the long ones; with many sequences they have their own.
+def many(q, window, f8, n=24, ring=None):
+    g = torch.Generator().manual_seed(100 * q + window)
+    ql = [q] + torch.randint(0, q + 1, (n - 1,), generator=g).tolist()
+    kl = [150 + q] + [max(a + b, 0) for a, b in zip(ql[1:], torch.randint(-2, 400, (n - 1,), generator=g).tolist())]
+    return Case(ql, kl, window=window, f8=f8, seed=q + window, ring=ring).gpu()
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("window", [0, 1, 100])
+@pytest.mark.parametrize("q", [1, 2, 3, 4, 5, 6, 7, 8, 9])
+def test_many_sequences(q, window, f8):
+    many(q, window, f8).check()
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("q,window", [(2, 0), (4, 0), (6, 100), (8, 0), (8, 20)])
+def test_many_sequences_hidden_and_not_finite(q, window, f8):
+    """Hidden keys of the first sequence change no bit; a value that is not
+    finite makes the rows that see it NaN and leaves all others their bits."""
+    c = many(q, window, f8, ring=30)
+    o, lse = c.check()
+    L = 150 + q
+    j = torch.arange(30 * PAGE, device="cuda")
+    hidden = (j >= L) | (j < (L - q - window + 1 if window else 0))
+    rows = (c.table[0].long()[j // PAGE] * PAGE + j % PAGE)[hidden]
+    for t, s in ((c.k, c.ks), (c.v, c.vs)):
+        if f8:
+            t.view(torch.uint8)[rows] = 0x7F
+            s.view(torch.uint8)[rows // PAGE, :, rows % PAGE] = 255
+        else:
+            t[rows] = math.nan
+    o2, lse2 = c.run()
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    at = q // 2
+    row = int(c.table[0, (L - q + at) // PAGE]) * PAGE + (L - q + at) % PAGE
+    if f8:
+        c.vs.view(torch.uint8)[row // PAGE, 2, row % PAGE] = 255
+    else:
+        c.v[row, 2, 7] = math.inf
+    o2, lse2 = c.run()
+    sees = torch.zeros(o.shape[:2], dtype=torch.bool, device="cuda")
+    sees[at:(min(q, at + window) if window else q), 16:24] = True
+    assert torch.equal(o[~sees], o2[~sees]) and bool(((lse - lse2).abs()[torch.isfinite(lse)] <= 1e-4).all())
+    assert not bool(torch.isfinite(o2[sees][:, 7]).any())
+
+
+@pytest.mark.parametrize("hq,hkv,q", [(8, 8, 20), (12, 4, 14), (10, 2, 8), (64, 1, 1), (40, 8, 6)])
+@pytest.mark.parametrize("f8", [False, True])
+def test_many_sequences_head_groups(hq, hkv, q, f8):
+    Case([q] * 40, [q + 7 * b for b in range(40)], hq=hq, hkv=hkv, f8=f8, seed=hq + q).gpu().check()
+
+
+@pytest.mark.parametrize("q", [1, 4, 40])
+def test_infinite_scores_make_their_rows_nan(q):
+    """A key of +infinity in one dim: the rows with a positive query there have an infinite score, and
+    infinity - infinity is no number; those with a negative one do not weigh it at all."""
+    c = Case([q], [200], seed=q).gpu()
+    pos = 200 - q   # every token sees it
+    row = int(c.table[0, pos // PAGE]) * PAGE + pos % PAGE
+    before = c.k[row, 3].clone()
+    c.k[row, 3, 9] = math.inf
+    o, lse = c.run()
+    up = torch.zeros(q, 64, dtype=torch.bool, device="cuda")
+    up[:, 24:32] = c.q[:, 24:32, 9] > 0
+    assert bool(torch.isnan(o[up]).all()) and bool(torch.isfinite(o[~up]).all())
+    c.k[row, 3] = before
+    c.check()
