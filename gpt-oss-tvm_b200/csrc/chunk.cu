@@ -1597,11 +1597,14 @@ int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, i
   //   bf16  9..16       1x2 on 512 15 / 13, on 8192 34 / 21;  but 4x2 on 8192 26 / 29
   //   8 bit 64 rows     16x8 on 2048 53 / 46, on 8192 114 / 122;  1x8 on 8192 76 / 35;  but 64x8 on 8192 363 / 446
   //   8 bit 17..48      1x4 on 512 17 / 19, on 8192 42 / 27;  1x6 on 8192 59 / 36;  but 4x4 on 8192 33 / 41
-  // and with up to 8 rows the keys kernel, 4x1 on 8192: 20 / 29, 8 bit 19 / 38.
+  // and with up to 8 rows the keys kernel, 4x1 on 8192: 20 / 29, 8 bit 19 / 38.  The keys a token can reach count the
+  // same way (`span`, from the window and the table): bf16 33..48 rows, 64x6 on 512 49 / 43, on 2048 88 / 90; 16x6 on
+  // 2048 38 / 33.
   const int64_t units = (int64_t)p.N * p.Hkv, sms = device_sm_count();
+  const int64_t pages = (int64_t)p.tstride * kChunkPage, span = p.window > 0 ? min64((int64_t)p.window + max_q, pages) : pages;
   const bool few = rows <= 8    ? false
                    : rows <= 16 ? !f8 && 16 * units <= sms
-                   : rows <= 48 ? (f8 ? 16 : 4) * units <= sms
+                   : rows <= 48 ? (f8 ? 16 : 4) * units <= sms || (!f8 && rows > 32 && span <= 2048)
                                 : !f8 || units <= sms;
   if (!few) {
     if (rows <= 16 && p.G <= 16) return f8 ? launch_keys<true, 16>(k, v, p, s) : launch_keys<false, 16>(k, v, p, s);

@@ -172,16 +172,28 @@ __device__ __forceinline__ long long warp_scan64(long long v) {
   }
   return v;
 }
-// Value of a shared variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t ld_cluster_u32(const void* p, uint32_t rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
-  return v;
+// Exchange in a cluster without its barriers (whose release waits for every store
+// of every warp, about 1600 cycles each): a value is written into another CTA's
+// shared memory together with the bytes that the mbarrier there counts.
+__device__ __forceinline__ void ver_push(void* slot, uint64_t* bar, uint32_t rank, long long v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
+                   mapa_shared(smem_u32(slot), rank)),
+               "l"(v), "r"(mapa_shared(smem_u32(bar), rank))
+               : "memory");
 }
-__device__ __forceinline__ long long ld_cluster_s64(const void* p, uint32_t rank) {
-  long long v;
-  asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
-  return v;
+// One thread: `bar` for `bytes` bytes.  Then all: ver_cluster_arrive, and ver_cluster_wait before the first push (every
+// CTA runs and has its barriers by then; nothing else is ordered, so the arrival may be relaxed).
+__device__ __forceinline__ void ver_expect(uint64_t* bar, uint32_t bytes) {
+  mbar_init(bar, 1);
+  fence_mbar_init();
+  mbar_arrive_expect_tx(bar, bytes);
+}
+__device__ __forceinline__ void ver_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void ver_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ bool ver_wait(uint64_t* bar) {
+  for (uint32_t i = 0; i < kWaitPolls; ++i)
+    if (mbar_try_wait(bar, 0u)) return true;
+  return false;
 }
 
 // The pieces [lo, hi) of a row that CTA `rank` of `n` takes.
@@ -240,10 +252,16 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
   T* keep = (T*)ver_smem;  // this CTA's slice, when `stash`
   __shared__ float wm[kVerWarps];
   __shared__ long long ws[kVerWarps];
-  __shared__ float cta_m;
-  __shared__ long long cta_s;
+  __shared__ long long maxima[kVerCluster], sums[kVerCluster];  // of the cluster's CTAs; the sums in the first one only
+  __shared__ uint64_t max_bar, sum_bar;
   cudaTriggerProgrammaticLaunchCompletion();  // the next kernel may take its place and wait
   const uint32_t rank = cluster_ctarank();
+  if (threadIdx.x == 0) {
+    ver_expect(&max_bar, (uint32_t)C * 8);
+    ver_expect(&sum_bar, (uint32_t)C * 8);
+  }
+  __syncwarp();
+  ver_cluster_arrive();
   const int64_t r = blockIdx.x / (unsigned)C;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* row = (const T*)p.logits + r * p.ld;
@@ -256,13 +274,14 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) wm[warp] = m;
   __syncthreads();
+  ver_cluster_wait();
   if (warp == 0) {
     m = lane < kVerWarps ? wm[lane] : -INFINITY;
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) cta_m = m;
+    if (lane < C) ver_push(&maxima[rank], &max_bar, (uint32_t)lane, (long long)__float_as_uint(m));
   }
-  cluster_sync_all();
-  m = lane < C ? __uint_as_float(ld_cluster_u32(&cta_m, lane)) : -INFINITY;
+  const bool came = ver_wait(&max_bar);
+  m = lane < C ? __uint_as_float((uint32_t)maxima[lane]) : -INFINITY;
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   // pass 2: the sums of the pieces' weights, or the lowest index of the maximum
   const T* src = stash ? keep + pad : row + lo;
@@ -295,18 +314,18 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
     if (lane == 0) ws[warp] = mi;
   }
   __syncthreads();
-  if (warp == 0) {
-    if (!p.greedy) {
-      const long long sum = warp_sum64(lane < kVerWarps ? ws[lane] : 0);
-      if (lane == 0) cta_s = sum;
-    } else {
-      const int mi = __reduce_min_sync(0xffffffffu, lane < kVerWarps ? (int)ws[lane] : 0x7FFFFFFF);
-      if (lane == 0) cta_s = mi;
-    }
+  // nothing comes here any more but to the first CTA, the others are done
+  if (warp != 0) return;
+  {
+    long long part = p.greedy ? __reduce_min_sync(0xffffffffu, lane < kVerWarps ? (int)ws[lane] : 0x7FFFFFFF)
+                              : warp_sum64(lane < kVerWarps ? ws[lane] : 0);
+    if (!came) part = -1;  // a bounded wait that ran out
+    if (lane == 0) ver_push(&sums[rank], &sum_bar, 0u, part);
   }
-  cluster_sync_all();
-  if (rank == 0 && warp == 0) {
-    const long long part = lane < C ? ld_cluster_s64(&cta_s, lane) : p.greedy ? 0x7FFFFFFF : 0;
+  if (rank == 0) {
+    const bool all = ver_wait(&sum_bar);
+    const long long part = lane < C ? sums[lane] : p.greedy ? 0x7FFFFFFF : 0;
+    const bool good = __all_sync(0xffffffffu, all && part >= 0);
     const long long z = p.greedy ? 0 : warp_sum64(part);
     const int mi = p.greedy ? __reduce_min_sync(0xffffffffu, (int)part) : -1;
     if (lane == 0) {
@@ -325,11 +344,10 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
       }
       p.row_max[r] = m;
       p.row_sum[r] = z;
-      p.row_top[r] = mi;
-      p.row_ok[r] = ok;
+      p.row_top[r] = good ? mi : -2;
+      p.row_ok[r] = good && ok;
     }
   }
-  cluster_sync_all();  // nobody leaves while its shared memory may be read
 }
 
 // One CTA per sequence, or with kDraft a cluster of kVerNextCluster.
@@ -338,7 +356,8 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
   extern __shared__ __align__(16) uint8_t ver_smem[];
   long long* mine = (long long*)ver_smem;  // kDraft: sums of this CTA's pieces
   __shared__ long long ws[kVerWarps];
-  __shared__ long long cta_s, found_run;
+  __shared__ long long sums[kVerNextCluster], found_run;
+  __shared__ uint64_t sum_bar;
   __shared__ int found;
   const uint32_t rank = kDraft ? cluster_ctarank() : 0u;
   const int b = blockIdx.x / (kDraft ? kVerNextCluster : 1);
@@ -362,11 +381,12 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
   }
   at = min64(at, r1 - 1);
   const bool last = at == r1 - 1;
+  const bool lost = p.row_top[at] == -2;  // its cluster's exchange did not come to its end
   if (rank == 0 && threadIdx.x == 0) {
     p.accepted[b] = (int32_t)(at - r0);
-    if (p.greedy) p.next[b] = p.row_top[at];
+    if (p.greedy || lost) p.next[b] = max(p.row_top[at], -1);
   }
-  if (p.greedy) return;
+  if (p.greedy || lost) return;
   const T* row = (const T*)p.logits + at * p.ld;
   const float* qrow = kDraft ? p.draft + at * p.ld_draft : nullptr;
   const float m = p.row_max[at];
@@ -427,6 +447,9 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
       ver_fix(fminf(fmaxf(__fsub_rn(__fdiv_rn(e, total), fmaxf(qrow[i], -INFINITY)), 0.0f), 1.0f), h, l);  // as in the sums
       return ver_join(h, l);
     };
+    if (threadIdx.x == 0) ver_expect(&sum_bar, kVerNextCluster * 8);
+    __syncwarp();
+    ver_cluster_arrive();
     const bool wide = ((uintptr_t)row & (4 * sizeof(T) - 1)) == 0, wide_q = ((uintptr_t)qrow & 15) == 0;
     int plo, phi;
     ver_slice(p.pieces, rank, kVerNextCluster, plo, phi);
@@ -457,19 +480,22 @@ __global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyPa
     }
     if (lane == 0) ws[warp] = sum;
     __syncthreads();
+    ver_cluster_wait();
     if (warp == 0) {
       sum = warp_sum64(lane < kVerWarps ? ws[lane] : 0);
-      if (lane == 0) cta_s = sum;
+      if (lane < kVerNextCluster) ver_push(&sums[rank], &sum_bar, (uint32_t)lane, sum);
     }
-    cluster_sync_all();
+    if (!__syncthreads_and(ver_wait(&sum_bar))) {  // a bounded wait that ran out
+      if (rank == 0 && threadIdx.x == 0) p.next[b] = -1;
+      return;
+    }
     long long before = 0, all = 0, here = 0;
     for (uint32_t c = 0; c < kVerNextCluster; ++c) {
-      const long long s = ld_cluster_s64(&cta_s, c);
-      if (c < rank) before += s;
-      if (c == rank) here = s;
-      all += s;
+      const long long v = sums[c];
+      if (c < rank) before += v;
+      if (c == rank) here = v;
+      all += v;
     }
-    cluster_sync_all();  // nobody leaves while its shared memory may be read
     if (all > 0) {
       const long long u = draw(all);
       if (u >= before && u < before + here)
