@@ -67,6 +67,8 @@ __device__ __forceinline__ uint32_t kv8_rest(uint32_t code) {
   return h | (h << 16);
 }
 
+constexpr int kKv8Tokens = 16, kKv8Blocks = 4;  // the most tokens of a block; blocks an SM holds
+
 struct Kv8Rope {
   float inv_freq[kKv8D / 2];
 };
@@ -77,19 +79,35 @@ struct Kv8Rope {
 // 16-byte loads, and the row's largest magnitude takes two shuffles.  The
 // rotation rounds as qkv_rope_kernel's does (the same q bits; k is rounded to
 // bf16 before it is quantised, so the cache holds e4m3 of the bf16 cache's k).
-// Measured, 64 + 2 x 8 heads: 8192 tokens in 39 us, 4.1 TB/s, 160 tokens in 4.4:
-// the rotation and a row's exponent stand between a token's loads and its stores,
-// and with 46 registers five blocks an SM do not cover that.
-__global__ void __launch_bounds__(256)
+// Measured, 64 + 2 x 8 heads: 8192 tokens in 34 us, 4.7 TB/s, 160 tokens in 4.0:
+// the rotation and a row's exponent stand between a token's loads and its stores.
+// Four blocks an SM with the next loads under way are ahead of five (36 us) and
+// six (42), one wave of them of twelve an SM (35) and of blocks of 4 tokens without
+// the early loads (38).
+__global__ void __launch_bounds__(256, kKv8Blocks)
     qkv_rope_append_f8_kernel(const uint16_t* __restrict__ qkv, const int32_t* __restrict__ pos,
                               const int32_t* __restrict__ slot, int64_t S, int64_t pool_rows, int32_t Hq, int32_t Hkv,
                               const Kv8Rope tab, float conc, int32_t tok_per_block, uint16_t* __restrict__ q_out,
                               uint8_t* __restrict__ kp, uint8_t* __restrict__ vp, uint8_t* __restrict__ kcode,
                               uint8_t* __restrict__ vcode) {
-  __shared__ __align__(16) float cos_s[8 * 32];
-  __shared__ __align__(16) float sin_s[8 * 32];
+  __shared__ __align__(16) float cos_s[kKv8Tokens * 32];
+  __shared__ __align__(16) float sin_s[kKv8Tokens * 32];
+  __shared__ int32_t slot_s[kKv8Tokens];
   const int64_t s0 = (int64_t)blockIdx.x * tok_per_block;
   const int nt = (int)min64(tok_per_block, S - s0);
+  const int32_t Ht = Hq + 2 * Hkv;
+  const int total = nt * Ht * 4;
+  // a lane's 32 bytes; those of the next round are on their way while one is worked on
+  uint4 na = make_uint4(0, 0, 0, 0), nb = na;
+  auto fetch = [&](int i) {
+    if (i < total) {
+      const uint16_t* xr = qkv + (s0 * Ht + (i >> 2)) * kKv8D + 8 * (i & 3);
+      na = ldg_nc_v4(xr);
+      nb = ldg_nc_v4(xr + 32);
+    }
+  };
+  fetch((int)threadIdx.x);
+  if ((int)threadIdx.x < nt && slot) slot_s[threadIdx.x] = slot[s0 + threadIdx.x];
   for (int i = threadIdx.x; i < nt * 32; i += blockDim.x) {
     const float ang = __fmul_rn((float)pos[s0 + (i >> 5)], tab.inv_freq[i & 31]);
     float sn, cs;
@@ -98,20 +116,14 @@ __global__ void __launch_bounds__(256)
     sin_s[i] = __fmul_rn(sn, conc);
   }
   __syncthreads();
-  const int32_t Ht = Hq + 2 * Hkv;
-  const int total = nt * Ht * 4;
   // whole groups of 4 lanes run or skip together; every lane of a warp stays in the loop for the shuffles
   for (int base = 0; base < total; base += blockDim.x) {
     const int i = base + threadIdx.x;
     const bool on = i < total;
     const int l = i & 3, h = on ? (i >> 2) % Ht : 0, tk = on ? (i >> 2) / Ht : 0;
     const int64_t s = s0 + tk;
-    const uint16_t* xr = qkv + (s * Ht + h) * kKv8D;
-    uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
-    if (on) {
-      xa = ldg_nc_v4(xr + 8 * l);
-      xb = ldg_nc_v4(xr + 32 + 8 * l);
-    }
+    const uint4 xa = na, xb = nb;
+    fetch(i + (int)blockDim.x);
     const uint32_t wa[4] = {xa.x, xa.y, xa.z, xa.w}, wb[4] = {xb.x, xb.y, xb.z, xb.w};
     float a[8], b[8];
 #pragma unroll
@@ -149,6 +161,7 @@ __global__ void __launch_bounds__(256)
         qd[4] = make_uint4(rb[0], rb[1], rb[2], rb[3]);
       }
     }
+    if (!__any_sync(0xffffffffu, on && h >= Hq)) continue;
     uint32_t am = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) am = max(am, max(abs_bits(a[k]), abs_bits(b[k])));
@@ -156,7 +169,7 @@ __global__ void __launch_bounds__(256)
     am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
     if (on && h >= Hq) {
       const int hk = h < Hq + Hkv ? h - Hq : h - Hq - Hkv;
-      const int64_t row = slot ? (int64_t)slot[s] : s;
+      const int64_t row = slot ? (int64_t)slot_s[tk] : s;
       if (row >= 0 && row < pool_rows) {
         const uint32_t code = kv8_code(am);
         const float inv = kv8_inv_scale(code);
@@ -279,7 +292,9 @@ int launch_qkv_rope_append_f8(const uint16_t* qkv, const int32_t* pos, const int
   if (S <= 0) return 0;
   Kv8Rope tab;
   for (int i = 0; i < kKv8D / 2; ++i) tab.inv_freq[i] = inv_freq[i];
-  const int tpb = S >= 8 * (int64_t)device_sm_count() ? 4 : 1;
+  // one wave of blocks: their tokens' loads, sincosf and stores overlap better than a second wave's start
+  const int64_t wave = (int64_t)device_sm_count() * kKv8Blocks;
+  const int tpb = (int)min64((S + wave - 1) / wave, kKv8Tokens);
   qkv_rope_append_f8_kernel<<<(unsigned)((S + tpb - 1) / tpb), 256, 0, s>>>(qkv, pos, slot, S, pool_rows, Hq, Hkv, tab,
                                                                             conc, tpb, q_out, kp, vp, kcode, vcode);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;

@@ -25,13 +25,14 @@
 //                       (the maximum, expf, floor and two sums), and a CTA's
 //                       load, cluster barrier and sums follow one another; four
 //                       CTAs an SM cover part of it.  168 rows of 201088 fp32
-//                       logits: 79 us, 1.7 TB/s
+//                       logits: 61 us, 2.2 TB/s (79 with cluster barriers)
 // verify_next_kernel    one CTA per sequence: the first rejected row, the piece
 //                       that holds the draw from the stored sums, and the
 //                       token in it.  Only with draft distributions the
 //                       residual needs the whole row again: then a cluster per
-//                       sequence sums its pieces first (48 sequences: 50 us,
-//                       51 instructions a value, an IEEE division among them)
+//                       sequence sums its pieces first (48 sequences: 37 us,
+//                       51 instructions a value, an IEEE division among them;
+//                       49 us where four CTAs fit an SM instead of five)
 #include "common.cuh"
 #include "launch.h"
 
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(kVerThreads) verify_rows_kernel(const VerifyPa
 
 // One CTA per sequence, or with kDraft a cluster of kVerNextCluster.
 template <typename T, bool kDraft>
-__global__ void __launch_bounds__(kVerThreads) verify_next_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerThreads, 5) verify_next_kernel(const VerifyParams p) {
   extern __shared__ __align__(16) uint8_t ver_smem[];
   long long* mine = (long long*)ver_smem;  // kDraft: sums of this CTA's pieces
   __shared__ long long ws[kVerWarps];
