@@ -879,16 +879,18 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
 // shared memory, TMEM) waits behind those.  So a step has few: the row's two
 // warps agree by one barrier whether a reference has to move (they exchange
 // maxima only then), and wait for O_t only then.  Measured, 2048 tokens on a
-// sequence of 32768: 1338 us in bf16, 800 TFLOP/s, 3000 cycles a key tile.  One
+// sequence of 32768: 1342 us in bf16, 794 TFLOP/s, 3000 cycles a key tile.  One
 // softmax warpgroup a tile took 1718, two that exchange every maximum 1504,
 // turns between the tiles by a barrier 1480; without the polynomial below 1421.
 //
 // 8-bit pages: two more warpgroups turn a tile's values into bf16 with their
 // power of two (exact) while those before are used: 60 instructions for 32 x 16
-// values; the rest of the kernel is the same.  1867 us for the same call: a key
+// values; the rest of the kernel is the same.  1872 us for the same call: a key
 // tile's conversion is a third of the instructions that its softmax is.  (One
 // converting warpgroup: 3121.)
 constexpr int kRowsKT = 128;
+// Bits 0 .. n set (none for n < 0).
+__device__ __forceinline__ uint32_t ch_bits_to(int32_t n) { return n < 0 ? 0u : n >= 31 ? ~0u : (2u << n) - 1u; }
 __device__ __forceinline__ float ch_max_nan(float a, float b) {
   float m;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
@@ -1333,11 +1335,12 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
           for (int e = 0; e < KW; e += 32) ch_ld32(s_col + e, r + e);
           tmem_ld_wait();
           if (!whole) {
+            // bit e: the row sees key e of the warp's 64
+            const int32_t top = pos - (j0 + KW * half), low = p.window > 0 ? top - p.window : -1;
+            const uint32_t see[2] = {ch_bits_to(top) & ~ch_bits_to(low), ch_bits_to(top - 32) & ~ch_bits_to(low - 32)};
 #pragma unroll
-            for (int e = 0; e < KW; ++e) {
-              const int32_t kj = j0 + KW * half + e;
-              if (kj > pos || (p.window > 0 && kj <= pos - p.window)) r[e] = __float_as_uint(-INFINITY);
-            }
+            for (int e = 0; e < KW; ++e)
+              if (!(see[e >> 5] >> (e & 31) & 1u)) r[e] = __float_as_uint(-INFINITY);
           }
           // the largest score of the row: both halves'
           float mx0 = __uint_as_float(r[0]), mx1 = __uint_as_float(r[1]);
@@ -1553,7 +1556,11 @@ int launch_rows(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
   p.TQ = 2 * tq1;
   p.HG = p.Hkv;
   p.lg_kt = 7;
-  p.ov = 3;
+  // A unit's ends cost about 3 key tiles (4 prompts of 1024: 104 us; with 2 112, with 5 114).  Where a window leaves it
+  // no more than that many tiles and every SM has several, a cut through one costs more than it evens out: 8 makes cuts
+  // fall between units (2048 tokens, window 128: 41 us, 52 with 3; but 32 x 5 tokens, under two an SM: 22.5, 21.4).
+  const bool small = p.window > 0 && p.window + p.TQ <= 3 * kRowsKT;
+  p.ov = small && (p.T / p.TQ + p.N) * p.HG > 3 * grid ? 8 : 3;
   if (!chunk_fits(p, kRowsKT)) return -12;
   p.part_ml = p.part_o + (int64_t)2 * grid * 256 * kChunkD;
   CUtensorMap tq, tk, tv;
