@@ -784,7 +784,8 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
               for (int e = 0; e < 8; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], o);
             if (lane == 0) {
 #pragma unroll
-              for (int e = 0; e < 8; e += 4) *(float4*)(red + sum_at * N + rb + r0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+              for (int e = 0; e < 8; e += 4)
+                *(float4*)(red + sum_at * N + rb + r0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             }
           }
         }
@@ -934,7 +935,7 @@ struct RowsCfg {
   static constexpr int kRawSide = kRowsKT * 64;
   static constexpr int kOffRaw = 2 * 128 * 128 + kStages * 2 * kSide;
   static constexpr int kOffCodes = kOffRaw + kRaw * 2 * kRawSide;
-  static constexpr int kOffNan = kOffCodes + kRaw * 2 * kRowsKT;  // per stage: a bit for each key whose V row is not finite
+  static constexpr int kOffNan = kOffCodes + kRaw * 2 * kRowsKT;  // per stage: a bit for each key, V row not finite
   static constexpr int kOffMax = kOffNan + kStages * 16;  // [tile][half][128]: maxima, at the end sums
   static constexpr int kOffPre = kOffMax + 2 * 2 * 128 * 4;
   static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
@@ -1324,7 +1325,8 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
           if (!bad) bad = !mbar_wait(&sfull[2 * t + (c & 1)], c >> 1 & 1u, p.err, kErrTimeoutAccum);
           tc_fence_after();
           if (!warp_on) {  // no row of this warp is in use
-            if (!F8 && t == 0 && !bad) bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
+            if (!F8 && t == 0 && !bad)
+              bad = !mbar_wait(&vready[st], (uint32_t)((it + i) / NS) & 1u, p.err, kErrTimeoutFull);
             tc_fence_before();
             if (lane == 0) mbar_arrive(&pfull[2 * t + (c & 1)]);
             continue;
@@ -1380,7 +1382,7 @@ __global__ void __launch_bounds__(RowsCfg<F8>::kThreads, 1)
               for (int e = 0; e < 16; ++e) {
                 const ch_f2 x = ch_fma2(((ch_f2)r[e0 + 2 * e + 1] << 32) | r[e0 + 2 * e], sc2, nm2);
                 float p0, p1;
-                if (!F8 && (e & 7) == 7) {  // an eighth by the polynomial; 8 bit: the converters need those instructions
+                if (!F8 && (e & 7) == 7) {  // an eighth; 8 bit: the converters need those instructions
                   ch_exp2_poly(x, p0, p1);
                 } else {
                   p0 = ch_exp2(ch_lo(x));

@@ -21,11 +21,11 @@
 //                       shared memory between the maximum and the sums, so the
 //                       logits are read once; the sums of pieces of 256 values
 //                       go to the scratch buffer
-//                       Bound by issue and latency: 33 instructions a value
+//                       Bound by issue and latency: 30 instructions a value
 //                       (the maximum, expf, floor and two sums), and a CTA's
-//                       load, cluster barrier and sums follow one another; four
+//                       load, exchange and sums follow one another; four
 //                       CTAs an SM cover part of it.  168 rows of 201088 fp32
-//                       logits: 61 us, 2.2 TB/s (79 with cluster barriers)
+//                       logits: 60 us, 2.2 TB/s (79 with cluster barriers)
 // verify_next_kernel    one CTA per sequence: the first rejected row, the piece
 //                       that holds the draw from the stored sums, and the
 //                       token in it.  Only with draft distributions the

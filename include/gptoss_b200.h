@@ -253,7 +253,7 @@ int gptoss_kv_pages_copy(uint16_t* k_pages, uint16_t* v_pages, int32_t Hkv, int3
  * j > pos_i - W; one that sees nothing (kv_len[b] smaller than its chunk, or a
  * seq_rows[b] outside the table) gives o = 0 and lse = -inf.  What keys and
  * values a token does not see hold does not matter to it, NaN included; one that
- * sees a value that is not finite gets NaN.
+ * sees a value that is not finite, or has a score of NaN or +infinity, gets NaN.
  * Pages: bf16, or with kv_f8 e4m3 values and codes as gptoss_qkv_rope_append_f8
  * writes them; num_pages pages in each pool.  max_q: the longest chunk, known
  * to the host (it picks the kernel; a longer chunk is still computed right).
@@ -358,7 +358,8 @@ int gptoss_sample_top_p_from_logits(const float* logits, int64_t B, int64_t V, d
  * temperature < 1e-6: a draft is accepted iff it is the argmax (lowest index),
  * and the next token is the argmax; the random numbers may be NULL.  A NaN
  * logit counts as -inf; a draft outside 0 .. V - 1 is not accepted; a sequence
- * without rows gives 0 and -1.  All memory on the device; V at most 2^22. */
+ * without rows gives 0 and -1, and a device wait that ran out -1.  All memory on
+ * the device; V at most 2^22. */
 int64_t gptoss_verify_drafts_scratch_bytes(int64_t T, int64_t V);
 int gptoss_verify_drafts(const void* logits, int32_t logits_bf16, int64_t ld_logits, const int32_t* tokens,
                          const int32_t* row_start, int64_t T, int32_t N, int32_t V, double temperature,
