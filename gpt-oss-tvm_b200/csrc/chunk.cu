@@ -16,8 +16,9 @@
 //
 // The output is rounded once, from fp32; P is rounded to bf16 as the operand
 // of P V (its relative error of 2^-9 an element is the size of the output's
-// own rounding; 8-bit pages split it into two e4m3 terms, with less error), the
-// sum l takes the unrounded values.
+// own rounding; chunk_keys_kernel over 8-bit pages splits it into two e4m3
+// terms, 2^-8 of itself, in units that follow each row's largest of a key tile,
+// see there), the sum l takes the unrounded values.
 #include "chunk.cuh"
 #include "launch.h"
 
@@ -41,6 +42,33 @@ __device__ __forceinline__ float ch_exp2(float x) {
 __device__ __forceinline__ uint32_t ch_e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two 16-bit floats as e4m3 bytes (nearest, ties to even; saturates) and back (exact).
+__device__ __forceinline__ uint32_t ch_e4m3x2_f16(uint32_t f16x2) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(f16x2));
+  return r;
+}
+__device__ __forceinline__ uint32_t ch_f16x2_e4m3(uint32_t e4m3x2) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)e4m3x2));
+  return r;
+}
+__device__ __forceinline__ uint32_t ch_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// a * b + c and a * b of two 16-bit floats
+__device__ __forceinline__ uint32_t ch_hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t ch_hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 // x rounded to 4 significant bits (half away from zero), exact in e4m3 for 2^-6 <= |x| <= 448
@@ -234,14 +262,21 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 // 8-bit pages are operands as they are (kind::f8f6f4).  The other side is then
 // e4m3 too, as two terms.  Q is scaled by a power of two per unit and head; hi =
 // Q to 4 significant bits and lo = the rest are two products into the same
-// columns (2^-18 of the largest).  P's terms have columns of their own, W = 2 N,
-// lo = 16 times the rest (2^-16 of the row's largest).  The key's power of two
-// meets the score in fp32; the value's goes into the exponent, t = s + e_v, and
-// the softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
+// columns (2^-18 of the largest).  P's terms have columns of their own, W = 2 N:
+// hi = P in e4m3, lo = 32 times what that leaves, 2^-8 of P in all.  The key's
+// power of two meets the score in fp32; the value's goes into the exponent, t = s
+// + e_v, and the softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
 //
-// The reference m of a row moves only when a score exceeds it by 8 (8-bit:
-// when P would pass 448), which one barrier of the stream's warps tells; then
-// O^T in TMEM is rescaled.
+// The reference m of a row moves up when a score exceeds it by 8, which one
+// barrier of the stream's warps tells; then O^T in TMEM is rescaled.  In 8 bits
+// it moves down, too, when no P of the row reaches 1 in a tile: the two terms end
+// at 2^-15, and thousands of keys that each fall below it may weigh as much as the
+// largest.  Each second tile is looked at (24 more instructions a thread), which
+// bounds what is lost: of the row's largest so far, which is 2^3 or more in units
+// of 2^m, 2^-18 a key; and of the 128 or 256 keys of a tile 2^-7 at most of the
+// tile before, whose largest P is 1 or more.  kDepth bounds the way down from the
+// row's highest reference, since O^T and l are multiplied on the way: keys that
+// far below it weigh nothing beside the one that set it.
 //
 // Measured, 32 sequences of 8192 keys, 8 kv heads: one token 91 us in bf16 (5.9
 // TB/s, the bytes bound it), 68 us in 8 bits (4.0 TB/s: a tile's chain of barrier
@@ -270,8 +305,9 @@ struct KeysCfg {
   static constexpr int kOffQ = kOffP + 2 * kP;
   static constexpr int kOffCodes = kOffQ + 2 * kQ;
   static constexpr int kOffRed = kOffCodes + kStages * kCodes;  // per stream: [kSums][N] maxima or sums
-  static constexpr int kOffRef = kOffRed + 2 * kSums * N * 4;   // per stream: -m [N], factor [N]
-  static constexpr int kOffPre = kOffRef + 2 * 2 * N * 4;
+  static constexpr int kOffRef = kOffRed + 2 * kSums * N * 4;   // per stream: -m [N], factor [N], 8 bit: -(highest m) [N]
+  static constexpr int kOffLow = kOffRef + 2 * 3 * N * 4;       // 8 bit, per stream: each warp's rows below 1
+  static constexpr int kOffPre = kOffLow + 2 * 8 * 4;
   static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
   static constexpr int kOffBar = kOffSeg + 2 * (int)sizeof(ChunkSeg);
   static constexpr int kAlloc = kOffBar + (4 * kStages + 4 + 10) * 8 + 32 + 1024;
@@ -481,12 +517,15 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
     const uint32_t tl = tmem + ((uint32_t)((wq & 3) * 32) << 16);
     const uint32_t t_s = tl + (C::kSplit ? s * N + rb : (s * (KT / 128) + part) * N), t_o = tl + C::kColO + s * W;
     float* red = (float*)(smem + C::kOffRed) + s * kSums * N;
-    float* nref = (float*)(smem + C::kOffRef) + s * 2 * N;  // -m of a row
+    float* nref = (float*)(smem + C::kOffRef) + s * 3 * N;  // -m of a row
     float* fac = nref + N;
+    float* ntop = fac + N;  // 8 bit: -m where m was highest
+    uint32_t* low = (uint32_t*)(smem + C::kOffLow) + s * 8;
     uint8_t* qs = smem + C::kOffQ + s * C::kQ;
     uint8_t* ps = smem + C::kOffP + s * C::kP;
-    constexpr float kUp = F8 ? 8.75f : 8.0f;   // P at most 2^kUp (448 is the most e4m3 holds)
-    constexpr float kBase = F8 ? 2.0f : 0.0f;  // log2 P of the largest when the reference moves
+    constexpr float kUp = 8.0f;                // P at most 2^kUp (8 bit: 32 times what e4m3 leaves of 256 is 256)
+    constexpr float kBase = F8 ? 3.0f : 0.0f;  // log2 P of the largest when the reference moves
+    constexpr float kDepth = 40.0f;
     for (int sn = 0;; ++sn) {
       const int sb = sn & 1;
       if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
@@ -559,7 +598,10 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
             *(uint2*)(qs + N * 64 + at) = make_uint2(l4[0], l4[1]);
           }
         }
-        if (tid < N) nref[tid] = tid < nrows ? INFINITY : -INFINITY;  // unused rows: P = 0
+        if (tid < N) {
+          nref[tid] = tid < nrows ? INFINITY : -INFINITY;  // unused rows: P = 0
+          ntop[tid] = INFINITY;
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         ch_named_sync(1 + s, kBar);
         if (lane == 0) mbar_arrive(&qfull[s]);
@@ -666,8 +708,31 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
               }
             }
           }
+          const bool check = F8 && (i & 1) && !again;
+          if (check) {
+            // a bit per row, 1: its t is below m (row mine_rows - 1 in bit 0)
+            uint32_t neg = 0;
+#pragma unroll
+            for (int r0 = 0; r0 < NR; r0 += 8) {
+              if (r0 < mine_rows) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  neg = __funnelshift_l((uint32_t)x[r0 / 2 + e], neg, 1);
+                  neg = __funnelshift_l((uint32_t)(x[r0 / 2 + e] >> 32), neg, 1);
+                }
+              }
+            }
+            neg = __reduce_and_sync(0xffffffffu, neg >> (-mine_rows & 7));
+            if (lane == 0) low[wq] = neg;
+          }
+          bool move = ch_named_or(1 + s, kBar, mx > kUp);
+          if (check) {  // (two votes or more lie between one tile's `low` and the next one's)
+            const uint4 a = *(const uint4*)low, b = *(const uint4*)(low + 4);
+            const uint32_t w0 = a.x & a.y & a.z & a.w, w1 = b.x & b.y & b.z & b.w;
+            move |= (C::kSplit ? w0 | w1 : w0 & w1) != 0u;
+          }
           // the second time round nothing is left above the reference's reach
-          if (!ch_named_or(1 + s, kBar, mx > kUp) || again) break;
+          if (!move || again) break;
           const ch_f2 zero[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll 1
           for (int r0 = 0; r0 < mine_rows; r0 += 8) {
@@ -684,7 +749,14 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
             float m = red[tid];
 #pragma unroll
             for (int w = 1; w < kSums; ++w) m = fmaxf(m, red[w * N + tid]);
-            const float m0 = -nref[tid], m1 = m > m0 + kUp ? m - kBase : m0;
+            const float m0 = -nref[tid];
+            float m1 = m > m0 + kUp ? m - kBase : m0;
+            if (F8) {
+              const float top = -ntop[tid];
+              // down, unless nothing in the tile is seen (or the row has seen an infinite score)
+              if (m < m0 && m > -INFINITY && m0 < INFINITY) m1 = fminf(m0, fmaxf(m - kBase, top - kDepth));
+              ntop[tid] = -fmaxf(top, m1);
+            }
             fac[tid] = m1 == m0 ? 1.0f : ch_exp2(m0 - m1);
             nref[tid] = -m1;
           }
@@ -735,11 +807,10 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
             if (!F8) {
               w[e] = ch_bf16x2(ch_lo(pe), ch_hi(pe));
             } else {
-              // hi: 4 significant bits; lo: 16 times the rest
-              const ch_f2 h = ch_pair(ch_round4(ch_lo(pe)), ch_round4(ch_hi(pe)));
-              const ch_f2 d = ch_mul2(ch_fma2(h, ch_pair(-1.f, -1.f), pe), ch_pair(16.f, 16.f));
-              w[e] = ch_e4m3x2(ch_lo(h), ch_hi(h));
-              hl[e] = ch_e4m3x2(ch_lo(d), ch_hi(d));
+              // hi: P in e4m3; lo: 32 times the rest, which 16 bits hold exactly (P to 2^-11 of itself and 2^-25)
+              const uint32_t p16 = ch_f16x2(ch_lo(pe), ch_hi(pe));
+              w[e] = ch_e4m3x2_f16(p16);
+              hl[e] = ch_e4m3x2_f16(ch_hfma2(p16, 0x50005000u, ch_hmul2(ch_f16x2_e4m3(w[e]), 0xD000D000u)));
             }
           }
           const int b = (rb + r0) * (F8 ? 1 : 2);  // byte of the row's place
@@ -803,7 +874,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   os[(r0 + e) * 64 + (wq & 3) * 16 + lane] =
-                      F8 ? fmaf(__uint_as_float(b[e]), 0.0625f, __uint_as_float(a[e])) : __uint_as_float(a[e]);
+                      F8 ? fmaf(__uint_as_float(b[e]), 0.03125f, __uint_as_float(a[e])) : __uint_as_float(a[e]);
               }
             }
           }

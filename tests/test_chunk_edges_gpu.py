@@ -1,0 +1,96 @@
+"""Chunk attention where its number formats end: weights far below a row's
+largest, queries and scores that are not finite, windows beyond every key."""
+import importlib
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from test_chunk_gpu import Case, D, PAGE, dequantise, quantise  # noqa: E402
+
+chunk = importlib.import_module("gpt-oss-tvm_b200.chunk")
+
+
+def one_context(n, q, k, v, f8, hq=64):
+    """A Case of n sequences that share one context, k and v [positions, heads, 64] bf16, q new tokens each."""
+    length, hkv, _ = k.shape
+    c = Case([q] * n, [length] * n, hq=hq, hkv=hkv, sinks=False, ring=1)
+    c.stride = length // PAGE
+    c.table = torch.arange(c.stride, dtype=torch.int32).repeat(n, 1)
+    c.k, c.v = k, v
+    if f8:
+        (c.k, c.ks), (c.v, c.vs) = quantise(k), quantise(v)
+    return c
+
+
+# 8 bits: P is two e4m3 terms in units that a row's largest weight sets to 2^3, and that follow a key tile's largest
+# down when it is below 1.  A term's rounding leaves 2^-8 of P, the 16-bit value that is split 2^-11, and what is too
+# small for a term's normal range 2^-15 of a unit: 2^-18 of the row's largest, for each key of a tile (256 at most) until
+# the units have followed.  bf16: 2^-9 of P.
+SPLIT = 1.02 * (2.0 ** -8 + 2.0 ** -11)
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("v0", [-1.0, -16.0])
+@pytest.mark.parametrize("length", [8192, 32768])
+@pytest.mark.parametrize("q", [1, 4, 6, 8])
+def test_a_dominant_key_before_a_long_tail(q, length, v0, f8):
+    """One key 7 to 16 nats above thousands of equal ones, whose small weights
+    are together as large as its own; 16, 32, 48 and 64 rows a unit."""
+    for nats in (7.0, 8.0, 9.0, 10.0, 12.0, 16.0):
+        k, v = torch.zeros(length, 8, D), torch.ones(length, 8, D)
+        k[0], v[0] = nats / 8.0, v0
+        c = one_context(24, q, k.bfloat16(), v.bfloat16(), f8)
+        c.q = torch.ones_like(c.q)
+        o, _ = c.gpu().run()
+        for i in range(q):
+            tail, top = length - q + i, math.exp(nats)
+            den = top + tail
+            exact = (v0 * top + tail) / den
+            tiles = 2 * 256 * 2.0 ** -18 * (top * abs(v0) + tail / 128) / den
+            tol = SPLIT * (abs(v0) * top + tail) / den + tiles + 2.0 ** -9 * abs(exact) + 2e-6
+            worst = (o[i::q].double() - exact).abs().max().item()
+            assert worst <= tol, f"{nats} nats, token {i}: {worst:.3e} off, {tol:.3e} allowed"
+
+
+@pytest.mark.parametrize("q", [1, 4, 6, 8, 40])
+@pytest.mark.parametrize("low", [6.0, 40.0, 90.0])
+def test_key_tiles_of_very_different_weight(q, low):
+    """Blocks of keys up to `low` nats below the largest, in no order, so that a
+    row's units move up and down: 2^-8 of each key's own weight and 2^-18 of the
+    row's largest (times 2, by which a V row's values may differ from its power
+    of two)."""
+    g = torch.Generator().manual_seed(int(low) + q)
+    length, n = 3200, 24 if q < 40 else 2
+    off = (torch.rand(length // 32, generator=g) * -low).repeat_interleave(32)
+    off[0] = 3.0  # one key on top of all
+    k = torch.randn(length, 8, D, generator=g) * 0.5
+    k[:, :, :8] = off[:, None, None]
+    v = torch.randn(length, 8, D, generator=g) + 1.0
+    c = one_context(n, q, k.bfloat16(), v.bfloat16(), True)
+    c.q = torch.randn(c.q.shape, generator=g).bfloat16()
+    c.q[..., :8] = 1.0
+    c.gpu()
+    o, lse = c.run()
+    kk, vv = dequantise(c.k, c.ks), dequantise(c.v, c.vs)
+    rep = 64 // 8
+    for b in range(0, n, max(1, n // 4)):
+        for i in range(q):
+            m = length - q + i + 1
+            kr, vr = kk[:m].repeat_interleave(rep, 1), vv[:m].repeat_interleave(rep, 1)
+            s = torch.einsum("hd,jhd->hj", c.q[b * q + i].double(), kr) / 8.0
+            p = torch.softmax(s, -1)
+            exact = torch.einsum("hj,jhd->hd", p, vr)
+            av = torch.einsum("hj,jhd->hd", p, vr.abs())
+            top = (p * vr.abs().amax(-1).t()).amax(-1)
+            # Q's terms move a score by 2^-18 of the largest product, below 2^-11 in base e
+            tol = (SPLIT + 2.0 ** -11) * av + (2 * m * 2.0 ** -18) * top[:, None] + 2.0 ** -9 * exact.abs() + 2e-6
+            over = ((o[b * q + i].double() - exact).abs() - tol).max().item()
+            assert over <= 0, f"o is {over:.3e} beyond its tolerance"
+            want = torch.logsumexp(s, -1) / math.log(2.0)
+            assert (lse[b * q + i].double() - want).abs().max().item() <= 5e-4
