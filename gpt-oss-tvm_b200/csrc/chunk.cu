@@ -557,12 +557,15 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
           }
           const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) am = max(am, max((w[e] << 16) & 0x7FFFFFFFu, w[e] & 0x7FFF0000u));
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t a = (w[e] << 16) & 0x7FFFFFFFu, b = w[e] & 0x7FFF0000u;
+            am = max(am, max(a >= 0x7F800000u ? 0u : a, b >= 0x7F800000u ? 0u : b));
+          }
         }
         float up = 1.0f;
         if (F8) {
           // largest magnitude of the unit's finite values into [128, 256)
-          am = __reduce_max_sync(0xffffffffu, am >= 0x7F800000u ? 0u : am);
+          am = __reduce_max_sync(0xffffffffu, am);
           if (lane == 0) fac[wq] = __uint_as_float(am);
           ch_named_sync(1 + s, kBar);
 #pragma unroll

@@ -94,3 +94,21 @@ def test_key_tiles_of_very_different_weight(q, low):
             assert over <= 0, f"o is {over:.3e} beyond its tolerance"
             want = torch.logsumexp(s, -1) / math.log(2.0)
             assert (lse[b * q + i].double() - want).abs().max().item() <= 5e-4
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("q", [1, 4, 5, 6, 8, 40])
+def test_a_query_that_is_not_finite_stays_with_its_row(q, value):
+    """8 bits: the rows of a unit share one scale for their queries, which the
+    finite values alone decide: the other rows keep their bits, also when one of
+    them is the largest by far."""
+    c = Case([q] * 24, [200] * 24, f8=True, seed=q).gpu()
+    big = q * 8 - 1 if q < 5 else 32   # row of the unit: token, head of the group
+    c.q[big // 8, big % 8] *= 2.0 ** 10
+    o, lse = c.run()
+    assert bool(torch.isfinite(o).all())
+    c.q[0, 0, ::2] = value
+    o2, lse2 = c.run()
+    assert bool(torch.isnan(o2[0, 0]).all())
+    o2[0, 0], lse2[0, 0] = o[0, 0], lse[0, 0]
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
