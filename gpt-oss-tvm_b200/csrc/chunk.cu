@@ -526,6 +526,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
     constexpr float kUp = 8.0f;                // P at most 2^kUp (8 bit: 32 times what e4m3 leaves of 256 is 256)
     constexpr float kBase = F8 ? 3.0f : 0.0f;  // log2 P of the largest when the reference moves
     constexpr float kDepth = 40.0f;
+    constexpr float kNoRef = 3.402823466e38f;
     for (int sn = 0;; ++sn) {
       const int sb = sn & 1;
       if (!bad) bad = !mbar_wait(&seg_full[sb], (uint32_t)(sn >> 1) & 1u, p.err, kErrTimeoutFull);
@@ -602,8 +603,10 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
           }
         }
         if (tid < N) {
-          nref[tid] = tid < nrows ? INFINITY : -INFINITY;  // unused rows: P = 0
-          ntop[tid] = INFINITY;
+          // no reference yet: one below every finite score (a score of -infinity, which has to weigh nothing, is NaN
+          // beside an infinite one); unused rows: P = 0
+          nref[tid] = tid < nrows ? kNoRef : -INFINITY;
+          ntop[tid] = kNoRef;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         ch_named_sync(1 + s, kBar);
@@ -756,7 +759,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
             float m1 = m > m0 + kUp ? m - kBase : m0;
             if (F8) {
               const float top = -ntop[tid];
-              // down, unless nothing in the tile is seen (or the row has seen an infinite score)
+              // down, unless nothing in the tile is seen (or the row has seen a score of infinity)
               if (m < m0 && m > -INFINITY && m0 < INFINITY) m1 = fminf(m0, fmaxf(m - kBase, top - kDepth));
               ntop[tid] = -fmaxf(top, m1);
             }

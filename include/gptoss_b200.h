@@ -253,7 +253,8 @@ int gptoss_kv_pages_copy(uint16_t* k_pages, uint16_t* v_pages, int32_t Hkv, int3
  * j > pos_i - W; one that sees nothing (kv_len[b] smaller than its chunk, or a
  * seq_rows[b] outside the table) gives o = 0 and lse = -inf.  What keys and
  * values a token does not see hold does not matter to it, NaN included; one that
- * sees a value that is not finite, or has a score of NaN or +infinity, gets NaN.
+ * sees a value that is not finite, or has a score of NaN or +infinity, gets NaN.  A
+ * score of -infinity weighs nothing; a token with no other gets o = 0, lse = -inf.
  * Pages: bf16, or with kv_f8 e4m3 values and codes as gptoss_qkv_rope_append_f8
  * writes them; num_pages pages in each pool.  max_q: the longest chunk, known
  * to the host (it picks the kernel; a longer chunk is still computed right).

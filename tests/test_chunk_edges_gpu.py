@@ -112,3 +112,51 @@ def test_a_query_that_is_not_finite_stays_with_its_row(q, value):
     assert bool(torch.isnan(o2[0, 0]).all())
     o2[0, 0], lse2[0, 0] = o[0, 0], lse[0, 0]
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("q", [1, 2, 4, 6, 8, 40])
+def test_scores_of_minus_infinity_weigh_nothing(q, n):
+    """Every key of the first tiles scores -infinity: those keys weigh nothing.
+    A row that has no other key gets zeros and an lse of -infinity, whichever
+    kernel runs."""
+    length = 700
+    c = Case([q] * n, [length] * n, seed=q).gpu()
+    j = torch.arange(512, device="cuda")
+    rows = torch.cat([c.table[b].long()[j // PAGE] * PAGE + j % PAGE for b in range(n)])
+    c.k[rows] = 0
+    c.k[rows, :, 9] = -math.inf
+    c.q[..., 9] = c.q[..., 9].abs() + 0.1
+    o, lse = c.run()
+    # the same call without those keys: a window that ends behind them (less for the chunk's later tokens)
+    assert bool(torch.isfinite(o).all()) and bool(torch.isfinite(lse).all())
+    w = Case([q] * n, [length] * n, seed=q).gpu()
+    w.q = c.q
+    exact_k = w.k.clone()
+    exact_k[rows] = 0
+    exact_k[rows, :, 9] = -1000.0 / 0.1  # 1250 nats below: no weight in 64 bits either
+    w.k = exact_k.to(torch.bfloat16)
+    eo, el, tol = w.exact()
+    assert bool(((o.double() - eo).abs() <= tol).all())
+    assert (lse.double() - el).abs().max().item() <= 1e-4
+    c.kv_len.fill_(300)
+    c.kl = [300] * n
+    c.k[...] = 0
+    c.k[..., 9] = -math.inf
+    o, lse = c.run()
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("n", [1, 24])
+@pytest.mark.parametrize("q", [1, 4, 8, 40])
+def test_scores_of_minus_infinity_in_8_bits(q, n):
+    """8-bit keys are finite; queries and keys of 2^60 and more bring their
+    product beyond fp32."""
+    c = Case([q] * n, [300] * n, f8=False, seed=q).gpu()
+    c.k[...] = 0
+    c.k[..., 9] = -(2.0 ** 68)
+    c.q[...] = 0
+    c.q[..., 9] = 2.0 ** 70
+    (c.k, c.ks), (c.v, c.vs) = quantise(c.k), quantise(c.v)
+    o, lse = c.run()
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
