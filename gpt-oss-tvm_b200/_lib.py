@@ -75,6 +75,7 @@ SIGNATURES = {
     "gptoss_attn_merge": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _P, _P, _P]),
     "gptoss_attn_sink_rescale": (ctypes.c_int, [_P, _P, _P, _I64, _I32, _I32, _P]),
     "gptoss_attn_chunk_workspace_bytes": (_I64, []),
+    "gptoss_attn_chunk_workspace_zero_bytes": (_I64, []),
     "gptoss_attn_chunk": (ctypes.c_int, [_P, _I64, _P, _P, _P, _P, _I32, _I64, _P, _I32, _I32, _P, _P, _P, _I32, _I64,
                                          _I32, _I32, _I32, _I32, _I32, _F, _P, _P, _I64, _P, _P, _P]),
     "gptoss_qkv_rope_append_f8": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _F, _P, _P, _P, _P, _P,

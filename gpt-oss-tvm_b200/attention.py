@@ -439,10 +439,13 @@ class DecodeScratch:
         self.buf = None
         self._chunk = None
 
-    def chunk(self) -> "chunk.ChunkWorkspace":
-        """The workspace of attend_chunks (made on its first use, before a
-        step is captured)."""
+    def chunk(self) -> "chunk.ChunkWorkspace | None":
+        """The workspace of attend_chunks, made on its first use; None in a
+        capture that nothing ran before (its calls bring their own)."""
         if self._chunk is None:
+            with torch.cuda.device(self.device):
+                if torch.cuda.is_current_stream_capturing():
+                    return None
             self._chunk = chunk.ChunkWorkspace(self.device)
         return self._chunk
 

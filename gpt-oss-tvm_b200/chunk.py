@@ -26,15 +26,29 @@ HEAD_DIM = 64
 _BF16, _F8, _E8 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
+def _zeroed(device) -> torch.Tensor:
+    """A workspace's memory; what has to be zero before its first use (counters
+    and the error word) is."""
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        buf = torch.empty(int(lib.gptoss_attn_chunk_workspace_bytes()), dtype=torch.uint8, device=device)
+        buf[:int(lib.gptoss_attn_chunk_workspace_zero_bytes())].zero_()
+    return buf
+
+
 class ChunkWorkspace:
     """Device memory of attend_chunks for partial results, zeroed once; used
-    by one stream at a time (one for all layers of a model)."""
+    by one stream at a time (one for all layers of a model).  Made before a
+    capture, not in one: its zeros would be a node of that graph."""
 
     def __init__(self, device="cuda"):
         self.device = torch.device(device)
         with torch.cuda.device(self.device):
-            self.nbytes = int(_lib.load().gptoss_attn_chunk_workspace_bytes())
-        self.buf = torch.zeros(self.nbytes, dtype=torch.uint8, device=self.device)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a ChunkWorkspace is made before a graph is captured (its zeros would be a node of "
+                                   "the graph)")
+        self.buf = _zeroed(self.device)
+        self.nbytes = self.buf.numel()
         self.ptr = self.buf.data_ptr()
 
     def error(self) -> int:
@@ -45,13 +59,25 @@ class ChunkWorkspace:
 _workspaces: dict = {}
 
 
-def _workspace(index: int, stream: int) -> ChunkWorkspace:
-    """The workspace of calls on this device and stream that bring none (a
-    program's own, as long as it runs: captured graphs keep using it)."""
+def _workspace(index: int) -> torch.Tensor:
+    """The workspace of a call on device `index` that brings none: the current
+    stream's, or, while that is being captured, memory of this call alone, zeroed
+    in the graph.  (Streams that capture are shared: a workspace kept by stream
+    would come to graphs that replay side by side, or before the one that holds
+    its zeros.)"""
+    device = torch.device("cuda", index)
+    if torch._C._cuda_getDevice() == index:
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(index):
+            capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        return _zeroed(device)
+    stream = torch._C._cuda_getCurrentRawStream(index)
     ws = _workspaces.get((index, stream))
     if ws is None:
-        ws = _workspaces[index, stream] = ChunkWorkspace(torch.device("cuda", index))
-    return ws
+        ws = _workspaces[index, stream] = ChunkWorkspace(device)
+    return ws.buf
 
 
 def _run(index: int, name: str, *args) -> None:
@@ -130,8 +156,11 @@ def attend_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     q: bf16, heads and values dense, any multiple of 8 elements between tokens
     (a slice of a wider projection will do).  q_start [N + 1], kv_len,
     seq_rows [N]: int32 on the device.  max_q: the longest chunk.  sinks
-    [heads] bf16.  Returns o [T, heads, 64] bf16, with return_lse also lse
-    [T, heads] fp32 (base 2, without the sink)."""
+    [heads] bf16.  workspace: a ChunkWorkspace of calls that run one after
+    another; without one a call has its stream's, or in a captured graph its own
+    (20 MB and a memset a call, so a graph of many calls brings one).  Returns o
+    [T, heads, 64] bf16, with return_lse also lse [T, heads] fp32 (base 2,
+    without the sink)."""
     if not q.is_cuda or q.dtype is not _BF16 or q.dim() != 3 or q.shape[2] != HEAD_DIM:
         _bad(f"q must be a CUDA bfloat16 tensor [tokens, heads, {HEAD_DIM}]")
     index = q.get_device()
@@ -155,16 +184,14 @@ def attend_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         _bad("out must be a dense bfloat16 tensor of q's shape on its device")
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and n:
-        ws = workspace
-        if ws is None:
-            ws = _workspace(index, torch._C._cuda_getCurrentRawStream(index))
-        elif ws.buf.get_device() != index:
+        ws = _workspace(index) if workspace is None else workspace.buf
+        if ws.get_device() != index:
             _bad("the workspace is on another device")
         _run(index, "gptoss_attn_chunk", q.data_ptr(), st[0] if T > 1 else Hq * HEAD_DIM, k_pages.data_ptr(),
              v_pages.data_ptr(), k_scale.data_ptr() if f8 else None, v_scale.data_ptr() if f8 else None, f8, pages,
              table_p, page_table.shape[0], page_table.shape[1], rows_p, start_p, len_p, n, T, max_q, Hq, hkv,
              HEAD_DIM, window, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
-             sinks.data_ptr() if sinks is not None else None, ws.ptr, ws.nbytes, out.data_ptr(),
+             sinks.data_ptr() if sinks is not None else None, ws.data_ptr(), ws.numel(), out.data_ptr(),
              lse.data_ptr() if return_lse else None)
     return (out, lse) if return_lse else out
 

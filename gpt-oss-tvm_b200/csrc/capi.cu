@@ -529,6 +529,7 @@ int gptoss_attn_sink_rescale(uint16_t* o, const float* lse, const uint16_t* sink
 
 // ------------------------------------------- chunks over the paged cache --
 int64_t gptoss_attn_chunk_workspace_bytes(void) { return chunk_workspace_bytes(); }
+int64_t gptoss_attn_chunk_workspace_zero_bytes(void) { return chunk_parts_at(); }
 
 int gptoss_attn_chunk(const uint16_t* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                       const uint8_t* k_codes, const uint8_t* v_codes, int32_t kv_f8, int64_t num_pages,

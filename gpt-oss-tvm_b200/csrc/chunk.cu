@@ -1659,9 +1659,10 @@ int launch_rows(const void* k, const void* v, ChunkParams p, cudaStream_t s) {
 
 }  // namespace
 
-// Workspace: 256 bytes (word 0: the error flags), a counter per CTA, then two
-// partial results per CTA (rows of 64 values, a maximum and a sum).
-static int64_t chunk_parts_at() { return 256 + ((int64_t)device_sm_count() * 4 + 255) / 256 * 256; }
+// Workspace: 256 bytes (word 0: the error flags), a counter per CTA (so far it has
+// to be zero before its first use), then two partial results per CTA (rows of 64
+// values, a maximum and a sum).
+int64_t chunk_parts_at() { return 256 + ((int64_t)device_sm_count() * 4 + 255) / 256 * 256; }
 int64_t chunk_workspace_bytes() {
   return chunk_parts_at() + (int64_t)device_sm_count() * 2 * kChunkSlotRows * (kChunkD + 2) * 4;
 }

@@ -165,6 +165,7 @@ int launch_sink_rescale(uint16_t* o, const float* lse, const uint16_t* sinks, in
 // chunk.cu: attention of the sequences' new tokens over the paged cache
 struct ChunkParams;
 int64_t chunk_workspace_bytes();
+int64_t chunk_parts_at();  // what lies before has to be zero at first
 int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, int32_t max_q, void* workspace,
                       cudaStream_t s);
 // kv8.cu: the 8-bit cache

@@ -262,10 +262,12 @@ int gptoss_kv_pages_copy(uint16_t* k_pages, uint16_t* v_pages, int32_t Hkv, int3
  * before the one rounding of o [T, Hq, D].  lse [T, Hq] fp32 or NULL, as above.
  * q_start, kv_len, seq_rows: device memory, so a CUDA graph may replay the call
  * with other lengths.  workspace: gptoss_attn_chunk_workspace_bytes() bytes of
- * device memory, zeroed once before its first use and used by one stream at a
- * time; word 0 collects device errors (a bounded wait that ran out: zero the
- * workspace again after one). */
+ * device memory, the first gptoss_attn_chunk_workspace_zero_bytes() of them zeroed
+ * once before its first use, used by one stream at a time (graphs that replay side
+ * by side have one each); word 0 collects device errors (a bounded wait that ran
+ * out: zero them again after one). */
 int64_t gptoss_attn_chunk_workspace_bytes(void);
+int64_t gptoss_attn_chunk_workspace_zero_bytes(void);
 int gptoss_attn_chunk(const uint16_t* q, int64_t q_stride, const void* k_pages, const void* v_pages,
                       const uint8_t* k_codes, const uint8_t* v_codes, int32_t kv_f8, int64_t num_pages,
                       const int32_t* page_table, int32_t table_rows, int32_t table_stride, const int32_t* seq_rows,

@@ -160,3 +160,62 @@ def test_scores_of_minus_infinity_in_8_bits(q, n):
     (c.k, c.ks), (c.v, c.vs) = quantise(c.k), quantise(c.v)
     o, lse = c.run()
     assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+
+
+def captured(c, out):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        chunk.attend_chunks(c.q, c.k, c.v, c.table, c.rows, c.q_start, c.kv_len, max_q=max(c.ql), sinks=c.sinks,
+                            k_scale=c.ks, v_scale=c.vs, out=out)
+    return g
+
+
+@pytest.mark.parametrize("f8", [False, True])
+def test_captured_calls_without_a_workspace_are_their_own(f8):
+    """Each captured call brings its memory and its zeros: graphs replay in any
+    order, at the same time on two streams, and leave nothing to later calls."""
+    known = set(chunk._workspaces)
+    a, b = Case([4, 1], [5000, 30], f8=f8, seed=1).gpu(), Case([300], [5200], f8=f8, seed=2).gpu()
+    for x in (a, b):
+        x.run()
+    torch.cuda.synchronize()
+    eager = set(chunk._workspaces)
+    oa, ob = torch.empty_like(a.q), torch.empty_like(b.q)
+    ga, gb = captured(a, oa), captured(b, ob)
+    # whatever the memory of a workspace held that a capture left behind
+    for key in set(chunk._workspaces) - eager - known:
+        chunk._workspaces[key].buf.fill_(0xFF)
+    wa, wb = a.run()[0], b.run()[0]
+    s = [torch.cuda.Stream() for _ in range(2)]
+    for rep in range(20):
+        oa.fill_(math.nan)
+        ob.fill_(math.nan)
+        torch.cuda.synchronize()
+        for g, st in ((gb, s[1]), (ga, s[0]))[::1 if rep % 2 else -1]:
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ob, wb) and torch.equal(oa, wa), f"replay {rep}"
+    assert set(chunk._workspaces) == eager | known
+
+
+def test_a_workspace_is_not_made_under_capture():
+    """Its zeros would be a node of that graph, run only when that graph is."""
+    t = torch.zeros(4, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="captur"):
+            chunk.ChunkWorkspace("cuda")
+        t.add_(1)
+    g.replay()
+    assert float(t[0]) == 1.0
+
+
+def test_a_model_s_scratch_has_no_workspace_of_a_capture():
+    att = importlib.import_module("gpt-oss-tvm_b200.attention")
+    scratch, t, g = att.DecodeScratch("cuda"), torch.zeros(4, device="cuda"), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t.add_(1)
+        assert scratch.chunk() is None
+    ws = scratch.chunk()
+    assert isinstance(ws, chunk.ChunkWorkspace) and ws.error() == 0 and scratch.chunk() is ws
