@@ -11,6 +11,13 @@ from . import _lib
 from .chunk import _bad, _i32, _run
 
 
+def _dense_rows(t: torch.Tensor) -> bool:
+    """Whether the values of each row of t are one after another (what is a
+    stride of one entry does not matter)."""
+    rows, n = t.shape
+    return rows == 0 or ((n <= 1 or t.stride(1) == 1) and (rows == 1 or t.stride(0) >= n))
+
+
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.Tensor,
                   accept_draws: torch.Tensor | None = None, next_draws: torch.Tensor | None = None, *,
                   temperature: float = 1.0, draft_probs: torch.Tensor | None = None):
@@ -27,7 +34,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.T
         _bad("logits must be a CUDA tensor [rows, vocabulary], float32 or bfloat16")
     index = logits.get_device()
     T, V = logits.shape
-    if T > 1 and (logits.stride(1) != 1 or logits.stride(0) < V):
+    if not _dense_rows(logits):
         _bad("the values of a row of logits must be dense")
     n = row_start.shape[0] - 1
     if n < 0:
@@ -40,8 +47,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.T
                     or t.get_device() != index):
                 _bad(f"{name} must be a dense float32 tensor of {m} entries on cuda:{index}")
     if draft_probs is not None and (draft_probs.dtype is not torch.float32 or draft_probs.shape != (T, V)
-                                    or draft_probs.get_device() != index
-                                    or (T > 1 and (draft_probs.stride(1) != 1 or draft_probs.stride(0) < V))):
+                                    or draft_probs.get_device() != index or not _dense_rows(draft_probs)):
         _bad(f"draft_probs must be a float32 tensor [{T}, {V}] with dense rows on cuda:{index}")
     # one allocation: the two answers, then the library's scratch
     nbytes = _lib.load().gptoss_verify_drafts_scratch_bytes(T, V)

@@ -151,3 +151,11 @@ def test_c_entries_check_before_they_launch():
                     acc=p, nxt=p, stream=None), **kw}
         r, msg = rc("gptoss_verify_drafts", *a.values())
         assert r < 0 and text in msg, (kw, r, msg)
+
+
+def test_rows_of_dense_values():
+    z = torch.zeros(4, 10)
+    dense = verify._dense_rows
+    assert dense(z) and dense(z[:, :7]) and dense(z[:1]) and dense(z[:0]) and dense(z[:, 3:4]) and dense(z[1:2, 3:4])
+    assert not dense(z[:, ::2]) and not dense(z.t()) and not dense(z[:1].expand(4, 10))
+    assert not dense(z[:1, ::2]) and not dense(z[:, 2:3].t()) and not dense(z[:1, :1].expand(1, 10))

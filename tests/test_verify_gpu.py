@@ -199,3 +199,25 @@ def test_refusals():
     ]:
         with pytest.raises(bad, match=match):
             verify.verify_drafts(*a, **kw)
+
+
+def test_one_row_has_dense_values_too():
+    """Every second value of a row, or a column as a row, is refused for a single
+    row as for many: the kernel reads values one after another."""
+    z, tok, start, ua, un, q = make([1], 64, 2, True)
+    wide, tall = torch.randn(1, 128, device="cuda"), torch.randn(64, 3, device="cuda").softmax(0)
+    ok = verify.verify_drafts(z, tok, start, ua, un, draft_probs=q)
+    assert ok[0].tolist() == [0]
+    for view in (wide[:, ::2], tall[:, 1:2].t(), wide[:, :1].expand(1, 64)):
+        with pytest.raises(ValueError, match="must be dense"):
+            verify.verify_drafts(view, tok, start, ua, un)
+        with pytest.raises(ValueError, match="draft_probs"):
+            verify.verify_drafts(z, tok, start, ua, un, draft_probs=view)
+    # what no stride of one entry says: a dense row, however it came about
+    row = wide[:, :64].as_strided((1, 64), (7, 1))
+    a, b = verify.verify_drafts(row, tok, start, ua, un), verify.verify_drafts(row.contiguous(), tok, start, ua, un)
+    assert torch.equal(a[1], b[1])
+    one = torch.zeros(2, 5, device="cuda")[:, 2:3]   # a vocabulary of one
+    t2 = torch.zeros(2, dtype=torch.int32, device="cuda")
+    a = verify.verify_drafts(one, t2, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), temperature=0.0)
+    assert a[0].tolist() == [1] and a[1].tolist() == [0]
