@@ -51,9 +51,17 @@ class ChunkWorkspace:
         self.nbytes = self.buf.numel()
         self.ptr = self.buf.data_ptr()
 
+    def error_word(self) -> torch.Tensor:
+        """Device error bits so far, int32 [1] on the device."""
+        return self.buf[:4].view(torch.int32)
+
     def error(self) -> int:
         """Device error bits so far (synchronises)."""
-        return int(self.buf[:4].view(torch.int32).item())
+        return int(self.error_word().item())
+
+    def reset(self) -> None:
+        """After a device error: the counters may be anything, and the error bits stay otherwise."""
+        self.buf.zero_()
 
 
 _workspaces: dict = {}

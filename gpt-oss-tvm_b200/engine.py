@@ -184,6 +184,11 @@ class Engine:
         self.paged_kv_cache.end_forward()
         return logits[0], ids.to(torch.int32), self.paged_kv_cache.q_start
 
+    def chunk_workspace(self):
+        """The attention workspace of ``extend_batch`` and of decode on an 8-bit
+        cache: its ``error_word`` tells of device waits that ran out."""
+        return self.model.model.block[0].attn.scratch.chunk()
+
     def verify(self, logits: torch.Tensor, ids: torch.Tensor, row_start: torch.Tensor,
                accept_draws: torch.Tensor | None = None, next_draws: torch.Tensor | None = None, *,
                temperature: float = 0.0, draft_probs: torch.Tensor | None = None):

@@ -54,15 +54,23 @@ class SpeculativeDecoder:
     def step(self, texts: dict[int, list[int]], room: dict[int, int]) -> None:
         """One forward for the sequences of ``texts`` (sequence id -> tokens,
         whose last is not in the cache yet); appends what it yields, at most
-        room[id] tokens."""
+        room[id] tokens.  Raises RuntimeError when the device reports a wait that
+        ran out, with texts and cache as they were before the step."""
         eng, seqs = self.engine, list(texts)
         chunks = [[texts[s][-1]] + list(self.draft(texts[s], min(self.draft_len, room[s] - 1))) for s in seqs]
         logits, ids, row_start = eng.extend_batch(chunks, seqs)
         greedy = self.temperature < 1e-6
         accepted, nxt = eng.verify(logits, ids, row_start, None if greedy else self._draws(ids.numel()),
                                    None if greedy else self._draws(len(seqs)), temperature=self.temperature)
-        got = torch.stack([accepted, nxt]).tolist()
-        for s, c, a, t in zip(seqs, chunks, *got):
+        n, workspace = len(seqs), eng.chunk_workspace()
+        got = torch.cat([accepted, nxt, workspace.error_word()]).tolist()
+        if got[-1] or min(got[n:2 * n]) < 0:
+            workspace.reset()
+            for s, c in zip(seqs, chunks):
+                eng.popn(s, len(c))
+            raise RuntimeError(f"a speculative step failed on the device (attention error bits {got[-1]:#x}, next "
+                               f"tokens {got[n:2 * n]})")
+        for s, c, a, t in zip(seqs, chunks, got[:n], got[n:2 * n]):
             texts[s] += c[1:1 + a] + [t]
             if len(c) - 1 > a:
                 eng.popn(s, len(c) - 1 - a)

@@ -159,3 +159,61 @@ def test_rows_of_dense_values():
     assert dense(z) and dense(z[:, :7]) and dense(z[:1]) and dense(z[:0]) and dense(z[:, 3:4]) and dense(z[1:2, 3:4])
     assert not dense(z[:, ::2]) and not dense(z.t()) and not dense(z[:1].expand(4, 10))
     assert not dense(z[:1, ::2]) and not dense(z[:, 2:3].t()) and not dense(z[:1, :1].expand(1, 10))
+
+
+class HostEngine:
+    """An engine without a model: its target always continues with token + 1."""
+
+    def __init__(self, **kw):
+        self.device, self.max_chunk, self.max_batch_size = torch.device("cpu"), 4, 2
+        self.paged_kv_cache = cache(max_chunk=4)
+        self.popn, self.clear_kv_cache = self.paged_kv_cache.popn, self.paged_kv_cache.clear
+        self.answer, self.error, self.resets = None, 0, 0
+
+    def prefill(self, tokens, s):
+        self.paged_kv_cache.begin_forward([s], [len(tokens)])
+
+    def extend_batch(self, chunks, seqs):
+        self.paged_kv_cache.begin_chunks(seqs, [len(c) for c in chunks])
+        return None, torch.tensor([t for c in chunks for t in c], dtype=torch.int32), self.paged_kv_cache.q_start
+
+    def verify(self, logits, ids, start, *draws, temperature):
+        acc, nxt = [], []
+        for a, b in zip(start.tolist(), start.tolist()[1:]):
+            seq, k = ids[a:b].tolist(), 0
+            while k + 1 < len(seq) and seq[k + 1] == seq[k] + 1:
+                k += 1
+            acc.append(k)
+            nxt.append(seq[k] + 1)
+        i32 = dict(dtype=torch.int32)
+        return torch.tensor(acc, **i32), torch.tensor(self.answer or nxt, **i32)
+
+    def chunk_workspace(self):
+        return self
+
+    def error_word(self):
+        return torch.tensor([self.error], dtype=torch.int32)
+
+    def reset(self):
+        self.error, self.resets = 0, self.resets + 1
+
+
+def test_a_speculative_step_that_fails_on_the_device_raises():
+    """A next token of -1 or an error of the attention: the step raises, and texts
+    and cache are as before, so that it can be taken again."""
+    eng = HostEngine()
+    dec = spec.SpeculativeDecoder(eng, draft_len=3, draft=lambda t, n: [t[-1] + 1, t[-1] + 2, 0][:n])
+    assert dec.generate([[5, 6], [9]], 7) == [list(range(7, 14)), list(range(10, 17))]
+    texts = {0: [1, 2, 3], 1: [7]}
+    eng.clear_kv_cache()
+    eng.prefill([1, 2], 0)
+    for answer, error in (([4, -1], 0), (None, 1 << 9)):
+        eng.answer, eng.error = answer, error
+        with pytest.raises(RuntimeError, match="on the device"):
+            dec.step(texts, {0: 9, 1: 9})
+        assert texts == {0: [1, 2, 3], 1: [7]} and eng.paged_kv_cache.lengths.tolist() == [2, 0]
+    eng.answer, drafted = None, dec.drafted
+    assert eng.resets == 2
+    dec.step(texts, {0: 9, 1: 9})
+    assert texts == {0: [1, 2, 3, 4, 5, 6], 1: [7, 8, 9, 10]} and dec.drafted == drafted + 6
+    assert eng.paged_kv_cache.lengths.tolist() == [5, 3]
