@@ -178,7 +178,12 @@ class Engine:
         lens = [len(t) for t in input_tokens]
         if lens and max(lens) > self.max_chunk:
             raise ValueError(f"extend_batch takes up to max_chunk = {self.max_chunk} tokens of a sequence")
-        ids = self._ids([int(t) for seq in input_tokens for t in seq])
+        tokens = [int(t) for seq in input_tokens for t in seq]
+        vocab = self.config.vocab_size
+        if tokens and not 0 <= min(tokens) <= max(tokens) < vocab:
+            raise ValueError(f"extend_batch: tokens {min(tokens)} to {max(tokens)} are not all in the vocabulary (0 to "
+                             f"{vocab - 1})")
+        ids = self._ids(tokens)
         self.paged_kv_cache.begin_chunks(sequence_ids, lens)
         logits, self.paged_kv_cache = self.model.chunk(self.model.embed(ids), self.paged_kv_cache)
         self.paged_kv_cache.end_forward()

@@ -57,7 +57,13 @@ class SpeculativeDecoder:
         room[id] tokens.  Raises RuntimeError when the device reports a wait that
         ran out, with texts and cache as they were before the step."""
         eng, seqs = self.engine, list(texts)
-        chunks = [[texts[s][-1]] + list(self.draft(texts[s], min(self.draft_len, room[s] - 1))) for s in seqs]
+        chunks = []
+        for s in seqs:
+            most = min(self.draft_len, room[s] - 1)
+            drafts = list(self.draft(texts[s], most))
+            if len(drafts) > max(most, 0):
+                raise ValueError(f"{len(drafts)} drafts where at most {most} were asked for")
+            chunks.append([texts[s][-1]] + drafts)
         logits, ids, row_start = eng.extend_batch(chunks, seqs)
         greedy = self.temperature < 1e-6
         accepted, nxt = eng.verify(logits, ids, row_start, None if greedy else self._draws(ids.numel()),

@@ -217,3 +217,23 @@ def test_a_speculative_step_that_fails_on_the_device_raises():
     dec.step(texts, {0: 9, 1: 9})
     assert texts == {0: [1, 2, 3, 4, 5, 6], 1: [7, 8, 9, 10]} and dec.drafted == drafted + 6
     assert eng.paged_kv_cache.lengths.tolist() == [5, 3]
+
+
+def test_tokens_outside_the_vocabulary_never_reach_the_embedding():
+    """Nor do drafts beyond what was asked for lengthen a text."""
+    import types
+    engm = importlib.import_module("gpt-oss-tvm_b200.engine")
+    c = cache(max_chunk=4)
+    planned = []
+    stub = types.SimpleNamespace(max_chunk=4, config=c.config, paged_kv_cache=c, _ids=planned.append)
+    for bad in ([[64]], [[1, 2], [-1]], [[3, 1 << 40]]):
+        with pytest.raises(ValueError, match="vocabulary"):
+            engm.Engine.extend_batch(stub, bad, list(range(len(bad))))
+    assert planned == [] and c.lengths.tolist() == [0, 0]
+    eng = HostEngine()
+    eng.prefill([1, 2], 0)
+    texts = {0: [1, 2, 3]}
+    for room in (9, 2, 1):
+        with pytest.raises(ValueError, match="drafts where at most"):
+            spec.SpeculativeDecoder(eng, draft_len=3, draft=lambda t, n: [4] * (n + 1)).step(texts, {0: room})
+    assert texts == {0: [1, 2, 3]} and eng.paged_kv_cache.lengths.tolist() == [2, 0]

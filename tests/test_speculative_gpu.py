@@ -194,3 +194,16 @@ def test_refusals():
     with pytest.raises(ValueError, match="kv_dtype"):
         engine("int8")
     eng.model.release()
+
+
+def test_tokens_outside_the_vocabulary_are_refused():
+    eng = engine("bfloat16", batch=2, chunk=4)
+    for bad in ([[512]], [[1], [-1]], [[1, 2, 1 << 20]]):
+        with pytest.raises(ValueError, match="vocabulary"):
+            eng.extend_batch(bad, list(range(len(bad))))
+    with pytest.raises(ValueError, match="vocabulary"):
+        spec.SpeculativeDecoder(eng, draft_len=3, draft=lambda t, n: [512][:n]).generate([[1]], 4)
+    eng.clear_kv_cache()
+    logits = eng.extend_batch([[0, 511]], [0])[0]
+    assert bool(torch.isfinite(logits).all())
+    eng.model.release()
