@@ -210,6 +210,7 @@ class KVCache:
             self._written[s] = max(self._written[s], start + n)
         self.lengths.copy_(new_len)
         self._cur = (list(seq_ids), list(append_lengths))
+        self.q_start = self.seq_rows = None  # another plan's chunks, see begin_chunks
         self.start = starts[0] if len(starts) == 1 else 0
         cat = lambda xs: torch.cat(xs) if xs else torch.zeros(0, dtype=torch.int32)  # noqa: E731
         pos, slots, slots_w = cat(pos), cat(slots), cat(slots_w)
@@ -274,6 +275,7 @@ class KVCache:
         from the page tables, length += 1.  The host mirror is advanced by
         ``commit_decode`` after the step has been issued."""
         self._cur = (list(range(batch)), [1] * batch)
+        self.q_start = self.seq_rows = None
         pos, slot, slot_w, kvl = (self._dec_pos[:batch], self._dec_slot[:batch], self._dec_slot_win[:batch],
                                   self._kv_len[:batch])
         pos.copy_(self.dev_lengths[:batch])

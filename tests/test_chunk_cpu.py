@@ -237,3 +237,17 @@ def test_tokens_outside_the_vocabulary_never_reach_the_embedding():
         with pytest.raises(ValueError, match="drafts where at most"):
             spec.SpeculativeDecoder(eng, draft_len=3, draft=lambda t, n: [4] * (n + 1)).step(texts, {0: room})
     assert texts == {0: [1, 2, 3]} and eng.paged_kv_cache.lengths.tolist() == [2, 0]
+
+
+def test_another_plan_ends_that_of_the_chunks():
+    """forward_to="chunk" after begin_forward or a device-planned decode step has
+    no chunks to attend, whatever an earlier begin_chunks left."""
+    c = cache(max_chunk=4)
+    for other in (lambda: c.begin_forward([0], [3]), lambda: c.begin_forward([1, 0], [1, 2]),
+                  lambda: c.begin_decode_on_device(2)):
+        c.begin_chunks([0, 1], [2, 1])
+        assert c.q_start.tolist() == [0, 2, 3]
+        other()
+        assert c.q_start is None and c.seq_rows is None
+    c.begin_chunks([1], [1])
+    assert c.q_start.tolist() == [0, 1] and c.seq_rows.tolist() == [1]

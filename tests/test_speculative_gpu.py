@@ -207,3 +207,13 @@ def test_tokens_outside_the_vocabulary_are_refused():
     logits = eng.extend_batch([[0, 511]], [0])[0]
     assert bool(torch.isfinite(logits).all())
     eng.model.release()
+
+
+def test_a_chunk_forward_needs_its_own_plan():
+    eng = engine("bfloat16", batch=2, chunk=4)
+    eng.extend_batch([[1, 2], [3]], [0, 1])
+    x = eng.model.embed(torch.tensor([4, 5, 6], device="cuda"))
+    eng.paged_kv_cache.begin_forward([0], [3])
+    with pytest.raises(ValueError, match="begin_chunks"):
+        eng.model.chunk(x, eng.paged_kv_cache)
+    eng.model.release()
