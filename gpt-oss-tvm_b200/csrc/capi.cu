@@ -573,7 +573,8 @@ int gptoss_attn_chunk(const uint16_t* q, int64_t q_stride, const void* k_pages, 
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = Hq / Hkv;
-  p.window = window > 0 ? window : 0;
+  // A window longer than a table row reaches hides nothing.  (The kernels add chunk positions to the others in 32 bits.)
+  p.window = window <= 0 || window > (int64_t)table_stride * 16 ? 0 : window < 0x7FFF0000 ? window : 0x7FFF0000;
   p.T = T;
   p.scale2 = sm_scale * 1.4426950408889634f;
   p.sinks = sinks;

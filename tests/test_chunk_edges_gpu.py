@@ -219,3 +219,15 @@ def test_a_model_s_scratch_has_no_workspace_of_a_capture():
         assert scratch.chunk() is None
     ws = scratch.chunk()
     assert isinstance(ws, chunk.ChunkWorkspace) and ws.error() == 0 and scratch.chunk() is ws
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 128, 2 ** 30, 4097])
+@pytest.mark.parametrize("ql,kl", [([1], [300]), ([5], [260]), ([6] * 24, [130 + b for b in range(24)]),
+                                   ([6] * 3, [130, 200, 300]), ([4] * 5, [4, 130, 129, 300, 255]),
+                                   ([40, 3], [290, 290]), ([400] * 3, [401, 700, 400])])
+def test_a_window_beyond_every_key_is_none(ql, kl, window, f8):
+    c = Case(ql, kl, f8=f8, seed=len(ql), window=0).gpu()
+    o, lse = c.run()
+    o2, lse2 = c.run(window=window)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
