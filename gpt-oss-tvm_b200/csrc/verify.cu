@@ -588,7 +588,8 @@ int launch_verify(const void* logits, int32_t bf16, int64_t ld, const int32_t* t
   p.V = V;
   p.pieces = (int32_t)ver_pieces(V);
   p.greedy = temperature < 1e-6;
-  p.inv_temp = p.greedy ? 1.0f : (float)(1.0 / temperature);
+  // 2^-126 at least: a zero would make a logit of -infinity no number (every finite one weighs 1 there, as it should)
+  p.inv_temp = p.greedy ? 1.0f : fmaxf((float)(1.0 / temperature), 1.17549435e-38f);
   p.accept_u = accept_u;
   p.next_u = next_u;
   p.draft = p.greedy ? nullptr : draft;

@@ -221,3 +221,18 @@ def test_one_row_has_dense_values_too():
     t2 = torch.zeros(2, dtype=torch.int32, device="cuda")
     a = verify.verify_drafts(one, t2, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), temperature=0.0)
     assert a[0].tolist() == [1] and a[1].tolist() == [0]
+
+
+@pytest.mark.parametrize("temperature", [1e30, 1e46, 1e300])
+def test_a_temperature_that_levels_everything(temperature):
+    """Weights of 1 for every finite logit, none for -infinity."""
+    V = 600
+    z = torch.randn(3, V, generator=torch.Generator().manual_seed(1)).cuda()
+    z[:, ::2] = -math.inf
+    tok = torch.tensor([0, 7, 4], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    u = torch.tensor([0.002, 0.002, 0.5], device="cuda")  # p is 1/300
+    for un in (0.0, 0.25, 0.9999):
+        # token 7 stands (0.002 < 1/300), token 4 has no weight; the next is one of the odd ones, each as likely
+        a, t = verify.verify_drafts(z, tok, start, u, torch.tensor([un], device="cuda"), temperature=temperature)
+        assert (int(a[0]), int(t[0])) == (1, 2 * int(un * 300) + 1)
