@@ -236,3 +236,20 @@ def test_a_temperature_that_levels_everything(temperature):
         # token 7 stands (0.002 < 1/300), token 4 has no weight; the next is one of the odd ones, each as likely
         a, t = verify.verify_drafts(z, tok, start, u, torch.tensor([un], device="cuda"), temperature=temperature)
         assert (int(a[0]), int(t[0])) == (1, 2 * int(un * 300) + 1)
+
+
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("V,dtype", [(500003, torch.float32), (1 << 20, torch.bfloat16), (1 << 22, torch.float32)])
+def test_vocabularies_beyond_what_stays_on_chip(V, dtype, probs):
+    """A row's part of a CTA no longer fits shared memory: the logits are read
+    twice.  (Weights in steps of 2^-40 of the largest over 2^22 values: 4e-6.)"""
+    z, tok, start, ua, un, q = make([2, 3], V, 7, probs, dtype)
+    check(z, tok, start, ua, un, q, 0.9)
+    tok[3] = 3
+    z[2, 7] = 50.0
+    z[0, V - 3], z[0, 5], z[3, V - 1] = 50.0, 50.0, 50.0   # greedy: the lowest index of a tie, the last value of a row
+    tok[1], tok[4] = 5, 0
+    acc, nxt = verify.verify_drafts(z, tok, start, temperature=0.0)
+    first = [int((row == row.max()).nonzero()[0, 0]) for row in z]
+    assert first[0] == 5 and first[3] == V - 1 and first[2] != int(tok[3])
+    assert acc.tolist() == [1, 0] and nxt.tolist() == [first[1], first[2]]
