@@ -263,20 +263,22 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 // e4m3 too, as two terms.  Q is scaled by a power of two per unit and head; hi =
 // Q to 4 significant bits and lo = the rest are two products into the same
 // columns (2^-18 of the largest).  P's terms have columns of their own, W = 2 N:
-// hi = P in e4m3, lo = 32 times what that leaves, 2^-8 of P in all.  The key's
+// hi = P in e4m3, lo = 28 times what that leaves, 2^-8 of P in all.  The key's
 // power of two meets the score in fp32; the value's goes into the exponent, t = s
 // + e_v, and the softmax reference follows t:  P = 2^(t - m), l = sum P 2^-e_v.
 //
-// The reference m of a row moves up when a score exceeds it by 8, which one
-// barrier of the stream's warps tells; then O^T in TMEM is rescaled.  In 8 bits
-// it moves down, too, when no P of the row reaches 1 in a tile: the two terms end
-// at 2^-15, and thousands of keys that each fall below it may weigh as much as the
-// largest.  Each second tile is looked at (24 more instructions a thread), which
-// bounds what is lost: of the row's largest so far, which is 2^3 or more in units
-// of 2^m, 2^-18 a key; and of the 128 or 256 keys of a tile 2^-7 at most of the
+// The reference m of a row moves up when a score exceeds it by 8 (8 bit: 8.75, P
+// up to 430), which one barrier of the stream's warps tells; then O^T in TMEM is
+// rescaled.  In 8 bits it moves down, too, when no P of the row reaches 1 in a
+// tile: the two terms end at 2^-14.8, and thousands of keys that each fall below it
+// may weigh as much as the largest.  Each second tile is looked at, which bounds
+// what is lost: 2^-18 a key of the row's largest so far, which is 2^3.5 or more in
+// units of 2^m; and by the 128 or 256 keys of a tile together 2^-6.8 at most of the
 // tile before, whose largest P is 1 or more.  kDepth bounds the way down from the
 // row's highest reference, since O^T and l are multiplied on the way: keys that
-// far below it weigh nothing beside the one that set it.
+// far below it weigh nothing beside the one that set it.  (32 sequences of 1 to 5
+// tokens on up to 8191 keys: 109 us without the way down, 114 with it, 120 where
+// every tile is looked at; units that begin at 2^3: 117, at 2^5: 120.)
 //
 // Measured, 32 sequences of 8192 keys, 8 kv heads: one token 91 us in bf16 (5.9
 // TB/s, the bytes bound it), 68 us in 8 bits (4.0 TB/s: a tile's chain of barrier
@@ -523,8 +525,8 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
     uint32_t* low = (uint32_t*)(smem + C::kOffLow) + s * 8;
     uint8_t* qs = smem + C::kOffQ + s * C::kQ;
     uint8_t* ps = smem + C::kOffP + s * C::kP;
-    constexpr float kUp = 8.0f;                // P at most 2^kUp (8 bit: 32 times what e4m3 leaves of 256 is 256)
-    constexpr float kBase = F8 ? 3.0f : 0.0f;  // log2 P of the largest when the reference moves
+    constexpr float kUp = F8 ? 8.75f : 8.0f;                // P at most 2^kUp (8 bit: 28 times what e4m3 leaves of 448 is 448)
+    constexpr float kBase = F8 ? 3.5f : 0.0f;  // log2 P of the largest when the reference moves
     constexpr float kDepth = 40.0f;
     constexpr float kNoRef = 3.402823466e38f;
     for (int sn = 0;; ++sn) {
@@ -813,10 +815,10 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
             if (!F8) {
               w[e] = ch_bf16x2(ch_lo(pe), ch_hi(pe));
             } else {
-              // hi: P in e4m3; lo: 32 times the rest, which 16 bits hold exactly (P to 2^-11 of itself and 2^-25)
+              // hi: P in e4m3; lo: 28 times the rest, which 16 bits hold exactly (P to 2^-11 of itself and 2^-25)
               const uint32_t p16 = ch_f16x2(ch_lo(pe), ch_hi(pe));
               w[e] = ch_e4m3x2_f16(p16);
-              hl[e] = ch_e4m3x2_f16(ch_hfma2(p16, 0x50005000u, ch_hmul2(ch_f16x2_e4m3(w[e]), 0xD000D000u)));
+              hl[e] = ch_e4m3x2_f16(ch_hfma2(p16, 0x4F004F00u, ch_hmul2(ch_f16x2_e4m3(w[e]), 0xCF00CF00u)));
             }
           }
           const int b = (rb + r0) * (F8 ? 1 : 2);  // byte of the row's place
@@ -880,7 +882,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                   os[(r0 + e) * 64 + (wq & 3) * 16 + lane] =
-                      F8 ? fmaf(__uint_as_float(b[e]), 0.03125f, __uint_as_float(a[e])) : __uint_as_float(a[e]);
+                      F8 ? fmaf(__uint_as_float(b[e]), 0.0357142857f, __uint_as_float(a[e])) : __uint_as_float(a[e]);
               }
             }
           }

@@ -28,9 +28,9 @@ def one_context(n, q, k, v, f8, hq=64):
     return c
 
 
-# 8 bits: P is two e4m3 terms in units that a row's largest weight sets to 2^3, and that follow a key tile's largest
+# 8 bits: P is two e4m3 terms in units that a row's largest weight sets to 2^3.5, and that follow a key tile's largest
 # down when it is below 1.  A term's rounding leaves 2^-8 of P, the 16-bit value that is split 2^-11, and what is too
-# small for a term's normal range 2^-15 of a unit: 2^-18 of the row's largest, for each key of a tile (256 at most) until
+# small for a term's normal range 2^-14.8 of a unit: 2^-18.3 of the row's largest, for each key of a tile (256 at most) until
 # the units have followed.  bf16: 2^-9 of P.
 SPLIT = 1.02 * (2.0 ** -8 + 2.0 ** -11)
 
