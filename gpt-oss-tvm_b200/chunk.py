@@ -26,16 +26,6 @@ HEAD_DIM = 64
 _BF16, _F8, _E8 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
-def _zeroed(device) -> torch.Tensor:
-    """A workspace's memory; what has to be zero before its first use (counters
-    and the error word) is."""
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        buf = torch.empty(int(lib.gptoss_attn_chunk_workspace_bytes()), dtype=torch.uint8, device=device)
-        buf[:int(lib.gptoss_attn_chunk_workspace_zero_bytes())].zero_()
-    return buf
-
-
 class ChunkWorkspace:
     """Device memory of attend_chunks for partial results, zeroed once; used
     by one stream at a time (one for all layers of a model).  Made before a
@@ -47,9 +37,16 @@ class ChunkWorkspace:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a ChunkWorkspace is made before a graph is captured (its zeros would be a node of "
                                    "the graph)")
-        self.buf = _zeroed(self.device)
-        self.nbytes = self.buf.numel()
+        self._allocate()
+
+    def _allocate(self):
+        lib = _lib.load()
+        with torch.cuda.device(self.device):
+            self.nbytes = int(lib.gptoss_attn_chunk_workspace_bytes())
+            self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=self.device)
+            self.buf[:int(lib.gptoss_attn_chunk_workspace_zero_bytes())].zero_()
         self.ptr = self.buf.data_ptr()
+        return self
 
     def error_word(self) -> torch.Tensor:
         """Device error bits so far, int32 [1] on the device."""
@@ -67,25 +64,26 @@ class ChunkWorkspace:
 _workspaces: dict = {}
 
 
-def _workspace(index: int) -> torch.Tensor:
+def _workspace(index: int) -> ChunkWorkspace:
     """The workspace of a call on device `index` that brings none: the current
     stream's, or, while that is being captured, memory of this call alone, zeroed
     in the graph.  (Streams that capture are shared: a workspace kept by stream
     would come to graphs that replay side by side, or before the one that holds
     its zeros.)"""
-    device = torch.device("cuda", index)
     if torch._C._cuda_getDevice() == index:
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = torch._C._cuda_isCurrentStreamCapturing()
     else:
         with torch.cuda.device(index):
-            capturing = torch.cuda.is_current_stream_capturing()
+            capturing = torch._C._cuda_isCurrentStreamCapturing()
     if capturing:
-        return _zeroed(device)
+        ws = ChunkWorkspace.__new__(ChunkWorkspace)
+        ws.device = torch.device("cuda", index)
+        return ws._allocate()
     stream = torch._C._cuda_getCurrentRawStream(index)
     ws = _workspaces.get((index, stream))
     if ws is None:
-        ws = _workspaces[index, stream] = ChunkWorkspace(device)
-    return ws.buf
+        ws = _workspaces[index, stream] = ChunkWorkspace(torch.device("cuda", index))
+    return ws
 
 
 def _run(index: int, name: str, *args) -> None:
@@ -192,14 +190,16 @@ def attend_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         _bad("out must be a dense bfloat16 tensor of q's shape on its device")
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if T and n:
-        ws = _workspace(index) if workspace is None else workspace.buf
-        if ws.get_device() != index:
+        ws = workspace
+        if ws is None:
+            ws = _workspace(index)
+        elif ws.buf.get_device() != index:
             _bad("the workspace is on another device")
         _run(index, "gptoss_attn_chunk", q.data_ptr(), st[0] if T > 1 else Hq * HEAD_DIM, k_pages.data_ptr(),
              v_pages.data_ptr(), k_scale.data_ptr() if f8 else None, v_scale.data_ptr() if f8 else None, f8, pages,
              table_p, page_table.shape[0], page_table.shape[1], rows_p, start_p, len_p, n, T, max_q, Hq, hkv,
              HEAD_DIM, window, HEAD_DIM ** -0.5 if sm_scale is None else sm_scale,
-             sinks.data_ptr() if sinks is not None else None, ws.data_ptr(), ws.numel(), out.data_ptr(),
+             sinks.data_ptr() if sinks is not None else None, ws.ptr, ws.nbytes, out.data_ptr(),
              lse.data_ptr() if return_lse else None)
     return (out, lse) if return_lse else out
 
