@@ -8,7 +8,7 @@
 //   l_i  = sum_j 2^(s2_ij - m_i),  lse_i = m_i + log2(l_i),  s2 = s * log2(e);
 //   a token that sees nothing gets o = 0 and lse = -inf.
 //
-// chunk_keys_kernel   up to 64 rows (tokens x heads of a kv head) against a
+// chunk_keys_kernel   up to 48 rows (tokens x heads of a kv head) against a
 //                     line of keys: S^T = K Q^T and O^T = V^T P^T on tcgen05
 //                     with the keys on the 128-row side
 // chunk_rows_kernel   longer chunks: 256 rows against the keys, S = Q K^T and
@@ -280,9 +280,9 @@ __device__ __forceinline__ void chunk_join(const ChunkParams& p, const ChunkSeg&
 // tokens on up to 8191 keys: 109 us without the way down, 114 with it, 120 where
 // every tile is looked at; units that begin at 2^3: 117, at 2^5: 120.)
 //
-// Measured, 32 sequences of 8192 keys, 8 kv heads: one token 91 us in bf16 (5.9
-// TB/s, the bytes bound it), 68 us in 8 bits (4.0 TB/s: a tile's chain of barrier
-// waits, products and softmax, not the bytes, bounds it); five tokens 118 and 136
+// Measured, 32 sequences of 8192 keys, 8 kv heads: one token 90 us in bf16 (6.0
+// TB/s, the bytes bound it), 71 us in 8 bits (3.9 TB/s: a tile's chain of barrier
+// waits, products and softmax, not the bytes, bounds it); five tokens 118 and 144
 // us (the softmax: 5 times the exponentials and, in 8 bits, P as two terms).
 template <bool F8, int N_>
 struct KeysCfg {
@@ -1676,30 +1676,31 @@ int launch_attn_chunk(ChunkParams p, const void* k, const void* v, int32_t f8, i
   p.counters = (uint32_t*)((uint8_t*)workspace + 256);
   p.part_o = (float*)((uint8_t*)workspace + chunk_parts_at());
   const int64_t rows = (int64_t)max_q * p.G;
-  // Rows of the longest chunk: up to 64 on the short side of the keys kernel, the smallest tile that holds them (32
-  // sequences of 8192 8-bit keys, one token: 68 us with 16 rows, 80 with 32, 90 with 48, 109 with 64; five tokens: 136
-  // with 48, 171 with 64).  The rows kernel pads them to 128 but takes a key tile in less time and has cheaper ends, so
-  // it is ahead with few (sequence, kv head) units, whose tiles are few per SM, and in bf16 with 64 rows always.  Keys /
-  // rows kernel in us, 8 kv heads, sequences x tokens on keys:
-  //   bf16  64 rows     64x8 on 512 67 / 44, on 8192 301 / 300;  16x8 on 8192 100 / 84;  1x8 on 8192 68 / 29
-  //   bf16  17..48      4x4 on 2048 23 / 17, on 8192 32 / 30;  1x6 on 8192 54 / 29;  but 16x4 on 8192 61 / 81
-  //   bf16  9..16       1x2 on 512 15 / 13, on 8192 34 / 21;  but 4x2 on 8192 26 / 29
-  //   8 bit 64 rows     16x8 on 2048 53 / 46, on 8192 114 / 122;  1x8 on 8192 76 / 35;  but 64x8 on 8192 363 / 446
-  //   8 bit 17..48      1x4 on 512 17 / 19, on 8192 42 / 27;  1x6 on 8192 59 / 36;  but 4x4 on 8192 33 / 41
-  // and with up to 8 rows the keys kernel, 4x1 on 8192: 20 / 29, 8 bit 19 / 38.  The keys a token can reach count the
-  // same way (`span`, from the window and the table): bf16 33..48 rows, 64x6 on 512 49 / 43, on 2048 88 / 90; 16x6 on
-  // 2048 38 / 33.
+  // Rows of the longest chunk: up to 48 on the short side of the keys kernel, the smallest tile that holds them (32
+  // sequences of 8192 8-bit keys, one token: 71 us with 16 rows, 84 with 32, 90 with 48; four tokens: 118 with 32, 131
+  // with 48).  The rows kernel pads them to 128 but takes a key tile in less time and has cheaper ends, so it is ahead
+  // from 64 rows on, and with few (sequence, kv head) units, whose tiles are few per SM.  Keys / rows kernel in us, 8 kv
+  // heads, sequences x tokens on keys:
+  //   bf16  64 rows     64x8 on 512 67 / 43, on 8192 296 / 298;  16x8 on 8192 98 / 87;  1x8 on 8192 67 / 30
+  //   bf16  17..48      4x4 on 2048 23 / 18, on 8192 34 / 32;  1x6 on 8192 58 / 29;  but 16x4 on 8192 61 / 82
+  //   bf16  9..16       1x2 on 512 15 / 13, on 8192 37 / 21;  but 4x2 on 8192 29 / 31
+  //   8 bit 64 rows     16x8 on 8192 157 / 122;  1x8 on 8192 74 / 33;  64x8 on 2048 182 / 133, on 8192 498 / 445
+  //   8 bit 33..48      1x6 on 8192 59 / 33;  4x6 on 2048 29 / 24, on 8192 44 / 43;  but 5x6 on 8192 46 / 49, 32x6 154 / 228
+  //   8 bit 17..32      1x4 on 512 17 / 16, on 8192 42 / 25;  2x4 on 8192 30 / 29;  but 3x4 on 8192 32 / 34
+  //   8 bit 9..16       1x2 on 512 15 / 16, on 8192 24 / 25;  4x2 on 8192 23 / 39
+  // and with up to 8 rows the keys kernel, 4x1 on 8192: 24 / 30, 8 bit 21 / 39; 1x1 on 512: 11.8 / 12.1, 8 bit 13 / 15, on
+  // 32768 31 / 34, 28 / 42 (but on 8192 23 / 21, 22 / 24).  The keys a token can reach count the same way (`span`, from the
+  // window and the table): bf16 33..48 rows, 64x6 on 512 53 / 42, on 2048 89 / 91; 16x6 on 2048 40 / 35.
   const int64_t units = (int64_t)p.N * p.Hkv, sms = device_sm_count();
   const int64_t pages = (int64_t)p.tstride * kChunkPage, span = p.window > 0 ? min64((int64_t)p.window + max_q, pages) : pages;
   const bool few = rows <= 8    ? false
                    : rows <= 16 ? !f8 && 16 * units <= sms
-                   : rows <= 48 ? (f8 ? 16 : 4) * units <= sms || (!f8 && rows > 32 && span <= 2048)
-                                : !f8 || units <= sms;
+                   : rows <= 48 ? (f8 && rows <= 32 ? 8 : 4) * units <= sms || (!f8 && rows > 32 && span <= 2048)
+                                : true;
   if (!few) {
     if (rows <= 16 && p.G <= 16) return f8 ? launch_keys<true, 16>(k, v, p, s) : launch_keys<false, 16>(k, v, p, s);
     if (rows <= 32 && p.G <= 32) return f8 ? launch_keys<true, 32>(k, v, p, s) : launch_keys<false, 32>(k, v, p, s);
     if (rows <= 48 && p.G <= 48) return f8 ? launch_keys<true, 48>(k, v, p, s) : launch_keys<false, 48>(k, v, p, s);
-    if (rows <= 64 && f8) return launch_keys<true, 64>(k, v, p, s);
   }
   return f8 ? launch_rows<true>(k, v, p, s) : launch_rows<false>(k, v, p, s);
 }
