@@ -576,9 +576,11 @@ class AttentionBlock:
             else:
                 _lib.call("gptoss_qkv_rope_append", _ptr(qkv), _ptr(pos), _ptr(kv_cache.slots_for(L)), T, Hq, Hkv, D,
                           self._inv_freq, ctypes.c_float(self._conc), _ptr(q), _ptr(kc), _ptr(vc), S)
-            chunk.attend_chunks(q, kc, vc, table, seq_rows, q_start, kv_cache.kv_len, max_q=max_q,
-                                window=self.sliding_window, sm_scale=self.sm_scale, sinks=self.sinks, k_scale=ks,
-                                v_scale=vs, out=o, workspace=self.scratch.chunk())
+            for n0 in range(0, len(seq_ids), chunk.MAX_CHUNKS):
+                n1 = min(n0 + chunk.MAX_CHUNKS, len(seq_ids))
+                chunk.attend_chunks(q, kc, vc, table, seq_rows[n0:n1], q_start[n0:n1 + 1], kv_cache.kv_len[n0:n1],
+                                    max_q=max_q, window=self.sliding_window, sm_scale=self.sm_scale, sinks=self.sinks,
+                                    k_scale=ks, v_scale=vs, out=o, workspace=self.scratch.chunk())
         elif forward_to == "decode":
             if any(n != 1 for n in lens) or min(seq_ids) != 0 or list(seq_ids) != list(range(len(seq_ids))):
                 raise ValueError("decode takes one token for each of sequences 0..B-1")

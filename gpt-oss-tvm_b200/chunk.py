@@ -23,6 +23,7 @@ from . import _lib
 
 PAGE_SIZE = 16
 HEAD_DIM = 64
+MAX_CHUNKS = 1024  # of one attend_chunks call
 _BF16, _F8, _E8 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -161,7 +162,8 @@ def attend_chunks(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
     q: bf16, heads and values dense, any multiple of 8 elements between tokens
     (a slice of a wider projection will do).  q_start [N + 1], kv_len,
-    seq_rows [N]: int32 on the device.  max_q: the longest chunk.  sinks
+    seq_rows [N]: int32 on the device, N at most MAX_CHUNKS (a slice of more of
+    them leaves the other tokens' rows of out as they are).  max_q: the longest chunk.  sinks
     [heads] bf16.  workspace: a ChunkWorkspace of calls that run one after
     another; without one a call has its stream's, or in a captured graph its own
     (20 MB and a memset a call, so a graph of many calls brings one).  Returns o

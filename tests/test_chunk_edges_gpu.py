@@ -231,3 +231,35 @@ def test_a_window_beyond_every_key_is_none(ql, kl, window, f8):
     o, lse = c.run()
     o2, lse2 = c.run(window=window)
     assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("kv_dtype", ["float8_e4m3", "bfloat16"])
+def test_more_sequences_than_one_call_takes(kv_dtype):
+    """A layer over 1030 sequences: a decode step (8 bit) and a chunk each, against
+    the same layer over the first and the last of them alone."""
+    att, cfgm = (importlib.import_module("gpt-oss-tvm_b200." + n) for n in ("attention", "config"))
+    cfg = cfgm.GPTOssConfig(num_hidden_layers=2, num_experts=16, vocab_size=64, context_window_size=1024)
+    n, g = chunk.MAX_CHUNKS + 6, torch.Generator(device="cuda").manual_seed(1)
+    block = att.AttentionBlock(cfg, layer_idx=1)
+    for w in (block.qkv_weight, block.out_weight):
+        w.copy_(torch.randn(w.shape, generator=g, device="cuda") * 0.02)
+    x = [torch.randn(1, n, cfg.hidden_size, generator=g, device="cuda").bfloat16().cpu() for _ in range(2)]
+    picked = [0, 1, chunk.MAX_CHUNKS - 1, chunk.MAX_CHUNKS, n - 1]
+
+    def steps(rows):
+        c = att.KVCache(cfg, len(rows), 32, 2, kv_dtype=kv_dtype, max_chunk=2)
+        out = []
+        for i, t in enumerate(x):
+            ids = list(range(len(rows)))
+            if i and c.f8:
+                pos, mode = c.begin_forward(ids, [1] * len(rows)), "decode"
+            else:
+                pos, mode = c.begin_chunks(ids, [1] * len(rows)), "chunk"
+            y = block.forward(t[:, rows].cuda(), c, pos, mode)[0]
+            out.append(y.float().cpu().reshape(len(rows), cfg.hidden_size))
+        return out
+
+    tol = 2e-2  # bf16 attention and projections, as in the tests of the layers
+    for many, few in zip(steps(list(range(n))), steps(picked)):
+        assert many.shape == (n, cfg.hidden_size)
+        assert float((many[picked] - few).abs().max()) <= tol * float(few.abs().max())
