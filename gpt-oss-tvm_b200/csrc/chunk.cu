@@ -307,7 +307,7 @@ struct KeysCfg {
   static constexpr int kOffQ = kOffP + 2 * kP;
   static constexpr int kOffCodes = kOffQ + 2 * kQ;
   static constexpr int kOffRed = kOffCodes + kStages * kCodes;  // per stream: [kSums][N] maxima or sums
-  static constexpr int kOffRef = kOffRed + 2 * kSums * N * 4;   // per stream: -m [N], factor [N], 8 bit: -(highest m) [N]
+  static constexpr int kOffRef = kOffRed + 2 * kSums * N * 4;   // per stream: -m, factor, 8 bit: -(highest m); [N] each
   static constexpr int kOffLow = kOffRef + 2 * 3 * N * 4;       // 8 bit, per stream: each warp's rows below 1
   static constexpr int kOffPre = kOffLow + 2 * 8 * 4;
   static constexpr int kOffSeg = kOffPre + (kChunkMaxSeqs + 1 + 15) / 16 * 64;
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
     uint32_t* low = (uint32_t*)(smem + C::kOffLow) + s * 8;
     uint8_t* qs = smem + C::kOffQ + s * C::kQ;
     uint8_t* ps = smem + C::kOffP + s * C::kP;
-    constexpr float kUp = F8 ? 8.75f : 8.0f;                // P at most 2^kUp (8 bit: 28 times what e4m3 leaves of 448 is 448)
+    constexpr float kUp = F8 ? 8.75f : 8.0f;   // P at most 2^kUp (8 bit: 28 times what e4m3 leaves of 448 is 448)
     constexpr float kBase = F8 ? 3.5f : 0.0f;  // log2 P of the largest when the reference moves
     constexpr float kDepth = 40.0f;
     constexpr float kNoRef = 3.402823466e38f;
@@ -967,7 +967,8 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
 // power of two (exact) while those before are used: 60 instructions for 32 x 16
 // values; the rest of the kernel is the same.  1872 us for the same call: a key
 // tile's conversion is a third of the instructions that its softmax is.  (One
-// converting warpgroup: 3121.)
+// converting warpgroup: 3121.)  Its 28 warps leave 72 registers a thread (88 for
+// the softmax): 222 bytes of one are spilled, 12 in bf16.
 constexpr int kRowsKT = 128;
 // Bits 0 .. n set (none for n < 0).
 __device__ __forceinline__ uint32_t ch_bits_to(int32_t n) { return n < 0 ? 0u : n >= 31 ? ~0u : (2u << n) - 1u; }

@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(256, kKv8Blocks)
 // Rows pos0 .. pos0 + n - 1 of one sequence: 4 lanes per (row, head), K and V
 // by the same lanes (two loads in flight); 16 values per lane, 16 bytes on the
 // 8-bit side and 32 on the bf16 side.  Bound by the bytes: 131072 rows of 8 heads
-// read back in 70 us, 5.8 TB/s.
+// read back in 70 us, 5.8 TB/s, written in 71 (8192 rows in 5.9, from L2; one row
+// and 1000 rows in 2.7 and 2.9, a launch).
 template <bool kToPages>
 __global__ void __launch_bounds__(256)
     kv_pages_f8_kernel(uint8_t* __restrict__ kp, uint8_t* __restrict__ vp, uint8_t* __restrict__ kcode,

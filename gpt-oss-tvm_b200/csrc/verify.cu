@@ -32,7 +32,8 @@
 //                       residual needs the whole row again: then a cluster per
 //                       sequence sums its pieces first (48 sequences: 37 us,
 //                       51 instructions a value, an IEEE division among them;
-//                       49 us where four CTAs fit an SM instead of five)
+//                       49 us where four CTAs fit an SM instead of five, for
+//                       which 56 bytes of a thread go to local memory)
 #include "common.cuh"
 #include "launch.h"
 

@@ -35,8 +35,9 @@ def prompt_lookup(tokens: list[int], n: int, ngram: int = 3) -> list[int]:
 class SpeculativeDecoder:
     """Decodes a batch of sequences of ``engine`` (created with max_chunk of at
     least draft_len + 1).  draft: (tokens so far, n) -> up to n drafts, without
-    a distribution of their own.  The random numbers come from one seeded
-    generator, so a run can be repeated."""
+    a distribution of their own.  Tokens are drawn from softmax(logits /
+    temperature), without the top-p cut of ``Engine.sample``.  The random numbers
+    come from one seeded generator, so a run can be repeated."""
 
     def __init__(self, engine: Engine, draft_len: int = 4, draft=prompt_lookup, temperature: float = 0.0,
                  seed: int = 0):

@@ -29,7 +29,9 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, row_start: torch.T
     drafts that were looked up, q = 1).  Returns int32 tensors on the device:
     accepted [N], the drafts before the first that is not, and next_token [N],
     drawn with next_draws [N] from what is left of p there, or from the last
-    row's p.  temperature < 1e-6: greedy, no draws needed."""
+    row's p.  temperature < 1e-6: greedy, no draws needed.  (Both are views of
+    one buffer that held the scratch, 8 bytes for each 256 logits: what is kept
+    for long is cloned.)"""
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
         _bad("logits must be a CUDA tensor [rows, vocabulary], float32 or bfloat16")
     index = logits.get_device()
