@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(KeysCfg<F8, N_>::kThreads, 1)
     uint8_t* ps = smem + C::kOffP + s * C::kP;
     constexpr float kUp = F8 ? 8.75f : 8.0f;   // P at most 2^kUp (8 bit: 28 times what e4m3 leaves of 448 is 448)
     constexpr float kBase = F8 ? 3.5f : 0.0f;  // log2 P of the largest when the reference moves
-    constexpr float kDepth = 40.0f;
+    constexpr float kDepth = 32.0f;            // (a V row of zeros counts up to 2^60 in l: 2^26 of them fit fp32 yet)
     constexpr float kNoRef = 3.402823466e38f;
     for (int sn = 0;; ++sn) {
       const int sb = sn & 1;

@@ -263,3 +263,25 @@ def test_more_sequences_than_one_call_takes(kv_dtype):
     for many, few in zip(steps(list(range(n))), steps(picked)):
         assert many.shape == (n, cfg.hidden_size)
         assert float((many[picked] - few).abs().max()) <= tol * float(few.abs().max())
+
+
+@pytest.mark.parametrize("nats", [5.0, 70.0, 140.0])
+@pytest.mark.parametrize("q", [1, 4, 6])
+def test_values_of_zero_on_top(q, nats):
+    """8 bits: rows of zeros have the smallest power of two, which P takes in and
+    the sum takes out again, 2^60 of it: keys with such rows far above all others,
+    before and between them."""
+    length = 4000
+    k, v = torch.zeros(length, 8, D), torch.ones(length, 8, D)
+    top = torch.zeros(length, dtype=torch.bool)
+    top[:300], top[2000:2010] = True, True
+    k[top], v[top] = nats / 8.0, 0.0
+    c = one_context(24, q, k.bfloat16(), v.bfloat16(), True)
+    c.q = torch.ones_like(c.q)
+    nats = 8 * float(dequantise(c.k, c.ks)[0, 0, 0])  # as the pages hold the key
+    o, lse = c.gpu().run()
+    for i in range(q):
+        m = length - q + i + 1 - 310
+        den = 310 * math.exp(nats) + m
+        assert (o[i::q].double() - m / den).abs().max().item() <= (SPLIT + 2.0 ** -9) * m / den + 1e-6
+        assert (lse[i::q].double() - math.log2(den)).abs().max().item() <= 5e-4
